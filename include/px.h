@@ -280,6 +280,80 @@ PX_API px_status px_pq_search_filtered(const px_pq* h, const float* queries, int
                                        int32_t k, const uint8_t* mask, int64_t* out_ids,
                                        float* out_dists);
 
+/* ------------------------------------------------------------------------
+ * Embedding rows: operators on arrays of rows in device memory, for programs
+ * that train, cut down or score the embeddings an index serves. No
+ * counterpart in the reference. Every pointer is device memory of `device`;
+ * arrays are row-major with a row stride in elements; the calls run on
+ * `stream` (NULL: the default stream), return without waiting, allocate
+ * nothing and keep nothing, so they can be captured into CUDA graphs. Rows
+ * and columns past the given sizes are neither read nor written.
+ * ------------------------------------------------------------------------ */
+enum { PX_F32 = 0, PX_F16 = 1, PX_BF16 = 2 };
+
+/* 8-bit rows: scales[i] = max_j |x_ij| / 127 and codes[i][j] = x_ij /
+ * scales[i] rounded to nearest (ties to even, exactly rounded quotients). A
+ * row of zeros has scale 0 and codes 0; a row holding a NaN or an infinity
+ * has scale NaN and codes 0. x is n x dim of `type`. */
+PX_API px_status px_quantize_rows_device(int32_t device, const void* x, int32_t type, int64_t n, int32_t dim,
+                                         int64_t ldx, int8_t* codes, int64_t ldc, float* scales, void* stream);
+/* out[i][j] = codes[i][j] * scales[i], n x dim of `type`. */
+PX_API px_status px_dequantize_rows_device(int32_t device, const int8_t* codes, int64_t ldc, const float* scales,
+                                           int64_t n, int32_t dim, int32_t type, void* out, int64_t ldo,
+                                           void* stream);
+
+/* The whole score matrix of m 8-bit queries and n 8-bit base rows:
+ * out[i][j] = (sum_l q[i][l] * x[j][l]) * q_scales[i] * x_scales[j] + bias[j]
+ * (bias may be NULL), m x n of `type`. The sums are exact in 32-bit integers
+ * (dim <= 131071). With bias[j] = -|x_j|^2 / 2 the descending order of a row
+ * of `out` is the ascending order of L2 distance. Code rows start on 16-byte
+ * boundaries (q, x 16-byte aligned; ldq, ldx multiples of 16). */
+PX_API px_status px_int8_scores_device(int32_t device, const int8_t* q, int64_t ldq, const float* q_scales, int64_t m,
+                                       const int8_t* x, int64_t ldx, const float* x_scales, int64_t n, int32_t dim,
+                                       const float* bias, int32_t type, void* out, int64_t ldo, void* stream);
+
+/* Softmax cross entropy of t queries over v base rows, without keeping the
+ * t x v logits z_ij = scale * queries_i . rows_j + bias_j:
+ *   loss[i] = log sum_j exp z_ij - z_i,targets[i],  lse[i] = log sum_j exp z_ij
+ * queries (t x dim) and rows (v x dim) are PX_F16 or PX_BF16 with rows on
+ * 16-byte boundaries; targets are row numbers; bias (v floats, 16-byte
+ * aligned) may be NULL, and -infinity in it leaves a row out of the softmax.
+ * A query whose target is ignore_index has loss 0 (its lse is still written);
+ * one whose target is any other number outside [0, v) has loss NaN; one whose
+ * target is left out, +infinity. total (2 floats) receives, for PX_REDUCE_SUM
+ * and PX_REDUCE_MEAN, the reduced loss and what it was divided by (1, or the
+ * number of queries not ignored; a mean over none is NaN). workspace: 16-byte
+ * aligned, px_softmax_xent_workspace_bytes(..., backward = 0) bytes, free
+ * once the call's work is done. */
+enum { PX_REDUCE_NONE = 0, PX_REDUCE_SUM = 1, PX_REDUCE_MEAN = 2 };
+PX_API int64_t px_softmax_xent_workspace_bytes(int32_t device, int64_t t, int64_t v, int32_t dim, int32_t backward);
+PX_API px_status px_softmax_xent_device(int32_t device, const void* queries, int64_t ldq, int64_t t, const void* rows,
+                                        int64_t ldr, int64_t v, int32_t dim, int32_t type, const int64_t* targets,
+                                        int64_t ignore_index, float scale, const float* bias, int32_t reduction,
+                                        float* loss, float* lse, float* total, float* divisor, void* workspace,
+                                        int64_t workspace_bytes, void* stream);
+/* Its gradient: with G_ij = g_i * (exp(z_ij - lse_i) - [j == targets_i]),
+ *   grad_queries = scale * G rows,  grad_rows = scale * G^T queries,
+ * of the operands' type (either may be NULL: not computed). g_i = grad[i *
+ * grad_stride] / divisor[0] (divisor may be NULL: 1), so a reduced loss passes
+ * its one gradient with stride 0 and the forward's divisor. loss and lse are the
+ * forward's. Queries that are ignored, or whose target is no row, add nothing
+ * (but queries and rows are multiplied with a weight of zero, so they must be
+ * finite). G takes the operands' 16 bits, in pieces of the base of at most
+ * 64 MB or 1024 columns. Results do not change from run to run. */
+PX_API px_status px_softmax_xent_backward_device(int32_t device, const void* queries, int64_t ldq, int64_t t,
+                                                 const void* rows, int64_t ldr, int64_t v, int32_t dim, int32_t type,
+                                                 const int64_t* targets, int64_t ignore_index, float scale,
+                                                 const float* bias, const float* loss, const float* lse,
+                                                 const float* grad, int32_t grad_stride, const float* divisor,
+                                                 void* grad_queries, int64_t ldgq, void* grad_rows, int64_t ldgr,
+                                                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Waits for `stream` and returns PX_ETIMEOUT if a bounded device-side wait of
+ * a row operator on `device` has given up since the last call (what it left
+ * undone is NaN in its outputs). */
+PX_API px_status px_rows_status_device(int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,6 +99,17 @@ SIGNATURES = {
     "px_pq_search": (_i32, [_vp, _f32p, _i64, _i32, _i64p, _f32p]),
     "px_pq_search_device": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp]),
     "px_pq_search_filtered": (_i32, [_vp, _f32p, _i64, _i32, _u8p, _i64p, _f32p]),
+    "px_quantize_rows_device": (_i32, [_i32, _vp, _i32, _i64, _i32, _i64, _vp, _i64, _vp, _vp]),
+    "px_dequantize_rows_device": (_i32, [_i32, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _i64, _vp]),
+    "px_int8_scores_device": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _i64,
+                                     _vp]),
+    "px_softmax_xent_workspace_bytes": (_i64, [_i32, _i64, _i64, _i32, _i32]),
+    "px_softmax_xent_device": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _c.c_float, _vp,
+                                      _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "px_softmax_xent_backward_device": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64,
+                                               _c.c_float, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp, _i64, _vp,
+                                               _i64, _vp]),
+    "px_rows_status_device": (_i32, [_i32, _vp]),
 }
 
 _lib = None

@@ -36,6 +36,7 @@
 
 #include "px_common.cuh"
 #include "px_kernels.h"
+#include "px_rows.h"
 #include "px_tc.cuh"
 
 namespace px {
@@ -900,6 +901,26 @@ cudaError_t encode_bf16_map(CUtensorMap* map, const void* plane, int64_t rows, i
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(plane), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// A row-major array of `rows` rows of `cols` values, `pitch` bytes apart, as a
+// TMA tensor with 128-byte swizzle and boxes of box_cols (128 bytes of them)
+// by box_rows. Values past the last column or row read as zeros.
+cudaError_t encode_rows_map(CUtensorMap* map, ElemType type, const void* base, int64_t cols, int64_t rows,
+                            int64_t pitch, int box_cols, int box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = get_encode_fn();
+  if (!fn) return cudaErrorNotSupported;
+  const CUtensorMapDataType dt = type == kElemS8    ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : type == kElemF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }

@@ -1,0 +1,278 @@
+// 8-bit rows: each embedding row as signed 8-bit codes and one fp32 scale,
+//     scale = max_j |x_j| / 127        (fp32 division)
+//     code_j = x_j / scale, rounded to nearest, ties to even
+// and back (code * scale). The codes are the exactly rounded quotients: a
+// product with the reciprocal gives a candidate, and its remainder
+// x - code * scale, which one fma computes without rounding, says whether a
+// neighbour is nearer. So the codes do not depend on how the division is
+// carried out, at the cost of an fma and a compare per value instead of a
+// division.
+//
+// A row of zeros (or one so small that its scale underflows to 0) has scale 0
+// and codes 0. A row that holds a NaN or an infinity has scale NaN and codes
+// 0, so every score of it is NaN.
+//
+// Both kernels move bytes and little else, so the layout is chosen for wide
+// coalesced accesses: a group of 4 to 32 lanes takes a row, the widest vector
+// that the row's address and pitch allow at a time (16 bytes where rows start
+// on 16-byte boundaries), the row staying in registers between the maximum
+// and the codes, so x is read once. Groups are as small as leaves a lane at
+// most four vectors: several short rows share a warp's load instruction.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "px_rows.h"
+
+namespace px {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <int BYTES> struct Word;
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<2> { using type = uint16_t; };
+template <> struct Word<1> { using type = uint8_t; };
+
+// A row's scale, and what its values are multiplied by before the division:
+// 2^96 for rows so small that 1 / scale would overflow (a power of two, so
+// nothing is rounded), else 1.
+struct RowScale {
+  float scale, lift, lifted, inverse;
+  __device__ __forceinline__ explicit RowScale(uint32_t peak_bits) {
+    if (peak_bits >= 0x7f800000u) {  // NaN or infinity in the row
+      scale = __int_as_float(0x7fc00000);
+      lift = lifted = inverse = 0.0f;
+      return;
+    }
+    scale = __fdiv_rn(__uint_as_float(peak_bits), 127.0f);
+    lift = scale < 1e-30f ? 0x1p96f : 1.0f;
+    lifted = scale * lift;
+    inverse = lifted > 0.0f ? __frcp_rn(lifted) : 0.0f;
+  }
+  __device__ __forceinline__ int code(float x) const {
+    if (inverse == 0.0f) return 0;
+    const float xs = x * lift;
+    float c = rintf(xs * inverse);
+    // |rest| <= scale * (1/2 + a few ulps): exact.
+    const float rest = fmaf(-c, lifted, xs);
+    const float twice = 2.0f * fabsf(rest);
+    if (twice > lifted || (twice == lifted && (__float2int_rn(c) & 1))) c += copysignf(1.0f, rest);
+    return __float2int_rn(fminf(fmaxf(c, -127.0f), 127.0f));
+  }
+};
+
+// VB: bytes per load; NV: loads per lane. A row's values stay in registers, at
+// most 32 per lane.
+template <typename T, int VB, int NV>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, int64_t ldx,
+                                                                 int8_t* __restrict__ codes, int64_t ldc,
+                                                                 float* __restrict__ scales, int group, bool vec_out) {
+  constexpr int VE = VB / static_cast<int>(sizeof(T));
+  using W = typename Word<VB>::type;
+  const int lane = threadIdx.x & (group - 1);
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
+  const bool live = row < n;  // a dead group still takes part in the shuffles
+  const T* xr = x + (live ? row : 0) * ldx;
+  const int nvec = (d + VE - 1) / VE;
+  float v[NV][VE];
+  uint32_t peak = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (i * group + lane) * VE;
+    if (live && at + VE <= d) {
+      const W w = __ldg(reinterpret_cast<const W*>(xr + at));
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) v[i][j] = to_f32(e[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) v[i][j] = live && at + j < d ? to_f32(__ldg(xr + at + j)) : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) peak = max(peak, __float_as_uint(v[i][j]) & 0x7fffffffu);
+  for (int s = group >> 1; s > 0; s >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, s));
+  if (!live) return;
+  const RowScale r(peak);
+  if (lane == 0) scales[row] = r.scale;
+  int8_t* out = codes + row * ldc;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int vec = i * group + lane;
+    if (vec >= nvec) break;
+    const int at = vec * VE;
+    using C = typename Word<VE>::type;
+    if (vec_out && at + VE <= d) {
+      C w;
+      int8_t* e = reinterpret_cast<int8_t*>(&w);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) e[j] = static_cast<int8_t>(r.code(v[i][j]));
+      *reinterpret_cast<C*>(out + at) = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < VE; ++j)
+        if (at + j < d) out[at + j] = static_cast<int8_t>(r.code(v[i][j]));
+    }
+  }
+}
+
+// Rows longer than a group's registers hold: a block per row, which reads the
+// row twice (the second time from cache).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* __restrict__ x, int64_t n, int d,
+                                                                      int64_t ldx, int8_t* __restrict__ codes,
+                                                                      int64_t ldc, float* __restrict__ scales) {
+  __shared__ uint32_t s_peak[kThreads / 32];
+  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+    const T* xr = x + row * ldx;
+    uint32_t peak = 0;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < d; j += kThreads) peak = max(peak, __float_as_uint(to_f32(__ldg(xr + j))) & 0x7fffffffu);
+    peak = __reduce_max_sync(0xffffffffu, peak);
+    if ((threadIdx.x & 31) == 0) s_peak[threadIdx.x >> 5] = peak;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) peak = max(peak, s_peak[w]);
+    __syncthreads();
+    const RowScale r(peak);
+    if (threadIdx.x == 0) scales[row] = r.scale;
+    int8_t* out = codes + row * ldc;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < d; j += kThreads) out[j] = static_cast<int8_t>(r.code(to_f32(__ldg(xr + j))));
+  }
+}
+
+// VE codes at a time; a group of lanes takes a row, as above.
+template <typename T, int VE>
+__global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const int8_t* __restrict__ codes, int64_t ldc,
+                                                                   const float* __restrict__ scales, int64_t n, int d,
+                                                                   T* __restrict__ out, int64_t ldo, int group) {
+  using C = typename Word<VE>::type;
+  using W = typename Word<VE * static_cast<int>(sizeof(T))>::type;
+  const int lane = threadIdx.x & (group - 1);
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
+  if (row >= n) return;
+  const float s = __ldg(scales + row);
+  const int8_t* c = codes + row * ldc;
+  T* o = out + row * ldo;
+#pragma unroll 4
+  for (int at = lane * VE; at < d; at += group * VE) {
+    if (at + VE <= d) {
+      const C w = __ldg(reinterpret_cast<const C*>(c + at));
+      const int8_t* e = reinterpret_cast<const int8_t*>(&w);
+      W r;
+      T* p = reinterpret_cast<T*>(&r);
+#pragma unroll
+      for (int j = 0; j < VE; ++j) p[j] = from_f32<T>(static_cast<float>(e[j]) * s);
+      *reinterpret_cast<W*>(o + at) = r;
+    } else {
+      for (int j = at; j < d; ++j) o[j] = from_f32<T>(static_cast<float>(__ldg(c + j)) * s);
+    }
+  }
+}
+
+// Lanes per row: the fewest (4 to 32) that leave a lane at most `most` vectors.
+int group_for(int64_t vectors, int most) {
+  int g = 4;
+  while (g < 32 && g * most < vectors) g *= 2;
+  return g;
+}
+
+bool aligned(const void* p, int64_t pitch, int bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && pitch % bytes == 0;
+}
+
+template <typename T, int VB>
+cudaError_t quantize_vec(const T* x, int64_t n, int d, int64_t ldx, int8_t* codes, int64_t ldc, float* scales,
+                         cudaStream_t stream) {
+  constexpr int VE = VB / static_cast<int>(sizeof(T));
+  constexpr int kMost = 32 / VE;  // vectors a lane's registers hold
+  const int64_t nvec = (d + VE - 1) / VE;
+  if (nvec > 32 * kMost) {
+    const int64_t grid = n < 65536 ? n : 65536;
+    quantize_long_rows_kernel<T><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(x, n, d, ldx, codes, ldc, scales);
+    return cudaGetLastError();
+  }
+  const int group = group_for(nvec, 4);
+  const int64_t blocks = (n * group + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  auto kern = nvec <= 4 * group ? quantize_rows_kernel<T, VB, 4> : quantize_rows_kernel<T, VB, kMost>;
+  kern<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(x, n, d, ldx, codes, ldc, scales, group,
+                                                               aligned(codes, ldc, VE));
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t quantize_typed(const T* x, int64_t n, int d, int64_t ldx, int8_t* codes, int64_t ldc, float* scales,
+                           cudaStream_t stream) {
+  const int64_t pitch = ldx * static_cast<int64_t>(sizeof(T));
+  if (aligned(x, pitch, 16)) return quantize_vec<T, 16>(x, n, d, ldx, codes, ldc, scales, stream);
+  if (aligned(x, pitch, 8)) return quantize_vec<T, 8>(x, n, d, ldx, codes, ldc, scales, stream);
+  if (aligned(x, pitch, 4)) return quantize_vec<T, 4>(x, n, d, ldx, codes, ldc, scales, stream);
+  return quantize_vec<T, static_cast<int>(sizeof(T))>(x, n, d, ldx, codes, ldc, scales, stream);
+}
+
+template <typename T, int VE>
+cudaError_t dequantize_vec(const int8_t* codes, int64_t ldc, const float* scales, int64_t n, int d, T* out, int64_t ldo,
+                           cudaStream_t stream) {
+  const int group = group_for((d + VE - 1) / VE, 4);
+  const int64_t blocks = (n * group + kThreads - 1) / kThreads;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  dequantize_rows_kernel<T, VE><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(codes, ldc, scales, n, d, out,
+                                                                                        ldo, group);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t dequantize_typed(const int8_t* codes, int64_t ldc, const float* scales, int64_t n, int d, T* out,
+                             int64_t ldo, cudaStream_t stream) {
+  constexpr int VE = 16 / static_cast<int>(sizeof(T));
+  const int64_t pitch = ldo * static_cast<int64_t>(sizeof(T));
+  if (aligned(codes, ldc, VE) && aligned(out, pitch, 16))
+    return dequantize_vec<T, VE>(codes, ldc, scales, n, d, out, ldo, stream);
+  if (aligned(codes, ldc, 2) && aligned(out, pitch, 2 * static_cast<int>(sizeof(T))))
+    return dequantize_vec<T, 2>(codes, ldc, scales, n, d, out, ldo, stream);
+  return dequantize_vec<T, 1>(codes, ldc, scales, n, d, out, ldo, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_rows(const void* x, ElemType type, int64_t n, int d, int64_t ldx, int8_t* codes,
+                                 int64_t ldc, float* scales, cudaStream_t stream) {
+  switch (type) {
+    case kElemF32: return quantize_typed(static_cast<const float*>(x), n, d, ldx, codes, ldc, scales, stream);
+    case kElemF16: return quantize_typed(static_cast<const __half*>(x), n, d, ldx, codes, ldc, scales, stream);
+    case kElemBf16: return quantize_typed(static_cast<const __nv_bfloat16*>(x), n, d, ldx, codes, ldc, scales, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_dequantize_rows(const int8_t* codes, int64_t ldc, const float* scales, int64_t n, int d,
+                                   ElemType type, void* out, int64_t ldo, cudaStream_t stream) {
+  switch (type) {
+    case kElemF32: return dequantize_typed(codes, ldc, scales, n, d, static_cast<float*>(out), ldo, stream);
+    case kElemF16: return dequantize_typed(codes, ldc, scales, n, d, static_cast<__half*>(out), ldo, stream);
+    case kElemBf16: return dequantize_typed(codes, ldc, scales, n, d, static_cast<__nv_bfloat16*>(out), ldo, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace px

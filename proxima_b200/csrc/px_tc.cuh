@@ -315,5 +315,47 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// The same with 8-bit signed integer operands and 32-bit integer sums
+// (kind::i8); K = 32 per instruction.
+__device__ __forceinline__ void mma_s8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: D s32, A/B s8 (kind::i8), both K-major, M x N.
+__host__ __device__ constexpr uint32_t idesc_s8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Instruction descriptor: D f32, A/B f16 or bf16 (kind::f16), each operand
+// K-major or MN-major (its tile holds, for every K, 64 consecutive M or N
+// values), M x N.
+__host__ __device__ constexpr uint32_t idesc_16(bool bf16, bool a_mn, bool b_mn, int m, int n) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Shared-memory matrix descriptor for an MN-major operand tile of 16-bit
+// values written by TMA with CU_TENSOR_MAP_SWIZZLE_128B in boxes of 64 M (or
+// N) values by 64 K rows: K rows are 128 bytes apart, groups of 8 K rows 1024
+// bytes (stride offset), and the next 64 M (or N) values lie one box, 8192
+// bytes, further (leading offset). Tiles are 1024-byte aligned; 16 K rows
+// move the start address by 2048 bytes.
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(8192 >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
 }  // namespace tc
 }  // namespace px
