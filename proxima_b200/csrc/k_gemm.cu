@@ -906,13 +906,15 @@ cudaError_t encode_bf16_map(CUtensorMap* map, const void* plane, int64_t rows, i
 }
 
 // A row-major array of `rows` rows of `cols` values, `pitch` bytes apart, as a
-// TMA tensor with 128-byte swizzle and boxes of box_cols (128 bytes of them)
-// by box_rows. Values past the last column or row read as zeros.
+// TMA tensor with boxes of box_cols (`swizzle` bytes of them: 64 or 128, and
+// that swizzle) by box_rows. Values past the last column or row read as zeros
+// and are not written.
 cudaError_t encode_rows_map(CUtensorMap* map, ElemType type, const void* base, int64_t cols, int64_t rows,
-                            int64_t pitch, int box_cols, int box_rows) {
+                            int64_t pitch, int box_cols, int box_rows, int swizzle) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = get_encode_fn();
   if (!fn) return cudaErrorNotSupported;
   const CUtensorMapDataType dt = type == kElemS8    ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : type == kElemF32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : type == kElemF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
@@ -920,8 +922,8 @@ cudaError_t encode_rows_map(CUtensorMap* map, ElemType type, const void* base, i
   cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 

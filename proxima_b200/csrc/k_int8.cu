@@ -22,17 +22,17 @@
 // than it must, and the clusters of different query groups read the same base
 // rows from L2.
 //
-// CTA roles (320 threads): warp 0 TMA producer, warp 1 TMEM owner and (even
-// CTA) MMA issuer, warps 2-9 epilogue: lanes by TMEM quarter, the two
-// warpgroups take alternate blocks of 32 queries. Two accumulators (512 TMEM
+// CTA roles (576 threads): warp 0 TMA producer, warp 1 TMEM owner and (even
+// CTA) MMA issuer, warps 2-17 epilogue: four per TMEM quarter, on alternate
+// blocks of 32 queries. Two accumulators (512 TMEM
 // columns) overlap the epilogue with the next tile. Barriers as in the bf16
 // candidate pass (k_gemm.cu); every wait is bounded, and a wait that gives up
 // makes the tiles it concerns NaN and raises the operators' error word.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "px_rows.cuh"
 #include "px_rows.h"
-#include "px_tc.cuh"
 
 namespace px {
 
@@ -45,9 +45,12 @@ constexpr int kRows = 128;        // base rows per CTA and tile
 constexpr int kSlice = 128;       // codes per slice
 constexpr int kA = kRows * kSlice;  // 16 KB
 constexpr int kMaxStages = 12;
-constexpr int kThreads = 64 + 256;
+constexpr int kGroups = 4;        // epilogue warps per TMEM quarter
+constexpr int kEpiWarps = 4 * kGroups;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kWarpScales = 256 / kGroups;  // query scales an epilogue warp needs
 constexpr int kBars = 2 * kMaxStages + 2 + 2 + 2 + 2;  // one spare: the scales after them stay 16-byte aligned
-constexpr size_t kFixed = 1024 + kBars * 8 + 16 + 8 * 128 * 4;
+constexpr size_t kFixed = 1024 + kBars * 8 + 16 + kEpiWarps * kWarpScales * 4;
 constexpr size_t kSmemLimit = 232448;  // 227 KB
 
 struct Params {
@@ -56,18 +59,13 @@ struct Params {
   const float* bias;
   void* out;
   int64_t ldo, m, n;
-  int64_t tiles;   // query groups x base tiles
+  int tiles;       // query groups x base tiles
   int base_tiles;
   int n_cols;      // queries per tile: a multiple of 32, at most 256
   int kc;          // slices
   int resident;    // queries stay in shared memory
   int stages, stage_bytes;
 };
-
-__device__ __forceinline__ void quiet_wait(uint32_t bar, uint32_t parity) {
-  int dummy = 0;
-  tc::mbar_wait(bar, parity, &dummy);
-}
 
 template <typename T>
 __device__ __forceinline__ T narrow(float x);
@@ -90,8 +88,74 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <>
-__device__ __forceinline__ uint32_t pack2<float>(float, float) { return 0; }  // not called
+// The scores of queries j and j + 1 and this lane's base row.
+__device__ __forceinline__ F2 two_scores(const uint32_t (&v)[32], int j, float w0, float w1, F2 xs, F2 bias) {
+  return fma2(f2(static_cast<float>(static_cast<int>(v[j])), static_cast<float>(static_cast<int>(v[j + 1]))),
+              mul2(f2(w0, w1), xs), bias);
+}
+
+// A pair's word of 16-bit scores: the even lane's both rows of query j, the
+// odd lane's of query j + 1.
+template <typename OT>
+__device__ __forceinline__ uint32_t trade(float s0, float s1, int odd) {
+  const uint32_t mine = pack2<OT>(s0, s1);
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+  return __byte_perm(mine, other, odd ? 0x3276 : 0x5410);
+}
+
+// Stores a block's scores, all 32 base rows of the warp being real. SOME: only
+// the first `count` queries are. The stores evict first: the matrix is larger
+// than what L2 should keep for the base.
+template <typename OT, bool PAIR, int SOME>
+__device__ __forceinline__ void store_queries(const uint32_t (&v)[32], const float* qs, float xs, float bias, OT* o,
+                                              int64_t ldo, int odd, int count) {
+  const float4* qs4 = reinterpret_cast<const float4*>(qs);
+  const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
+#pragma unroll
+  for (int j4 = 0; j4 < 8; ++j4) {
+    if (SOME && 4 * j4 >= count) break;
+    const float4 w = qs4[j4];
+    float s[4];
+    unpack(two_scores(v, 4 * j4, w.x, w.y, xs2, bias2), s[0], s[1]);
+    unpack(two_scores(v, 4 * j4 + 2, w.z, w.w, xs2, bias2), s[2], s[3]);
+    if constexpr (PAIR) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t word = trade<OT>(s[2 * h], s[2 * h + 1], odd);
+        if (!SOME || 4 * j4 + 2 * h + odd < count) __stcs(reinterpret_cast<uint32_t*>(o), word);
+        o += 2 * ldo;
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (!SOME || 4 * j4 + h < count) __stcs(o, narrow<OT>(s[h]));
+        o += ldo;
+      }
+    }
+  }
+}
+
+// The same for the base's last rows.
+template <typename OT, bool PAIR>
+__device__ __forceinline__ void store_ragged(const uint32_t (&v)[32], const float* qs, float xs, float bias, OT* o,
+                                             int64_t ldo, int odd, int count, int keep) {
+  const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    if (j >= count) break;
+    float s0, s1;
+    unpack(two_scores(v, j, qs[j], qs[j + 1], xs2, bias2), s0, s1);
+    if constexpr (PAIR) {
+      const uint32_t word = trade<OT>(s0, s1, odd);
+      if (j + odd < count && keep == 2) *reinterpret_cast<uint32_t*>(o) = word;
+      if (j + odd < count && keep == 1) *reinterpret_cast<unsigned short*>(o) = static_cast<unsigned short>(word);
+    } else {
+      if (keep > 0) *o = narrow<OT>(s0);
+      if (keep > 0 && j + 1 < count) o[ldo] = narrow<OT>(s1);
+    }
+    o += 2 * ldo;
+  }
+}
 
 // PAIR: 16-bit scores leave in pairs of base rows (out and its rows 4-byte
 // aligned).
@@ -107,7 +171,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + b_bytes + p.stages * p.stage_bytes);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  float* s_scale = reinterpret_cast<float*>(s_tmem + 4);  // 8 warps x 128 query scales
+  float* s_scale = reinterpret_cast<float*>(s_tmem + 4);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -130,7 +194,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     }
     for (int a = 0; a < 2; ++a) {
       tc::mbar_init(tfull_bar(a), 1);
-      tc::mbar_init(tempty_bar(a), 16);
+      tc::mbar_init(tempty_bar(a), 2 * kEpiWarps);
     }
     tc::mbar_init(bfull_bar, 1);
     tc::mbar_init(bempty_bar, 1);
@@ -153,8 +217,11 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   const uint32_t tmem_base = *s_tmem;
   const int64_t cluster = tc::cluster_id_x();
   const int64_t nclusters = tc::nclusters_x();
-  const int64_t t0 = p.tiles * cluster / nclusters;
-  const int64_t t1 = p.tiles * (cluster + 1) / nclusters;
+  const int t0 = static_cast<int>(p.tiles * cluster / nclusters);
+  const int t1 = static_cast<int>(p.tiles * (cluster + 1) / nclusters);
+  // Query group and base tile of t0; the roles count on from there.
+  const int group0 = t0 / p.base_tiles;
+  const int base0 = t0 - group0 * p.base_tiles;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -162,20 +229,20 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       int64_t loads = 0;  // ring slots filled so far: load l uses stage l % stages
       int stage = 0;
       uint32_t phase = 0;
-      int64_t group = -1;
+      bool fresh = true;    // the queries changed
       uint32_t groups = 0;  // resident query groups loaded so far
+      int qg = group0, bt = base0;
       bool ok = true;
-      for (int64_t t = t0; ok && t < t1; ++t) {
-        const int64_t qg = t / p.base_tiles;
-        const int q0 = static_cast<int>(qg * p.n_cols + rank * (p.n_cols / 2));
-        const int r0 = static_cast<int>((t - qg * p.base_tiles) * (2 * kRows) + rank * kRows);
-        if (p.resident && qg != group) {
+      for (int t = t0; ok && t < t1; ++t) {
+        const int q0 = qg * p.n_cols + static_cast<int>(rank) * (p.n_cols / 2);
+        const int r0 = bt * (2 * kRows) + static_cast<int>(rank) * kRows;
+        if (p.resident && fresh) {
           if (groups > 0 && !tc::mbar_wait(bempty_bar, (groups - 1) & 1, s_abort)) break;
           const uint32_t fb = tc::mapa_shared(bfull_bar, 0);
           if (leader) tc::mbar_arrive_expect_tx(bfull_bar, 2 * b_bytes);
           for (int kc = 0; kc < p.kc; ++kc)
             tc::tma_load_2d_pair(smem_base + kc * b_slice, &tm_q, fb, kc * kSlice, q0);
-          group = qg;
+          fresh = false;
           ++groups;
         }
         for (int kc = 0; kc < p.kc; ++kc) {
@@ -194,6 +261,11 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             phase ^= 1;
           }
         }
+        if (++bt == p.base_tiles) {
+          bt = 0;
+          ++qg;
+          fresh = true;
+        }
       }
       // Both CTAs' loads complete on the even CTA's barriers: it waits for
       // the last phase of each before shared memory goes away.
@@ -205,79 +277,93 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
-    if (leader && lane == 0) {
+    // The whole warp walks the loop, so that descriptors and addresses stay in
+    // uniform registers (issued by a lone lane, a slice's four MMAs took about
+    // 900 clocks of address arithmetic); one elected lane issues.
+    if (leader) {
+      const bool issuer = tc::elect_one();
       const uint32_t idesc = tc::idesc_s8(2 * kRows, p.n_cols);
+      const uint64_t kind = tc::sw128_kmajor_desc(0);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
-      int64_t group = -1;
+      bool fresh = true;
       uint32_t groups = 0;
+      int bt = base0;
       bool ok = true;
-      for (int64_t t = t0; ok && t < t1; ++t) {
-        if (!tc::mbar_wait(tempty_bar(acc), acc_phase ^ 1, s_abort)) break;
-        const int64_t qg = t / p.base_tiles;
-        if (p.resident && qg != group) {
-          if (!tc::mbar_wait(bfull_bar, groups & 1, s_abort)) break;
-          group = qg;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, s_abort)) != 0;
+      };
+      for (int t = t0; ok && t < t1; ++t) {
+        if (!wait(tempty_bar(acc), acc_phase ^ 1)) break;
+        if (p.resident && fresh) {
+          if (!wait(bfull_bar, groups & 1)) break;
+          fresh = false;
           ++groups;
         }
-        tc::tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
         for (int kc = 0; kc < p.kc; ++kc) {
-          if (!tc::mbar_wait(full_bar(stage), phase, s_abort)) {
+          if (!wait(full_bar(stage), phase)) {
             ok = false;
             break;
           }
           tc::tc_fence_after();
           const uint32_t a_addr = ring + stage * p.stage_bytes;
-          const uint64_t a_desc = tc::sw128_kmajor_desc(a_addr);
-          const uint64_t b_desc = tc::sw128_kmajor_desc(p.resident ? smem_base + kc * b_slice : a_addr + kA);
+          const uint64_t a_desc = kind + (a_addr >> 4);
+          const uint64_t b_desc = kind + ((p.resident ? smem_base + kc * b_slice : a_addr + kA) >> 4);
+          if (issuer) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint64_t off = static_cast<uint64_t>(kk * 32) >> 4;
-            tc::mma_s8_pair(d_tmem, a_desc + off, b_desc + off, idesc, (kc > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < 4; ++kk)
+              tc::mma_s8_pair(d_tmem, a_desc + 2 * kk, b_desc + 2 * kk, idesc, (kc > 0 || kk > 0) ? 1u : 0u);
+            tc::mma_commit_pair_both(empty_bar(stage));
           }
-          tc::mma_commit_pair_both(empty_bar(stage));
+          __syncwarp();
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        tc::mma_commit_pair_both(tfull_bar(acc));
-        if (p.resident && t + 1 < t1 && (t + 1) / p.base_tiles != qg) tc::mma_commit_pair_both(bempty_bar);
+        if (issuer) tc::mma_commit_pair_both(tfull_bar(acc));
+        if (++bt == p.base_tiles) {
+          bt = 0;
+          fresh = true;
+          if (issuer && p.resident && t + 1 < t1) tc::mma_commit_pair_both(bempty_bar);
+        }
+        __syncwarp();
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
-      tc::mma_commit_pair_both(done_bar);
+      if (issuer) tc::mma_commit_pair_both(done_bar);
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int half = (warp - 2) >> 2;  // which alternate blocks of 32 queries
-    const int quarter = warp & 3;      // TMEM lanes this warp may access
+    const int grp = (warp - 2) >> 2;  // which blocks of 32 queries: grp, grp + 4
+    const int quarter = warp & 3;     // TMEM lanes this warp may access
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    float* scale = s_scale + (warp - 2) * 128;
+    float* scale = s_scale + (warp - 2) * kWarpScales;
     OT* out = static_cast<OT*>(p.out);
     int acc = 0;
     uint32_t acc_phase = 0;
-    int64_t group = -1;
+    int qg = group0, bt = base0;
+    bool fresh = true;  // the queries changed
     bool lost = false;  // a wait gave up: the scores that remain are NaN
-    for (int64_t t = t0; t < t1; ++t) {
-      const int64_t qg = t / p.base_tiles;
-      const int64_t q0 = qg * p.n_cols;
-      const int64_t row = (t - qg * p.base_tiles) * (2 * kRows) + rank * kRows + quarter * 32 + lane;
-      if (qg != group) {
+    for (int t = t0; t < t1; ++t) {
+      const int64_t q0 = static_cast<int64_t>(qg) * p.n_cols;
+      const int64_t row = static_cast<int64_t>(bt) * (2 * kRows) + rank * kRows + quarter * 32 + lane;
+      if (fresh) {
         __syncwarp();
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int64_t qi = q0 + (2 * b + half) * 32 + lane;
+        for (int b = 0; b < kWarpScales / 32; ++b) {
+          const int64_t qi = q0 + (kGroups * b + grp) * 32 + lane;
           scale[b * 32 + lane] = qi < p.m ? __ldg(p.q_scale + qi) : 0.0f;
         }
         __syncwarp();
-        group = qg;
+        fresh = false;
       }
       float xs = 0.0f, bias = 0.0f;
       if (row < p.n) {
@@ -288,53 +374,30 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       if (lost) xs = __int_as_float(0x7fc00000);
       tc::tc_fence_after();
       const int64_t row_warp = row - lane;
-      for (int b = half; b * 32 < p.n_cols; b += 2) {
+      for (int b = grp; b * 32 < p.n_cols; b += kGroups) {
         const int64_t qb = q0 + b * 32;
         if (qb >= p.m || row_warp >= p.n) break;  // warp-uniform
         __syncwarp();
         uint32_t v[32];
         tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * 256 + b * 32), v);
         tc::tmem_ld_wait();
-        const float4* qs4 = reinterpret_cast<const float4*>(scale + (b >> 1) * 32);
+        const float* qs = scale + b / kGroups * 32;
         const int count = p.m - qb < 32 ? static_cast<int>(p.m - qb) : 32;
-        const bool whole = count == 32 && row_warp + 32 <= p.n;
-        if (PAIR) {
-          // Lanes 2i and 2i + 1 trade scores: the even one leaves with both
-          // rows of query j, the odd one with both rows of query j + 1.
-          const int odd = lane & 1;
-          OT* o = out + (qb + odd) * p.ldo + (row - odd);
-          const bool two = row - odd + 1 < p.n;
-#pragma unroll
-          for (int j4 = 0; j4 < 8; ++j4) {
-            const float4 qs = qs4[j4];
-            const float w[4] = {qs.x, qs.y, qs.z, qs.w};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int j = 4 * j4 + 2 * h;
-              const float s0 = fmaf(static_cast<float>(static_cast<int>(v[j])), w[2 * h] * xs, bias);
-              const float s1 = fmaf(static_cast<float>(static_cast<int>(v[j + 1])), w[2 * h + 1] * xs, bias);
-              const float got = __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, 1);
-              const uint32_t both = odd ? pack2<OT>(got, s1) : pack2<OT>(s0, got);
-              if (whole || (j + odd < count && two))
-                __stcs(reinterpret_cast<uint32_t*>(o + j * p.ldo), both);
-              else if (j + odd < count && row - odd < p.n)  // the last base row has no partner
-                *reinterpret_cast<unsigned short*>(o + j * p.ldo) = static_cast<unsigned short>(both);
-            }
+        // Lanes 2i and 2i + 1 trade 16-bit scores when these leave in pairs:
+        // the even one stores both rows' of query j, the odd one of j + 1.
+        const int odd = PAIR ? lane & 1 : 0;
+        OT* o = out + (qb + odd) * p.ldo + (row - odd);
+        if (row_warp + 32 <= p.n) {
+          if (count == 32) {
+            store_queries<OT, PAIR, 0>(v, qs, xs, bias, o, p.ldo, odd, 32);
+          } else {
+            store_queries<OT, PAIR, 1>(v, qs, xs, bias, o, p.ldo, odd, count);
           }
         } else {
-          OT* o = out + qb * p.ldo + row;
-#pragma unroll
-          for (int j4 = 0; j4 < 8; ++j4) {
-            const float4 qs = qs4[j4];
-            const float w[4] = {qs.x, qs.y, qs.z, qs.w};
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const int j = 4 * j4 + h;
-              const OT s = narrow<OT>(fmaf(static_cast<float>(static_cast<int>(v[j])), w[h] * xs, bias));
-              if (whole || (j < count && row < p.n)) __stcs(o, s);
-              o += p.ldo;
-            }
-          }
+          // The last base rows. keep: this lane's pair exists (2), or its
+          // first row alone (1: the last of an odd count), or nothing (0).
+          const int64_t left = p.n - (row - odd);
+          store_ragged<OT, PAIR>(v, qs, xs, bias, o, p.ldo, odd, count, left >= 2 ? 2 : left < 0 ? 0 : static_cast<int>(left));
         }
       }
       tc::tc_fence_before();
@@ -343,6 +406,11 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
+      }
+      if (++bt == p.base_tiles) {
+        bt = 0;
+        ++qg;
+        fresh = true;
       }
     }
   }
@@ -380,7 +448,8 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   const int64_t groups = (a.m + 255) / 256;
   p.n_cols = static_cast<int>(((a.m + groups - 1) / groups + 31) / 32 * 32);
   p.base_tiles = static_cast<int>((a.n + 2 * kRows - 1) / (2 * kRows));
-  p.tiles = groups * p.base_tiles;
+  if (groups * p.base_tiles > 0x7fffffff) return cudaErrorInvalidValue;
+  p.tiles = static_cast<int>(groups * p.base_tiles);
   p.kc = (a.d + kSlice - 1) / kSlice;
   const int b_slice = p.n_cols / 2 * kSlice;
   // Resident queries leave at least six ring stages, as many as the bf16
@@ -392,10 +461,10 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   p.stages = fit < kMaxStages ? fit : kMaxStages;
   const size_t smem = kFixed + b_bytes + static_cast<size_t>(p.stages) * p.stage_bytes;
   CUtensorMap maps[2];
-  cudaError_t e = encode_rows_map(&maps[0], kElemS8, a.x, a.d, a.n, a.ldx, kSlice, kRows);
-  if (e == cudaSuccess) e = encode_rows_map(&maps[1], kElemS8, a.q, a.d, a.m, a.ldq, kSlice, p.n_cols / 2);
+  cudaError_t e = encode_rows_map(&maps[0], kElemS8, a.x, a.d, a.n, a.ldx, kSlice, kRows, 128);
+  if (e == cudaSuccess) e = encode_rows_map(&maps[1], kElemS8, a.q, a.d, a.m, a.ldq, kSlice, p.n_cols / 2, 128);
   if (e != cudaSuccess) return e;
-  if (p.tiles < clusters) clusters = static_cast<int>(p.tiles);
+  if (p.tiles < clusters) clusters = p.tiles;
   const bool pair = reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.ldo % 2 == 0;
   switch (a.type) {
     case kElemF32: return launch_typed<float, false>(maps, p, clusters, smem, stream);

@@ -5,37 +5,54 @@
 //     G_ij = g_i (exp(z_ij - lse_i) - [j = y(i)]),  dq = scale * G r,  dr = scale * G^T q
 //
 // Forward: one pass over the products, whose epilogue keeps a running maximum
-// and sum per query and split of the base; a second kernel joins the splits.
-// The target's own logit stays out of the sum, so the loss is
+// and sum per query over the other rows; a second kernel joins them. The
+// target's own logit stays out of the sum, so the loss is
 //     softplus(log sum_{j != y} exp z_ij - z_iy),
-// which does not cancel when the target holds nearly all of the softmax.
+// which does not cancel when the target holds nearly all of the softmax. z_iy
+// is a dot product of its own in the joining kernel, in fp32 with rounding:
+// the tensor cores cut the bits their accumulators cannot hold, an error of
+// one sign that a loss near zero would show.
 //
 // Backward: the base is taken in pieces of columns. For each piece the
 // products are computed again, their epilogue writes the piece of G in the
-// operands' 16-bit type (a buffer of at most 64 MB, so it is read back from
-// L2), and two more products read it: dq accumulates over the pieces in fp32
-// slabs (one per split of the piece, added to in the same order every time,
-// so results do not change from run to run), dr is complete per piece.
-// G's rounding to 16 bits is the one rounding beside the outputs': relative
-// 2^-9 (bf16) or 2^-12 (fp16) of each entry, as the outputs' own. Entries are
+// operands' 16-bit type, and two more products read it: dq accumulates over
+// the pieces in fp32 slabs (one per split of the piece, added to in the same
+// order every time, so results do not change from run to run), dr is complete
+// per piece.
+// G's rounding to 16 bits is relative 2^-9 (bf16) or 2^-12 (fp16) of each
+// entry, as the outputs' own. Of thousands of probabilities it averages out;
+// the target's entry, which alone makes up most of a gradient, would carry it
+// into the result whole, so its rounding error is added back in fp32 (in dq
+// always, in dr for the first kHits queries that share a target). Entries are
 // relative to the largest |g_i|, times 2^14 for fp16, whose smallest normal
 // would otherwise lie above the probabilities of a large base.
 //
 // All three products are one kernel, instantiated per role: CTA pairs
-// (tcgen05.mma cta_group::2, kind::f16), 256 x N tiles with N <= 256, a
-// 6-stage TMA ring of 64-deep slices, two TMEM accumulators, the epilogue
-// (8 warps per CTA) overlapping the next tile. The three read their operands
-// as they lie: G^T, the base as dq's right operand and the queries as dr's are
-// MN-major tiles, so nothing is transposed in memory.
+// (tcgen05.mma cta_group::2, kind::f16), 256 M rows per pair, K slices of 64.
+// Operands stream through a ring of twelve 16 KB slots, each with its own
+// barriers. The three read their operands as they lie: G^T, the base as dq's
+// right operand and the queries as dr's are MN-major tiles, so nothing is
+// transposed in memory.
+//   Logits (kStats, kWeights): 256 x 256 tiles, two accumulators so that the
+//   epilogue overlaps the next tile. A pair walks along the base with its
+//   queries' slices kept in shared memory (the first seven; d <= 448 keeps
+//   all), which halves what it fetches from L2: streaming both operands asks
+//   L2 for 64 bytes per SM and clock at the full rate, more than it gives.
+//   Tiles are numbered query tile major and dealt to the pairs in equal runs.
+//   Gradients (kGradQ, kGradRows): tiles as wide as d up to 512 columns, for
+//   the same reason (53 bytes per SM and clock at 384); up to 256 columns the
+//   accumulator is doubled.
+// 16 epilogue warps: four per TMEM quarter, on alternate 32-column blocks.
 //
 // Bound: the tensor pipe for d >= 256 or so (2 t v d operations forward, three
 // times that backward, of which the logits again are the price of not keeping
-// them); the forward at small d by the exponentials (one per logit).
+// them); the forward at small d by the exponentials (one per logit, 16 per SM
+// and clock).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "px_rows.cuh"
 #include "px_rows.h"
-#include "px_tc.cuh"
 
 namespace px {
 
@@ -45,14 +62,19 @@ namespace {
 __device__ unsigned g_xent_err;
 
 constexpr int kHalf = 128;   // M rows per CTA (TMEM lanes)
-constexpr int kTile = 256;   // M rows per pair, and the most N columns
+constexpr int kTile = 256;   // M rows per pair; N columns of a logits tile
 constexpr int kSlice = 64;   // K values per slice: 128 bytes
-constexpr int kStages = 6;
-constexpr int kOperand = kHalf * 128;  // 16 KB
-constexpr int kStage = 2 * kOperand;
-constexpr int kThreads = 64 + 256;
-constexpr int kBars = 2 * kStages + 2 + 2 + 1;
-constexpr size_t kSmem = 1024 + kStages * kStage + kBars * 8 + 16;
+constexpr int kSlots = 12;
+constexpr int kSlot = kHalf * 128;  // 16 KB
+constexpr int kKeep = 7;     // query slices kept in shared memory at most
+constexpr int kGroups = 4;   // epilogue warps per TMEM quarter
+constexpr int kEpiWarps = 4 * kGroups;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kOutBuf = 2048;  // staging of an epilogue warp's stores: 32 rows of 64 bytes
+constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 1;
+constexpr size_t kSmem = 1024 + kSlots * kSlot + kEpiWarps * kOutBuf + kBars * 8 + 16;
+constexpr int kHits = 4;     // queries per base row whose target entry is corrected in dr
+constexpr int kAhead = 8;    // blocks of 32 targets looked through at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
@@ -60,80 +82,60 @@ constexpr float kInf = __builtin_huge_valf();
 enum Role { kStats, kWeights, kGradQ, kGradRows };
 
 template <int ROLE> struct Shape {
+  static constexpr bool LOGITS = ROLE == kStats || ROLE == kWeights;
   static constexpr bool A_MN = ROLE == kGradRows;
-  static constexpr bool B_MN = ROLE == kGradQ || ROLE == kGradRows;
+  static constexpr bool B_MN = !LOGITS;
+};
+
+// What the backward derives a query's G from.
+struct RowGrad {
+  const float* loss;
+  const float* lse;
+  const float* grad;
+  const float* top;      // the largest |grad| (grad itself when grad_stride is 0)
+  const float* divisor;  // or null
+  int grad_stride;
+  float lift;
 };
 
 struct Args {
   int64_t t, v;
   int d;
-  int m_tiles, n_tiles;  // tiles of the product (kStats: n_tiles base tiles in all)
-  int splits, per_split; // kStats: base tiles per split; kGradQ: K slices per split
-  int n_items;
-  int n_cols;            // N of a tile
+  int m_tiles, n_tiles;
+  int tiles;             // logits: m_tiles * n_tiles; gradients: items
+  int per_split;         // kGradQ: K slices per split
+  int n_cols;            // N of a tile: 256 (logits), else a multiple of 32 up to 512
   int k_slices;
-  int64_t v0;            // first base row of the piece
-  int64_t piece;         // its columns
-  uint32_t idesc;
+  int keep;              // logits: query slices kept in shared memory
+  int v0;                // first base row of the piece
+  int piece;             // its columns
+  int lists;             // kStats: (max, sum) pairs per query
+  uint32_t idesc, idesc2;  // of the first 256 columns, and of the rest
   float c;               // scale * log2(e)
+  float scale;
   const float* bias;
   const int64_t* targets;
   int64_t ignore_index;
-  float2* part;          // kStats: [t][splits * 2] (max, sum), log2 units
-  float* target_z;       // kStats: [t] the target's logit, log2 units
-  const float* lse2;     // kWeights: [t], log2 units
-  const float* row_factor;  // kWeights: [t]
-  const float* target_g;    // kWeights: [t] the target's entry before the row factor
-  void* g;               // kWeights: [t][ldg]
-  int64_t ldg;
-  float* slab;           // kGradQ: [splits][m_tiles * 256][ld_slab]
-  int64_t ld_slab;
-  int accumulate;
-  const float* out_scale;  // kGradRows: one value
-  void* out;             // kGradRows: rows v0 .. of the base's gradient
+  float2* part;          // kStats: [t][lists] (max, sum), log2 units
+  unsigned* counter;     // kStats: cleared for the joining kernel
+  RowGrad row;           // kWeights, kGradRows
+  const uint16_t* q;     // kGradRows
+  int64_t ldq;
+  int accumulate;        // kGradQ
+  uint16_t* out;         // kGradRows: the base's gradient, where TMA cannot store it
   int64_t ldo;
-  int vec_out;
+  int tma_out;
 };
-
-// Item -> the tiles a pair computes: M tile, first N tile and their count, K
-// slices [k0, k1).
-struct Item {
-  int m, n, n_end, k0, k1, split;
-};
-
-template <int ROLE>
-__device__ __forceinline__ Item item_of(const Args& p, int i) {
-  Item it;
-  it.k0 = 0;
-  it.k1 = p.k_slices;
-  it.split = 0;
-  it.m = i % p.m_tiles;
-  const int rest = i / p.m_tiles;
-  if (ROLE == kStats) {
-    it.split = rest;
-    it.n = rest * p.per_split;
-    it.n_end = min(p.n_tiles, it.n + p.per_split);
-  } else if (ROLE == kGradQ) {
-    it.n = rest % p.n_tiles;
-    it.n_end = it.n + 1;
-    it.split = rest / p.n_tiles;
-    it.k0 = it.split * p.per_split;
-    it.k1 = min(p.k_slices, it.k0 + p.per_split);
-  } else {
-    it.n = rest;
-    it.n_end = it.n + 1;
-  }
-  return it;
-}
-
-__device__ __forceinline__ void quiet_wait(uint32_t bar, uint32_t parity) {
-  int dummy = 0;
-  tc::mbar_wait(bar, parity, &dummy);
-}
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -147,74 +149,183 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Logits of 32 columns in log2 units: c * (q . r) + bias * log2(e). Columns
-// past the base, and base rows left out by a bias of -inf, are -inf whatever
-// their product.
-template <bool BIAS>
-__device__ __forceinline__ void logits32(const uint32_t (&v)[32], const Args& p, int64_t col0, float (&z)[32]) {
-  const bool whole = col0 + 32 <= p.v;
-  if (BIAS) {
-    if (whole) {
-      const float4* b4 = reinterpret_cast<const float4*>(p.bias + col0);
+template <bool BF>
+__device__ __forceinline__ float2 widen2(uint32_t w) {
+  if (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// x rounded to the operands' type.
+template <bool BF>
+__device__ __forceinline__ float rounded(float x) {
+  return BF ? __bfloat162float(__float2bfloat16_rn(x)) : __half2float(__float2half_rn(x));
+}
+
+__device__ __forceinline__ bool counts(int64_t y, int64_t ignore_index, int64_t v) {
+  return y != ignore_index && y >= 0 && y < v;
+}
+
+// A query's factor: its gradient relative to the largest, lifted; 0 for one
+// that adds nothing.
+__device__ __forceinline__ float row_factor(const RowGrad& r, bool used, int64_t t) {
+  const float top = fabsf(__ldg(r.top));
+  if (!used || top == 0.0f) return 0.0f;
+  return __ldg(r.grad + t * r.grad_stride) / top * r.lift;
+}
+
+// What the products of G are multiplied by at the end.
+__device__ __forceinline__ float out_scale(const RowGrad& r, float scale) {
+  const float top = fabsf(__ldg(r.top));
+  return top * scale / r.lift / (r.divisor != nullptr ? __ldg(r.divisor) : 1.0f);
+}
+
+// The target's entry: exp(-loss) - 1 is its share minus one, without
+// cancellation.
+__device__ __forceinline__ float target_entry(const RowGrad& r, int64_t t, float factor) {
+  return expm1f(-__ldg(r.loss + t)) * factor;
+}
+
+__device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
+  float a[10];
 #pragma unroll
-      for (int j4 = 0; j4 < 8; ++j4) {
-        const float4 b = __ldg(b4 + j4);
-        const float w[4] = {b.x, b.y, b.z, b.w};
+  for (int i = 0; i < 10; ++i)
+    a[i] = max3(__uint_as_float(v[3 * i]), __uint_as_float(v[3 * i + 1]), __uint_as_float(v[3 * i + 2]));
+  const float b0 = max3(a[0], a[1], a[2]);
+  const float b1 = max3(a[3], a[4], a[5]);
+  const float b2 = max3(a[6], a[7], a[8]);
+  const float b3 = max3(a[9], __uint_as_float(v[30]), __uint_as_float(v[31]));
+  return fmaxf(max3(b0, b1, b2), b3);
+}
+
+// Adds the bias: v becomes c * v + bias * log2(e), log2 units. Columns past
+// the base count as left out.
+__device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, int left, float c) {
+  const F2 cc = f2(c, c), le = f2(kLog2e, kLog2e);
+  if (left >= 32) {
+    const float4* b4 = reinterpret_cast<const float4*>(bias);
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
-          z[4 * j4 + h] = w[h] == -kInf ? -kInf : fmaf(__uint_as_float(v[4 * j4 + h]), p.c, w[h] * kLog2e);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float b = col0 + j < p.v ? __ldg(p.bias + col0 + j) : -kInf;
-        z[j] = b == -kInf ? -kInf : fmaf(__uint_as_float(v[j]), p.c, b * kLog2e);
-      }
+    for (int j4 = 0; j4 < 8; ++j4) {
+      const float4 b = __ldg(b4 + j4);
+      float x, y;
+      unpack(fma2(f2(__uint_as_float(v[4 * j4]), __uint_as_float(v[4 * j4 + 1])), cc, mul2(f2(b.x, b.y), le)), x, y);
+      v[4 * j4] = __float_as_uint(x);
+      v[4 * j4 + 1] = __float_as_uint(y);
+      unpack(fma2(f2(__uint_as_float(v[4 * j4 + 2]), __uint_as_float(v[4 * j4 + 3])), cc, mul2(f2(b.z, b.w), le)), x, y);
+      v[4 * j4 + 2] = __float_as_uint(x);
+      v[4 * j4 + 3] = __float_as_uint(y);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) z[j] = whole || col0 + j < p.v ? __uint_as_float(v[j]) * p.c : -kInf;
+    for (int j = 0; j < 32; ++j)
+      v[j] = __float_as_uint(j < left ? fmaf(__uint_as_float(v[j]), c, __ldg(bias + j) * kLog2e) : -kInf);
   }
+}
+
+// One 2-D tile store (or fp32 add) from shared memory, 64-byte swizzle; what
+// lies past the array is left out.
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void tma_add(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// A warp's 32 rows x 64 bytes into its staging buffer, as 64-byte swizzle
+// lays them out (16-byte piece p of row r at p ^ (r / 2 % 4): eight
+// consecutive lanes cover all banks), then one store by lane 0. The caller's
+// previous store has been read when this returns from its first wait.
+__device__ __forceinline__ void stage_row(uint32_t buf, int lane, const uint32_t (&w)[16]) {
+  if (lane == 0) store_wait_read();
+  __syncwarp();
+  const uint32_t row = buf + lane * 64;
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((p ^ ((lane >> 1) & 3)) << 4)), "r"(w[4 * p]),
+                 "r"(w[4 * p + 1]), "r"(w[4 * p + 2]), "r"(w[4 * p + 3])
+                 : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// Gradient item i: M tile, N tile, K slices [k0, k1).
+struct Item {
+  int m, n, split, k0, k1;
+};
+
+template <int ROLE>
+__device__ __forceinline__ Item item_of(const Args& p, int i) {
+  Item it;
+  it.m = i % p.m_tiles;
+  const int rest = i / p.m_tiles;
+  it.n = rest % p.n_tiles;
+  it.split = rest / p.n_tiles;
+  it.k0 = ROLE == kGradQ ? it.split * p.per_split : 0;
+  it.k1 = ROLE == kGradQ ? min(p.k_slices, it.k0 + p.per_split) : p.k_slices;
+  return it;
+}
+
+// Logits tiles [first, last) of pair `i` of `n`, and the pair that has tile x.
+__host__ __device__ __forceinline__ int run_begin(int64_t tiles, int i, int n) {
+  return static_cast<int>(tiles * i / n);
+}
+__host__ __device__ __forceinline__ int run_of(int64_t tiles, int64_t x, int n) {
+  return static_cast<int>(((x + 1) * n - 1) / tiles);
 }
 
 template <int ROLE, bool BF, bool BIAS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const Args p) {
+xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                 const __grid_constant__ CUtensorMap tm_out, const Args p) {
   using S = Shape<ROLE>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStage);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kSlots * kSlot + kEpiWarps * kOutBuf);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = tc::cluster_ctarank();
+  const int rank = static_cast<int>(tc::cluster_ctarank());
   const bool leader = rank == 0;
   const uint32_t smem_base = tc::smem_addr(smem);
   auto full_bar = [&](int s) { return tc::smem_addr(&bars[s]); };
-  auto empty_bar = [&](int s) { return tc::smem_addr(&bars[kStages + s]); };
-  auto tfull_bar = [&](int a) { return tc::smem_addr(&bars[2 * kStages + a]); };
-  auto tempty_bar = [&](int a) { return tc::smem_addr(&bars[2 * kStages + 2 + a]); };
-  const uint32_t done_bar = tc::smem_addr(&bars[2 * kStages + 4]);
+  auto empty_bar = [&](int s) { return tc::smem_addr(&bars[kSlots + s]); };
+  auto tfull_bar = [&](int a) { return tc::smem_addr(&bars[2 * kSlots + a]); };
+  auto tempty_bar = [&](int a) { return tc::smem_addr(&bars[2 * kSlots + 2 + a]); };
+  const uint32_t kfull_bar = tc::smem_addr(&bars[2 * kSlots + 4]);   // kept query slices loaded
+  const uint32_t kempty_bar = tc::smem_addr(&bars[2 * kSlots + 5]);  // and no longer read
+  const uint32_t done_bar = tc::smem_addr(&bars[2 * kSlots + 6]);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kSlots; ++s) {
       tc::mbar_init(full_bar(s), 1);
       tc::mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
       tc::mbar_init(tfull_bar(a), 1);
-      tc::mbar_init(tempty_bar(a), 16);
+      tc::mbar_init(tempty_bar(a), 2 * kEpiWarps);
     }
+    tc::mbar_init(kfull_bar, 1);
+    tc::mbar_init(kempty_bar, 1);
     tc::mbar_init(done_bar, 1);
     *s_abort = 0;
     tc::fence_mbarrier_init_cluster();
+    if (ROLE == kStats && blockIdx.x == 0) *p.counter = 0;
   }
   if (warp == 0 && lane == 0) {
     tc::prefetch_tmap(&tm_a);
     tc::prefetch_tmap(&tm_b);
+    if (ROLE != kStats) tc::prefetch_tmap(&tm_out);
   }
   if (warp == 1) {
     tc::tmem_alloc_pair(tc::smem_addr(s_tmem), 512);
@@ -227,248 +338,431 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   const uint32_t tmem_base = *s_tmem;
   const int cluster = static_cast<int>(tc::cluster_id_x());
   const int nclusters = static_cast<int>(tc::nclusters_x());
-  // Boxes of 64 columns that hold this CTA's half of an MN-major B tile.
-  const int b_boxes = S::B_MN ? (p.n_cols / 2 + 63) / 64 : 1;
+  // This pair's tiles: a run (logits), or every nclusters-th item (gradients).
+  const int first = S::LOGITS ? run_begin(p.tiles, cluster, nclusters) : cluster;
+  const int last = S::LOGITS ? run_begin(p.tiles, cluster + 1, nclusters) : p.tiles;
+  const int step = S::LOGITS ? 1 : nclusters;
+  // The first `keep` slots of shared memory hold kept query slices, the rest
+  // are the ring.
+  const int keep = S::LOGITS ? p.keep : 0;
+  const int ring = kSlots - keep;
+  const uint32_t ring_base = smem_base + keep * kSlot;
+  // An MN-major B tile: the columns of the first MMA (up to 256) and of the
+  // second, in boxes of 64 per CTA.
+  const int n_first = min(p.n_cols, kTile);
+  const int n_second = p.n_cols - n_first;
+  const int accs = p.n_cols > kTile ? 1 : 2;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      const uint32_t bytes = kOperand + (S::B_MN ? b_boxes * 8192 : kOperand);
       int64_t loads = 0;
-      int stage = 0;
+      int slot = 0;
       uint32_t phase = 0;
+      int kept = -1;          // query tile whose slices are kept
+      uint32_t keeps = 0;
       bool ok = true;
-      for (int i = cluster; ok && i < p.n_items; i += nclusters) {
-        const Item it = item_of<ROLE>(p, i);
-        const int m0 = it.m * kTile + static_cast<int>(rank) * kHalf;
-        for (int n = it.n; ok && n < it.n_end; ++n) {
-          const int n0 = n * p.n_cols + static_cast<int>(rank) * (p.n_cols / 2);
+      // The next ring slot, armed for both CTAs' bytes; 0 when a wait gave up.
+      auto next_slot = [&](uint32_t bytes, uint32_t& fb) -> uint32_t {
+        if (!tc::mbar_wait(empty_bar(slot), phase ^ 1, s_abort)) return 0;
+        const uint32_t dst = ring_base + slot * kSlot;
+        fb = tc::mapa_shared(full_bar(slot), 0);
+        if (leader) tc::mbar_arrive_expect_tx(full_bar(slot), 2 * bytes);
+        ++loads;
+        if (++slot == ring) {
+          slot = 0;
+          phase ^= 1;
+        }
+        return dst;
+      };
+      for (int i = first; ok && i < last; i += step) {
+        uint32_t fb, dst;
+        if (S::LOGITS) {
+          const int m = i / p.n_tiles, n = i - m * p.n_tiles;
+          const int m0 = m * kTile + rank * kHalf;
+          const int n0 = p.v0 + n * kTile + rank * kHalf;
+          if (m != kept) {
+            if (keeps > 0 && !tc::mbar_wait(kempty_bar, (keeps - 1) & 1, s_abort)) break;
+            fb = tc::mapa_shared(kfull_bar, 0);
+            if (leader) tc::mbar_arrive_expect_tx(kfull_bar, 2 * keep * kSlot);
+            for (int k = 0; k < keep; ++k) tc::tma_load_2d_pair(smem_base + k * kSlot, &tm_a, fb, k * kSlice, m0);
+            kept = m;
+            ++keeps;
+          }
+          for (int k = 0; k < p.k_slices; ++k) {
+            if (k >= keep) {
+              if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
+              tc::tma_load_2d_pair(dst, &tm_a, fb, k * kSlice, m0);
+            }
+            if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
+            tc::tma_load_2d_pair(dst, &tm_b, fb, k * kSlice, n0);
+          }
+        } else {
+          const Item it = item_of<ROLE>(p, i);
+          const int m0 = it.m * kTile + rank * kHalf;
+          const int n0 = it.n * p.n_cols;
+          const int boxes1 = (n_first / 2 + 63) / 64, boxes2 = (n_second / 2 + 63) / 64;
           for (int k = it.k0; k < it.k1; ++k) {
-            if (!tc::mbar_wait(empty_bar(stage), phase ^ 1, s_abort)) {
-              ok = false;
-              break;
-            }
-            const uint32_t a_dst = smem_base + stage * kStage;
-            const uint32_t b_dst = a_dst + kOperand;
-            const uint32_t fb = tc::mapa_shared(full_bar(stage), 0);
-            if (leader) tc::mbar_arrive_expect_tx(full_bar(stage), 2 * bytes);
+            if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
             if (S::A_MN) {
-              tc::tma_load_2d_pair(a_dst, &tm_a, fb, m0, k * kSlice);
-              tc::tma_load_2d_pair(a_dst + 8192, &tm_a, fb, m0 + 64, k * kSlice);
+              tc::tma_load_2d_pair(dst, &tm_a, fb, m0, k * kSlice);
+              tc::tma_load_2d_pair(dst + 8192, &tm_a, fb, m0 + 64, k * kSlice);
             } else {
-              tc::tma_load_2d_pair(a_dst, &tm_a, fb, k * kSlice, m0);
+              tc::tma_load_2d_pair(dst, &tm_a, fb, k * kSlice, m0);
             }
-            if (S::B_MN) {
-              const int k_row = k * kSlice + (ROLE == kGradQ ? static_cast<int>(p.v0) : 0);
-              for (int b = 0; b < b_boxes; ++b)
-                tc::tma_load_2d_pair(b_dst + b * 8192, &tm_b, fb, n0 + 64 * b, k_row);
-            } else {
-              tc::tma_load_2d_pair(b_dst, &tm_b, fb, k * kSlice, static_cast<int>(p.v0) + n0);
-            }
-            ++loads;
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1;
+            const int k_row = k * kSlice + (ROLE == kGradQ ? p.v0 : 0);
+            if ((dst = next_slot(boxes1 * 8192, fb)) == 0) { ok = false; break; }
+            for (int b = 0; b < boxes1; ++b)
+              tc::tma_load_2d_pair(dst + b * 8192, &tm_b, fb, n0 + rank * (n_first / 2) + 64 * b, k_row);
+            if (n_second > 0) {
+              if ((dst = next_slot(boxes2 * 8192, fb)) == 0) { ok = false; break; }
+              for (int b = 0; b < boxes2; ++b)
+                tc::tma_load_2d_pair(dst + b * 8192, &tm_b, fb, n0 + n_first + rank * (n_second / 2) + 64 * b, k_row);
             }
           }
         }
       }
       // Both CTAs' loads complete on the even CTA's barriers: it waits for
       // the last phase of each before shared memory goes away.
-      if (leader)
-        for (int64_t l = loads > kStages ? loads - kStages : 0; l < loads; ++l)
-          quiet_wait(full_bar(static_cast<int>(l % kStages)), static_cast<uint32_t>(l / kStages) & 1);
+      if (leader) {
+        for (int64_t l = loads > ring ? loads - ring : 0; l < loads; ++l)
+          quiet_wait(full_bar(static_cast<int>(l % ring)), static_cast<uint32_t>(l / ring) & 1);
+        if (keeps > 0) quiet_wait(kfull_bar, (keeps - 1) & 1);
+      }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
-    if (leader && lane == 0) {
-      int stage = 0;
+    // The whole warp walks the loop, so that descriptors and addresses stay in
+    // uniform registers; one elected lane issues.
+    if (leader) {
+      const bool issuer = tc::elect_one();
+      const uint64_t a_kind = S::A_MN ? tc::sw128_mnmajor_desc(0) : tc::sw128_kmajor_desc(0);
+      const uint64_t b_kind = S::B_MN ? tc::sw128_mnmajor_desc(0) : tc::sw128_kmajor_desc(0);
+      constexpr uint32_t kAStep = (S::A_MN ? 2048 : 32) >> 4, kBStep = (S::B_MN ? 2048 : 32) >> 4;
+      int slot = 0;
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
+      uint32_t keeps = 0;
       bool ok = true;
-      for (int i = cluster; ok && i < p.n_items; i += nclusters) {
-        const Item it = item_of<ROLE>(p, i);
-        for (int n = it.n; ok && n < it.n_end; ++n) {
-          if (!tc::mbar_wait(tempty_bar(acc), acc_phase ^ 1, s_abort)) {
-            ok = false;
-            break;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, s_abort)) != 0;
+      };
+      // The next filled ring slot; false when a wait gave up.
+      auto next_slot = [&](int& at) {
+        if (!wait(full_bar(slot), phase)) return false;
+        at = slot;
+        if (++slot == ring) {
+          slot = 0;
+          phase ^= 1;
+        }
+        return true;
+      };
+      int n_left = S::LOGITS ? p.n_tiles - first % p.n_tiles : 0;  // tiles until the queries change
+      bool fresh = true;
+      for (int i = first; ok && i < last; i += step) {
+        if (!wait(tempty_bar(acc), acc_phase ^ 1)) break;
+        int k0 = 0, k1 = p.k_slices;
+        if (S::LOGITS) {
+          if (fresh) {
+            if (!wait(kfull_bar, keeps & 1)) break;
+            ++keeps;
+            fresh = false;
           }
+        } else {
+          const Item it = item_of<ROLE>(p, i);
+          k0 = it.k0;
+          k1 = it.k1;
+        }
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kTile);
+        for (int k = k0; k < k1; ++k) {
+          int slot_a = -1, slot_b = -1, slot_c = -1;
+          const bool streamed = !S::LOGITS || k >= keep;
+          if (streamed && !next_slot(slot_a)) { ok = false; break; }
+          if (!next_slot(slot_b)) { ok = false; break; }
+          if (n_second > 0 && !next_slot(slot_c)) { ok = false; break; }
           tc::tc_fence_after();
-          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kTile);
-          for (int k = it.k0; k < it.k1; ++k) {
-            if (!tc::mbar_wait(full_bar(stage), phase, s_abort)) {
-              ok = false;
-              break;
-            }
-            tc::tc_fence_after();
-            const uint32_t a_addr = smem_base + stage * kStage;
-            const uint32_t b_addr = a_addr + kOperand;
-            const uint64_t a_desc = S::A_MN ? tc::sw128_mnmajor_desc(a_addr) : tc::sw128_kmajor_desc(a_addr);
-            const uint64_t b_desc = S::B_MN ? tc::sw128_mnmajor_desc(b_addr) : tc::sw128_kmajor_desc(b_addr);
+          const uint32_t a_at = (streamed ? ring_base + slot_a * kSlot : smem_base + k * kSlot) >> 4;
+          const uint64_t a_desc = a_kind + a_at;
+          const uint64_t b_desc = b_kind + ((ring_base + slot_b * kSlot) >> 4);
+          const uint64_t c_desc = b_kind + ((ring_base + slot_c * kSlot) >> 4);
+          const uint32_t more = k > k0 ? 1u : 0u;
+          if (issuer) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint64_t a_off = static_cast<uint64_t>(kk * (S::A_MN ? 2048 : 32)) >> 4;
-              const uint64_t b_off = static_cast<uint64_t>(kk * (S::B_MN ? 2048 : 32)) >> 4;
-              tc::mma_bf16_pair(d_tmem, a_desc + a_off, b_desc + b_off, p.idesc, (k > it.k0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < 4; ++kk)
+              tc::mma_bf16_pair(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, p.idesc, kk > 0 ? 1u : more);
+            if (S::B_MN && n_second > 0) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                tc::mma_bf16_pair(d_tmem + kTile, a_desc + kk * kAStep, c_desc + kk * kBStep, p.idesc2,
+                                  kk > 0 ? 1u : more);
             }
-            tc::mma_commit_pair_both(empty_bar(stage));
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1;
-            }
+            if (streamed) tc::mma_commit_pair_both(empty_bar(slot_a));
+            tc::mma_commit_pair_both(empty_bar(slot_b));
+            if (S::B_MN && n_second > 0) tc::mma_commit_pair_both(empty_bar(slot_c));
           }
-          if (!ok) break;
-          tc::mma_commit_pair_both(tfull_bar(acc));
-          if (++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1;
-          }
+          __syncwarp();
         }
-      }
-      tc::mma_commit_pair_both(done_bar);
-    }
-  } else {
-    // ------------------------------------------------------------ epilogue
-    const int half = (warp - 2) >> 2;  // which alternate blocks of 32 columns
-    const int quarter = warp & 3;      // TMEM lanes this warp may access
-    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const float nan = __int_as_float(0x7fc00000);
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    bool lost = false;  // a wait gave up: what remains is NaN
-    for (int i = cluster; i < p.n_items; i += nclusters) {
-      const Item it = item_of<ROLE>(p, i);
-      const int64_t m_warp = static_cast<int64_t>(it.m) * kTile + rank * kHalf + quarter * 32;
-      const int64_t m = m_warp + lane;
-      const bool live = ROLE == kGradRows ? m < p.piece : m < p.t;
-      int64_t target = -1;
-      float run_max = -kInf, run_sum = 0.0f;
-      float lse2 = 0.0f, factor = 0.0f, target_g = 0.0f;
-      float out_scale = 0.0f;
-      if (ROLE == kStats || ROLE == kWeights) {
-        if (live) target = __ldg(p.targets + m);
-        if (target == p.ignore_index) target = -1;
-      }
-      if (ROLE == kWeights && live) {
-        lse2 = __ldg(p.lse2 + m);
-        factor = __ldg(p.row_factor + m);
-        target_g = __ldg(p.target_g + m);
-      }
-      if (ROLE == kGradRows) out_scale = __ldg(p.out_scale);
-      for (int n = it.n; n < it.n_end; ++n) {
-        if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
-        tc::tc_fence_after();
-        const int64_t n0 = static_cast<int64_t>(n) * p.n_cols;
-        if (m_warp < (ROLE == kGradRows ? p.piece : p.t)) {
-          for (int b = half; b * 32 < p.n_cols; b += 2) {
-            const int64_t col = n0 + b * 32;  // within the product
-            if (ROLE == kStats && col >= p.v) break;
-            if (ROLE == kWeights && col >= p.piece) break;
-            if (ROLE == kGradRows && col >= p.d) break;
-            __syncwarp();
-            uint32_t v[32];
-            tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTile + b * 32), v);
-            tc::tmem_ld_wait();
-            if (lost) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
-            }
-            if (ROLE == kStats) {
-              float z[32];
-              logits32<BIAS>(v, p, col, z);
-              const int64_t at = target - col;
-              if (at >= 0 && at < 32) {  // the target's logit leaves the sum
-                float zt = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (j == at) {
-                    zt = z[j];
-                    z[j] = -kInf;
-                  }
-                p.target_z[m] = zt;
-              }
-              float top = run_max;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) top = fmaxf(top, z[j]);
-              const float base = top == -kInf ? 0.0f : top;
-              float sum = run_sum * ex2(run_max - base);
-              float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-              for (int j = 0; j < 32; ++j) s[j & 3] += ex2(z[j] - base);
-              run_sum = sum + ((s[0] + s[1]) + (s[2] + s[3]));
-              run_max = top;
-            }
-            if (ROLE == kWeights) {
-              float z[32];
-              logits32<BIAS>(v, p, p.v0 + col, z);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) z[j] = factor == 0.0f ? 0.0f : ex2(z[j] - lse2) * factor;
-              const int64_t at = target - (p.v0 + col);
-              if (at >= 0 && at < 32) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (j == at) z[j] = factor == 0.0f ? 0.0f : target_g * factor;
-              }
-              if (live) {
-                uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.g) + m * p.ldg + col);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  uint4 w;
-                  w.x = pack2<BF>(z[8 * j], z[8 * j + 1]);
-                  w.y = pack2<BF>(z[8 * j + 2], z[8 * j + 3]);
-                  w.z = pack2<BF>(z[8 * j + 4], z[8 * j + 5]);
-                  w.w = pack2<BF>(z[8 * j + 6], z[8 * j + 7]);
-                  o[j] = w;
-                }
-              }
-            }
-            if (ROLE == kGradQ && live) {
-              float4* o = reinterpret_cast<float4*>(
-                  p.slab + (static_cast<int64_t>(it.split) * p.m_tiles * kTile + m) * p.ld_slab + col);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                float4 w = p.accumulate ? o[j] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                w.x += __uint_as_float(v[4 * j]);
-                w.y += __uint_as_float(v[4 * j + 1]);
-                w.z += __uint_as_float(v[4 * j + 2]);
-                w.w += __uint_as_float(v[4 * j + 3]);
-                o[j] = w;
-              }
-            }
-            if (ROLE == kGradRows && live) {
-              uint16_t* o = static_cast<uint16_t*>(p.out) + (p.v0 + m) * p.ldo + col;
-              uint32_t w[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                w[j] = pack2<BF>(__uint_as_float(v[2 * j]) * out_scale, __uint_as_float(v[2 * j + 1]) * out_scale);
-              if (p.vec_out && col + 32 <= p.d) {
-                uint4* o4 = reinterpret_cast<uint4*>(o);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) __stcs(o4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
-              } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  if (col + 2 * j < p.d) o[2 * j] = static_cast<uint16_t>(w[j]);
-                  if (col + 2 * j + 1 < p.d) o[2 * j + 1] = static_cast<uint16_t>(w[j] >> 16);
-                }
-              }
-            }
-          }
+        if (!ok) break;
+        if (issuer) tc::mma_commit_pair_both(tfull_bar(acc));
+        if (S::LOGITS && --n_left == 0) {
+          n_left = p.n_tiles;
+          fresh = true;
+          if (issuer && i + 1 < last) tc::mma_commit_pair_both(kempty_bar);
         }
-        tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
-        if (++acc == 2) {
+        if (++acc == accs) {
           acc = 0;
           acc_phase ^= 1;
         }
       }
-      if (ROLE == kStats && live) {
-        if (lost) run_sum = nan;
-        p.part[(m * p.splits + it.split) * 2 + half] = make_float2(run_max, run_sum);
+      if (issuer) tc::mma_commit_pair_both(done_bar);
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int group = (warp - 2) >> 2;  // which 32-column blocks: group, group + 4, ...
+    const int quarter = warp & 3;       // TMEM lanes this warp may access
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t out_buf = smem_base + kSlots * kSlot + (warp - 2) * kOutBuf;
+    const int row_in_pair = rank * kHalf + quarter * 32 + lane;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool lost = false;  // a wait gave up: what remains is NaN
+    int m_now = -1;
+    // kStats / kWeights: the query's state.
+    int target = -1;
+    float run_max = -kInf, run_sum = 0.0f;
+    float lse2 = 0.0f, factor = 0.0f, at_target = 0.0f;
+    auto flush = [&]() {  // kStats: this pair's (max, sum) of query tile m_now
+      const int64_t q = static_cast<int64_t>(m_now) * kTile + row_in_pair;
+      if (q < p.t) {
+        const int slot = cluster - run_of(p.tiles, static_cast<int64_t>(m_now) * p.n_tiles, nclusters);
+        p.part[q * p.lists + slot * kGroups + group] =
+            make_float2(BIAS || run_max == -kInf ? run_max : run_max * p.c, lost ? __int_as_float(0x7fc00000) : run_sum);
+      }
+    };
+    for (int i = first; i < last; i += step) {
+      int m, n, split = 0;
+      if (S::LOGITS) {
+        m = i / p.n_tiles;
+        n = i - m * p.n_tiles;
+      } else {
+        const Item it = item_of<ROLE>(p, i);
+        m = it.m;
+        n = it.n;
+        split = it.split;
+      }
+      const int64_t row = static_cast<int64_t>(m) * kTile + row_in_pair;
+      const int64_t row_warp = row - lane;
+      if (S::LOGITS && m != m_now) {
+        if (ROLE == kStats && m_now >= 0) flush();
+        m_now = m;
+        run_max = -kInf;
+        run_sum = 0.0f;
+        target = -1;
+        factor = 0.0f;
+        if (row < p.t) {
+          const int64_t y = __ldg(p.targets + row);
+          const bool used = counts(y, p.ignore_index, p.v);
+          if (used) target = static_cast<int>(y) - p.v0;
+          if (ROLE == kWeights) {
+            const float l = __ldg(p.row.lse + row);
+            lse2 = l == -kInf ? kInf : l * kLog2e;
+            factor = row_factor(p.row, used, row);
+            at_target = target_entry(p.row, row, factor);
+          }
+        }
+      }
+      float final_scale = 0.0f;
+      int hits[kHits];  // kGradRows: queries whose target this base row is
+      int n_hits = 0;
+      if (ROLE == kGradRows) {
+        final_scale = out_scale(p.row, p.scale);
+        // Collected while the products run. Every lane looks for its own row
+        // among 32 * kAhead targets at a time.
+#pragma unroll
+        for (int h = 0; h < kHits; ++h) hits[h] = -1;
+        const int64_t lo = p.v0 + row_warp;
+        for (int64_t t0 = 0; t0 < p.t; t0 += 32 * kAhead) {
+          int rel[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {  // loads in flight together
+            const int64_t t = t0 + 32 * u + lane;
+            const int64_t y = t < p.t ? __ldg(p.targets + t) : -1;
+            rel[u] = counts(y, p.ignore_index, p.v) && t < p.t && y >= lo && y < lo + 32 ? static_cast<int>(y - lo) : -1;
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            unsigned some = __ballot_sync(0xffffffffu, rel[u] >= 0);
+            while (some != 0) {
+              const int j = __ffs(some) - 1;
+              some &= some - 1;
+              if (__shfl_sync(0xffffffffu, rel[u], j) == lane) {
+#pragma unroll
+                for (int h = 0; h < kHits; ++h)
+                  if (h == n_hits) hits[h] = static_cast<int>(t0) + 32 * u + j;
+                ++n_hits;
+              }
+            }
+          }
+        }
+        n_hits = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(min(n_hits, kHits)));
+      }
+      if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
+      tc::tc_fence_after();
+      const int64_t rows = ROLE == kGradRows ? p.piece : p.t;
+      if (row_warp < rows) {
+        for (int b = group; b * 32 < p.n_cols; b += kGroups) {
+          const int col = n * p.n_cols + b * 32;  // within the product
+          const int cols = ROLE == kStats ? static_cast<int>(p.v) : ROLE == kWeights ? p.piece : p.d;
+          if (col >= cols) break;
+          __syncwarp();
+          uint32_t v[32];
+          tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTile + b * 32), v);
+          tc::tmem_ld_wait();
+          if (lost) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
+          }
+          const int at = target - col;  // the target's place in the block
+          if (ROLE == kStats) {
+            const int left = cols - col;
+            if (BIAS) {
+              add_bias(v, p.bias + col, left, p.c);
+            } else if (left < 32) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j >= left) v[j] = __float_as_uint(-kInf);
+            }
+            if (at >= 0 && at < 32) {  // the target's logit stays out of the sum
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == at) v[j] = __float_as_uint(-kInf);
+            }
+            const float c = BIAS ? 1.0f : p.c;
+            const float top = fmaxf(run_max, largest(v));
+            const float base = top == -kInf ? 0.0f : top * c;
+            const F2 cc = f2(c, c), minus = f2(-base, -base);
+            const float carry = run_sum * ex2(fmaf(run_max, c, -base));
+            F2 s[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float x, y;
+              unpack(fma2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), cc, minus), x, y);
+              s[(j >> 1) & 1] = add2(s[(j >> 1) & 1], f2(ex2(x), ex2(y)));
+            }
+            float x, y;
+            unpack(add2(s[0], s[1]), x, y);
+            run_sum = carry + (x + y);
+            run_max = top;
+          }
+          if (ROLE == kWeights) {
+            if (BIAS) add_bias(v, p.bias + p.v0 + col, static_cast<int>(p.v) - p.v0 - col, p.c);
+            const float c = BIAS ? 1.0f : p.c;
+            const F2 cc = f2(c, c), minus = f2(-lse2, -lse2), ff = f2(factor, factor);
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float x, y;
+              unpack(fma2(f2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), cc, minus), x, y);
+              unpack(mul2(f2(ex2(x), ex2(y)), ff), x, y);
+              w[j] = pack2<BF>(x, y);
+            }
+            if (at >= 0 && at < 32) {
+              const uint32_t e = pack2<BF>(at_target, at_target);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                if (2 * j == at) w[j] = (w[j] & 0xffff0000u) | (e & 0xffffu);
+                if (2 * j + 1 == at) w[j] = (w[j] & 0xffffu) | (e & 0xffff0000u);
+              }
+            }
+            stage_row(out_buf, lane, w);
+            if (lane == 0) {
+              tma_store(&tm_out, out_buf, col, static_cast<int>(row_warp));
+              store_commit();
+            }
+          }
+          if (ROLE == kGradQ) {
+            // The split's slab, 16 fp32 columns at a time.
+            const int slab_row = split * p.m_tiles * kTile + static_cast<int>(row_warp);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = v[16 * h + j];
+              stage_row(out_buf, lane, w);
+              if (lane == 0) {
+                if (p.accumulate)
+                  tma_add(&tm_out, out_buf, col + 16 * h, slab_row);
+                else
+                  tma_store(&tm_out, out_buf, col + 16 * h, slab_row);
+                store_commit();
+              }
+            }
+          }
+          if (ROLE == kGradRows) {
+            for (int h = 0; h < n_hits; ++h) {
+              int t = -1;
+#pragma unroll
+              for (int k = 0; k < kHits; ++k)
+                if (k == h) t = hits[k];
+              if (t >= 0) {
+                const float entry = target_entry(p.row, t, row_factor(p.row, true, t));
+                const float rest = entry - rounded<BF>(entry);
+                const uint16_t* q = p.q + t * p.ldq + col;
+                if (col + 32 <= p.d) {
+                  const uint4* q4 = reinterpret_cast<const uint4*>(q);
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const uint4 x = __ldg(q4 + k);
+                    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                      const float2 f = widen2<BF>(u[j]);
+                      v[8 * k + 2 * j] = __float_as_uint(fmaf(rest, f.x, __uint_as_float(v[8 * k + 2 * j])));
+                      v[8 * k + 2 * j + 1] = __float_as_uint(fmaf(rest, f.y, __uint_as_float(v[8 * k + 2 * j + 1])));
+                    }
+                  }
+                } else {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    if (col + j < p.d)
+                      v[j] = __float_as_uint(fmaf(rest, widen2<BF>(__ldg(q + j)).x, __uint_as_float(v[j])));
+                }
+              }
+            }
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[j] = pack2<BF>(__uint_as_float(v[2 * j]) * final_scale, __uint_as_float(v[2 * j + 1]) * final_scale);
+            if (p.tma_out) {
+              stage_row(out_buf, lane, w);
+              if (lane == 0) {
+                tma_store(&tm_out, out_buf, col, p.v0 + static_cast<int>(row_warp));
+                store_commit();
+              }
+            } else if (row < p.piece) {
+              uint16_t* o = p.out + (p.v0 + row) * p.ldo + col;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                if (col + 2 * j < p.d) o[2 * j] = static_cast<uint16_t>(w[j]);
+                if (col + 2 * j + 1 < p.d) o[2 * j + 1] = static_cast<uint16_t>(w[j] >> 16);
+              }
+            }
+          }
+        }
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+      if (++acc == accs) {
+        acc = 0;
+        acc_phase ^= 1;
       }
     }
+    if (ROLE == kStats && m_now >= 0) flush();
+    if (ROLE != kStats && lane == 0) store_wait();
   }
 
   if (warp == 1 && lane == 0) quiet_wait(done_bar, 0);
@@ -480,62 +774,106 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   if (threadIdx.x == 0 && *s_abort) atomicOr(&g_xent_err, 1u);
 }
 
-// One warp per query: joins the splits' (max, sum) and forms the loss.
-__global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part, int per_row,
-                                                        const float* __restrict__ target_z,
-                                                        const int64_t* __restrict__ targets, int64_t ignore_index,
-                                                        int64_t t, int64_t v, float* __restrict__ loss,
-                                                        float* __restrict__ lse) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= t) return;
-  const int lane = threadIdx.x & 31;
-  const float2* pr = part + row * per_row;
-  float top = -kInf;
-  for (int i = lane; i < per_row; i += 32) top = fmaxf(top, pr[i].x);
+// q . r of 16-bit values in fp32, a warp; rows start on 16-byte boundaries.
+template <bool BF>
+__device__ __forceinline__ float warp_dot(const uint16_t* q, const uint16_t* r, int d, int lane) {
+  float s = 0.0f;
+  for (int at = lane * 8; at < d; at += 256) {
+    if (at + 8 <= d) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(q + at));
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(r + at));
+      const uint32_t u[4] = {a.x, a.y, a.z, a.w}, w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-  const float base = top == -kInf ? 0.0f : top;
-  float sum = 0.0f;
-  for (int i = lane; i < per_row; i += 32) sum += pr[i].y * exp2f(pr[i].x - base);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-  if (lane != 0) return;
-  const int64_t y = targets[row];
-  const float others = (base + log2f(sum)) * kLn2;  // -inf where no other row takes part
-  if (y == ignore_index) {
-    // target_z was not written, and nothing left the sum.
-    loss[row] = 0.0f;
-    lse[row] = others;
-  } else if (y < 0 || y >= v) {
-    loss[row] = __int_as_float(0x7fc00000);
-    lse[row] = others;
-  } else {
-    const float zt = target_z[row] * kLn2;
-    if (zt == -kInf) {  // the target is left out
-      loss[row] = sum == sum ? kInf : sum;
-      lse[row] = others;
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = widen2<BF>(u[j]), y = widen2<BF>(w[j]);
+        s = fmaf(x.x, y.x, s);
+        s = fmaf(x.y, y.y, s);
+      }
     } else {
-      const float a = others - zt;
-      const float tail = log1pf(expf(-fabsf(a)));
-      loss[row] = fmaxf(a, 0.0f) + tail + (a != a ? a : 0.0f);
-      lse[row] = fmaxf(others, zt) + tail;
+      for (int j = at; j < d; ++j) s = fmaf(widen2<BF>(__ldg(q + j)).x, widen2<BF>(__ldg(r + j)).x, s);
     }
   }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+  return s;
 }
 
-// One block: the reduced loss and its divisor, summed in 64 bits in a fixed
-// order.
-__global__ void __launch_bounds__(1024) xent_total_kernel(const float* __restrict__ loss,
-                                                          const int64_t* __restrict__ targets, int64_t ignore_index,
-                                                          int64_t t, int mean, float* __restrict__ total,
-                                                          float* __restrict__ divisor_out) {
-  __shared__ double s_sum[32];
-  __shared__ long long s_count[32];
+struct JoinArgs {
+  const float2* part;
+  int lists;           // pairs per query in part
+  int n_tiles, pairs;  // base tiles, and how many CTA pairs shared the tiles
+  int64_t tiles;
+  const uint16_t *q, *rows;
+  int64_t ldq, ldr, t, v;
+  int d;
+  float scale;
+  const float* bias;
+  const int64_t* targets;
+  int64_t ignore_index;
+  float *loss, *lse;
+  int reduction;
+  float *total, *divisor;
+  unsigned* counter;
+};
+
+// One warp per query: joins the pairs' (max, sum), forms the target's logit
+// and the loss. The last block to finish sums the losses, in 64 bits and a
+// fixed order.
+template <bool BF>
+__global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row < p.t) {
+    const int64_t m = row / kTile;
+    const int used = kGroups * (run_of(p.tiles, (m + 1) * p.n_tiles - 1, p.pairs) - run_of(p.tiles, m * p.n_tiles, p.pairs) + 1);
+    const float2* pr = p.part + row * p.lists;
+    float top = -kInf;
+    for (int i = lane; i < used; i += 32) top = fmaxf(top, pr[i].x);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float base = top == -kInf ? 0.0f : top;
+    float sum = 0.0f;
+    for (int i = lane; i < used; i += 32) sum += pr[i].y * exp2f(pr[i].x - base);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    const float others = (base + log2f(sum)) * kLn2;  // -inf where no other row takes part
+    const int64_t y = p.targets[row];
+    float loss, lse = others;
+    if (y == p.ignore_index) {
+      loss = 0.0f;
+    } else if (y < 0 || y >= p.v) {
+      loss = __int_as_float(0x7fc00000);
+    } else {
+      float zt = warp_dot<BF>(p.q + row * p.ldq, p.rows + y * p.ldr, p.d, lane) * p.scale;
+      if (p.bias != nullptr) zt += __ldg(p.bias + y);
+      if (zt == -kInf) {  // the target is left out
+        loss = sum == sum ? kInf : sum;
+      } else {
+        const float a = others - zt;
+        const float tail = log1pf(expf(-fabsf(a)));
+        loss = fmaxf(a, 0.0f) + tail + (a != a ? a : 0.0f);
+        lse = fmaxf(others, zt) + tail;
+      }
+    }
+    if (lane == 0) {
+      p.loss[row] = loss;
+      p.lse[row] = lse;
+    }
+  }
+  if (p.reduction == 0) return;
+  __shared__ bool s_last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(p.counter, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __shared__ double s_sum[8];
+  __shared__ long long s_count[8];
   double sum = 0.0;
   long long count = 0;
-  for (int64_t i = threadIdx.x; i < t; i += 1024)
-    if (targets[i] != ignore_index) {
-      sum += loss[i];
+  for (int64_t i = threadIdx.x; i < p.t; i += 256)
+    if (p.targets[i] != p.ignore_index) {
+      sum += __ldcg(p.loss + i);
       ++count;
     }
 #pragma unroll
@@ -543,147 +881,180 @@ __global__ void __launch_bounds__(1024) xent_total_kernel(const float* __restric
     sum += __shfl_xor_sync(0xffffffffu, sum, s);
     count += __shfl_xor_sync(0xffffffffu, count, s);
   }
-  if ((threadIdx.x & 31) == 0) {
+  if (lane == 0) {
     s_sum[threadIdx.x >> 5] = sum;
     s_count[threadIdx.x >> 5] = count;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) {
+    for (int w = 1; w < 8; ++w) {
       sum += s_sum[w];
       count += s_count[w];
     }
-    const double divisor = mean ? static_cast<double>(count) : 1.0;
-    total[0] = static_cast<float>(sum / divisor);
-    divisor_out[0] = static_cast<float>(divisor);
+    const double divisor = p.reduction == 2 ? static_cast<double>(count) : 1.0;
+    p.total[0] = static_cast<float>(sum / divisor);
+    p.divisor[0] = static_cast<float>(divisor);
   }
 }
 
-// One block: the queries' factors relative to the largest gradient, and what
-// the products are multiplied by at the end.
-__global__ void __launch_bounds__(1024) xent_factors_kernel(const float* __restrict__ loss,
-                                                            const float* __restrict__ lse,
-                                                            const float* __restrict__ grad, int grad_stride,
-                                                            const float* __restrict__ divisor,
-                                                            const int64_t* __restrict__ targets, int64_t ignore_index,
-                                                            int64_t t, int64_t v, float scale, float lift,
-                                                            float* __restrict__ lse2, float* __restrict__ row_factor,
-                                                            float* __restrict__ target_g,
-                                                            float* __restrict__ out_scale) {
+// One block: the largest |grad| of the queries that count.
+__global__ void __launch_bounds__(1024) xent_top_kernel(const float* __restrict__ grad,
+                                                        const int64_t* __restrict__ targets, int64_t ignore_index,
+                                                        int64_t t, int64_t v, float* __restrict__ out) {
   __shared__ float s_top[32];
   float top = 0.0f;
-  if (grad_stride == 0) {
-    top = fabsf(grad[0]);
-  } else {
-    for (int64_t i = threadIdx.x; i < t; i += 1024)
-      if (targets[i] != ignore_index) top = fmaxf(top, fabsf(grad[i]));
+  for (int64_t i = threadIdx.x; i < t; i += 1024)
+    if (counts(targets[i], ignore_index, v)) top = fmaxf(top, fabsf(grad[i]));
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < 32; ++w) top = fmaxf(top, s_top[w]);
-  }
-  if (threadIdx.x == 0) out_scale[0] = top * scale / lift / (divisor != nullptr ? divisor[0] : 1.0f);
-  for (int64_t i = threadIdx.x; i < t; i += 1024) {
-    const int64_t y = targets[i];
-    const float g = grad[grad_stride == 0 ? 0 : i];
-    const bool used = y != ignore_index && y >= 0 && y < v;
-    row_factor[i] = used && top != 0.0f ? g / top * lift : 0.0f;
-    // exp(-loss) - 1 is the target's share minus one, without cancellation.
-    target_g[i] = expm1f(-loss[i]);
-    lse2[i] = lse[i] == -kInf ? kInf : lse[i] * kLog2e;
+  for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) top = fmaxf(top, s_top[w]);
+    out[0] = top;
   }
 }
 
-// The sum of dq's slabs, scaled and rounded to the queries' type.
+struct GradQArgs {
+  const float* slab;
+  int splits;
+  int64_t slab_rows, ld_slab, t, v;
+  int d;
+  RowGrad row;
+  const int64_t* targets;
+  int64_t ignore_index;
+  const uint16_t* rows;
+  int64_t ldr;
+  float scale;
+  uint16_t* out;
+  int64_t ldo;
+};
+
+// The sum of dq's slabs plus what the target's entry lost when it was rounded,
+// scaled and rounded to the queries' type.
 template <bool BF>
-__global__ void __launch_bounds__(256) xent_grad_q_kernel(const float* __restrict__ slab, int splits, int64_t slab_rows,
-                                                          int64_t ld_slab, int64_t t, int d,
-                                                          const float* __restrict__ out_scale, uint16_t* __restrict__ out,
-                                                          int64_t ldo) {
+__global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int quads = (d + 3) / 4;
-  if (i >= t * quads) return;
+  const int quads = (p.d + 3) / 4;
+  if (i >= p.t * quads) return;
   const int64_t row = i / quads;
   const int col = static_cast<int>(i - row * quads) * 4;
-  const float4* s = reinterpret_cast<const float4*>(slab + row * ld_slab + col);
-  const int64_t step = slab_rows * ld_slab / 4;
+  const float4* s = reinterpret_cast<const float4*>(p.slab + row * p.ld_slab + col);
+  const int64_t step = p.slab_rows * p.ld_slab / 4;
   float4 sum = s[0];
 #pragma unroll 4
-  for (int k = 1; k < splits; ++k) {
+  for (int k = 1; k < p.splits; ++k) {
     const float4 w = s[k * step];
     sum.x += w.x;
     sum.y += w.y;
     sum.z += w.z;
     sum.w += w.w;
   }
-  const float f = out_scale[0];
-  const uint32_t lo = pack2<BF>(sum.x * f, sum.y * f), hi = pack2<BF>(sum.z * f, sum.w * f);
-  uint16_t* o = out + row * ldo + col;
-  if (col + 4 <= d && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+  float r[4] = {sum.x, sum.y, sum.z, sum.w};
+  const int64_t y = __ldg(p.targets + row);
+  if (counts(y, p.ignore_index, p.v)) {
+    const float entry = target_entry(p.row, row, row_factor(p.row, true, row));
+    const float rest = entry - rounded<BF>(entry);
+    const uint16_t* x = p.rows + y * p.ldr + col;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < p.d) r[j] = fmaf(rest, widen2<BF>(__ldg(x + j)).x, r[j]);
+  }
+  const float f = out_scale(p.row, p.scale);
+  const uint32_t lo = pack2<BF>(r[0] * f, r[1] * f), hi = pack2<BF>(r[2] * f, r[3] * f);
+  uint16_t* o = p.out + row * p.ldo + col;
+  if (col + 4 <= p.d && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
     *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
   } else {
     o[0] = static_cast<uint16_t>(lo);
-    if (col + 1 < d) o[1] = static_cast<uint16_t>(lo >> 16);
-    if (col + 2 < d) o[2] = static_cast<uint16_t>(hi);
-    if (col + 3 < d) o[3] = static_cast<uint16_t>(hi >> 16);
+    if (col + 1 < p.d) o[1] = static_cast<uint16_t>(lo >> 16);
+    if (col + 2 < p.d) o[2] = static_cast<uint16_t>(hi);
+    if (col + 3 < p.d) o[3] = static_cast<uint16_t>(hi >> 16);
   }
 }
 
 template <int ROLE>
 cudaError_t launch_role(const CUtensorMap* maps, const Args& p, bool bf, int clusters, cudaStream_t stream) {
-  const bool bias = (ROLE == kStats || ROLE == kWeights) && p.bias != nullptr;
   constexpr bool kB = ROLE == kStats || ROLE == kWeights;
+  const bool bias = kB && p.bias != nullptr;
   auto kern = bf ? (bias ? xent_gemm_kernel<ROLE, true, kB> : xent_gemm_kernel<ROLE, true, false>)
                  : (bias ? xent_gemm_kernel<ROLE, false, kB> : xent_gemm_kernel<ROLE, false, false>);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
   if (e != cudaSuccess) return e;
-  const int n = p.n_items < clusters ? p.n_items : clusters;
-  kern<<<2 * n, kThreads, kSmem, stream>>>(maps[0], maps[1], p);
+  kern<<<2 * clusters, kThreads, kSmem, stream>>>(maps[0], maps[1], maps[2], p);
   return cudaGetLastError();
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t align_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+template <typename T>
+T least(T a, T b) { return a < b ? a : b; }
 
-// Splits of the base for the forward: those whose items (query tile, split)
-// take the fewest base tiles of the busiest pair, an item's start and end
-// counted as one more tile.
-int stats_splits(int64_t m_tiles, int64_t n_tiles, int clusters) {
-  int best = 1;
-  int64_t best_cost = 0;
-  for (int s = 1; s <= 4 * clusters && s <= n_tiles; ++s) {
-    const int64_t per = ceil_div(n_tiles, s);
-    if (ceil_div(n_tiles, per) != s) continue;
-    const int64_t cost = ceil_div(m_tiles * s, clusters) * (per + 1);
-    if (best_cost == 0 || cost < best_cost) {
-      best = s;
-      best_cost = cost;
-    }
+// Pairs that share the forward's tiles. A multiple of the query tiles where
+// that leaves at most a tenth idle: the runs of all query tiles then begin at
+// the same base tiles, and the pairs that read the same base rows do so at the
+// same time, from L2.
+int stats_pairs(int64_t m_tiles, int64_t n_tiles, int clusters) {
+  if (m_tiles * n_tiles <= clusters) return static_cast<int>(m_tiles * n_tiles);
+  const int64_t even = clusters / m_tiles * m_tiles;
+  return static_cast<int>(even * 10 >= clusters * 9 ? even : clusters);
+}
+
+// (max, sum) pairs per query: those of the most CTA pairs that share a query
+// tile.
+int stats_lists(int64_t m_tiles, int64_t n_tiles, int pairs) {
+  int most = 1;
+  for (int64_t m = 0; m < m_tiles; ++m) {
+    const int n = run_of(m_tiles * n_tiles, (m + 1) * n_tiles - 1, pairs) - run_of(m_tiles * n_tiles, m * n_tiles, pairs) + 1;
+    most = n > most ? n : most;
   }
-  return best;
+  return most * kGroups;
 }
 
-// Columns of the base per piece of the backward: a G of 64 MB at most, whole
-// tiles, at least four of them.
-constexpr int64_t kPieceBytes = int64_t(64) << 20;
-int64_t piece_cols(int64_t t, int64_t v) {
-  const int64_t fit = kPieceBytes / 2 / t / kTile * kTile;
-  const int64_t cols = fit < 4 * kTile ? 4 * kTile : fit;
-  const int64_t all = align_up(v, kTile);
-  if (all <= cols) return all;
-  // Equal pieces: the last one is not left with a sliver.
-  return align_up(ceil_div(all, ceil_div(all, cols)), kTile);
-}
-
-// Tiles of the gradients' N side (d columns): equal widths, a multiple of 32.
+// Tiles of the gradients' N side (d columns): equal widths up to 512, a
+// multiple of 32.
 struct GradTiles {
   int n_tiles, n_cols;
   explicit GradTiles(int d) {
-    n_tiles = static_cast<int>(ceil_div(d, kTile));
+    n_tiles = static_cast<int>(ceil_div(d, 2 * kTile));
     n_cols = static_cast<int>(align_up(ceil_div(d, n_tiles), 32));
   }
 };
+
+// Base tiles (of 256 columns) per piece of the backward. A piece's G is at
+// most kPieceBytes; among the sizes that fit, the one whose waves of logits
+// and dr tiles take least, counted in slices of K per pair, with a price per
+// piece for its three launches and the add into dq's slabs (about 16 us) and one for what does not stay in
+// L2 (written once, read twice at the rate of HBM).
+constexpr int64_t kPieceBytes = int64_t(160) << 20;
+constexpr int64_t kCacheBytes = int64_t(80) << 20;
+int64_t piece_tiles(int64_t t, int64_t v, int d, int clusters) {
+  const GradTiles gt(d);
+  const int64_t all = ceil_div(v, kTile), m_tiles = ceil_div(t, kTile);
+  const int64_t per_tile = t * kTile * 2;  // bytes of G
+  const int64_t fit = least(all, kPieceBytes / per_tile > 4 ? kPieceBytes / per_tile : int64_t(4));
+  const double logits = ceil_div(d, kSlice) * 512.0, dr = ceil_div(t, kSlice) * 2.0 * gt.n_cols;  // clocks per tile
+  auto cost = [&](int64_t tiles) {
+    double c = 30000.0 + logits * ceil_div(tiles * m_tiles, clusters) + dr * ceil_div(tiles * gt.n_tiles, clusters);
+    const double over = static_cast<double>(tiles * per_tile - kCacheBytes);
+    return over > 0 ? c + 3 * over / 3400.0 : c;  // bytes per clock of HBM
+  };
+  int64_t best = fit;
+  double best_cost = 0;
+  // Sizes that fill whole waves, and equal divisions of the base.
+  auto consider = [&](int64_t tiles) {
+    if (tiles < 1 || tiles > fit) return;
+    const int64_t rest = all % tiles;
+    const double c = (all / tiles) * cost(tiles) + (rest > 0 ? cost(rest) : 0);
+    if (best_cost == 0 || c < best_cost) {
+      best_cost = c;
+      best = tiles;
+    }
+  };
+  for (int64_t n = ceil_div(all, fit); n <= ceil_div(all, fit) + 8; ++n) consider(ceil_div(all, n));
+  for (int64_t w = 1; w <= 16; ++w) consider(w * clusters / gt.n_tiles);
+  return best;
+}
 
 int grad_q_splits(int64_t m_tiles, int64_t n_tiles, int64_t slices, int clusters) {
   int64_t s = clusters / (m_tiles * n_tiles);
@@ -703,190 +1074,209 @@ struct Carve {
   }
 };
 
-struct ForwardWs {
+struct ForwardPlan {
+  int m_tiles, n_tiles, pairs, lists;
   float2* part;
-  float* target_z;
+  unsigned* counter;
   int64_t bytes;
-  ForwardWs(char* base, int64_t t, int splits) {
-    Carve c{base};
-    part = c.take<float2>(t * splits * 2);
-    target_z = c.take<float>(t);
+  ForwardPlan(void* ws, int64_t t, int64_t v, int clusters) {
+    m_tiles = static_cast<int>(ceil_div(t, kTile));
+    n_tiles = static_cast<int>(ceil_div(v, kTile));
+    pairs = stats_pairs(m_tiles, n_tiles, clusters);
+    lists = stats_lists(m_tiles, n_tiles, pairs);
+    Carve c{static_cast<char*>(ws)};
+    part = c.take<float2>(t * lists);
+    counter = c.take<unsigned>(1);
     bytes = c.used;
   }
 };
 
-struct BackwardWs {
-  float *lse2, *row_factor, *target_g, *out_scale, *slab;
+struct BackwardPlan {
+  GradTiles gt;
+  int m_tiles, q_splits;
+  int64_t piece, slab_rows, ld_slab;  // columns of a piece
+  float *top, *slab;
   uint16_t* g;
   int64_t bytes;
-  BackwardWs(char* base, int64_t t, int64_t piece, int splits, int64_t slab_rows, int64_t ld_slab) {
-    Carve c{base};
-    lse2 = c.take<float>(t);
-    row_factor = c.take<float>(t);
-    target_g = c.take<float>(t);
-    out_scale = c.take<float>(1);
-    slab = c.take<float>(splits * slab_rows * ld_slab);
+  BackwardPlan(void* ws, int64_t t, int64_t v, int d, int clusters) : gt(d) {
+    m_tiles = static_cast<int>(ceil_div(t, kTile));
+    piece = piece_tiles(t, v, d, clusters) * kTile;
+    q_splits = grad_q_splits(m_tiles, gt.n_tiles, least(piece, v) / kSlice + 1, clusters);
+    slab_rows = static_cast<int64_t>(m_tiles) * kTile;
+    ld_slab = static_cast<int64_t>(gt.n_tiles) * gt.n_cols;
+    Carve c{static_cast<char*>(ws)};
+    top = c.take<float>(1);
+    slab = c.take<float>(q_splits * slab_rows * ld_slab);
     g = c.take<uint16_t>(t * piece);
     bytes = c.used;
   }
 };
 
-}  // namespace
-
-int64_t xent_forward_workspace(int64_t t, int64_t v, int clusters) {
-  return ForwardWs(nullptr, t, stats_splits(ceil_div(t, kTile), ceil_div(v, kTile), clusters)).bytes;
-}
-
-int64_t xent_backward_workspace(int64_t t, int64_t v, int d, int clusters) {
-  const GradTiles gt(d);
-  const int64_t piece = piece_cols(t, v), m_tiles = ceil_div(t, kTile);
-  return BackwardWs(nullptr, t, piece, grad_q_splits(m_tiles, gt.n_tiles, piece / kSlice, clusters), m_tiles * kTile,
-                    static_cast<int64_t>(gt.n_tiles) * gt.n_cols)
-      .bytes;
-}
-
-cudaError_t launch_xent_forward(const XentProblem& x, float* loss, float* lse, int reduction, float* total,
-                                float* divisor, void* ws, int clusters, cudaStream_t stream, int* launches) {
+Args common_args(const XentProblem& x) {
   Args p = {};
   p.t = x.t;
   p.v = x.v;
   p.d = x.d;
-  p.m_tiles = static_cast<int>(ceil_div(x.t, kTile));
-  p.n_tiles = static_cast<int>(ceil_div(x.v, kTile));
-  p.splits = stats_splits(p.m_tiles, p.n_tiles, clusters);
-  p.per_split = static_cast<int>(ceil_div(p.n_tiles, p.splits));
-  p.n_items = p.m_tiles * p.splits;
-  p.n_cols = kTile;
-  p.k_slices = static_cast<int>(ceil_div(x.d, kSlice));
-  const bool bf = x.type == kElemBf16;
-  p.idesc = tc::idesc_16(bf, false, false, kTile, kTile);
   p.c = x.scale * kLog2e;
+  p.scale = x.scale;
   p.bias = x.bias;
   p.targets = x.targets;
   p.ignore_index = x.ignore_index;
-  const ForwardWs w(static_cast<char*>(ws), x.t, p.splits);
-  p.part = w.part;
-  p.target_z = w.target_z;
-  CUtensorMap maps[2];
-  cudaError_t e = encode_rows_map(&maps[0], x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kHalf);
-  if (e == cudaSuccess) e = encode_rows_map(&maps[1], x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kHalf);
-  if (e == cudaSuccess) e = launch_role<kStats>(maps, p, bf, clusters, stream);
+  return p;
+}
+
+// The logits' tiles: queries x n_tiles base tiles.
+void logits_args(Args& p, bool bf, int m_tiles, int n_tiles) {
+  p.m_tiles = m_tiles;
+  p.n_tiles = n_tiles;
+  p.tiles = m_tiles * n_tiles;
+  p.n_cols = kTile;
+  p.k_slices = static_cast<int>(ceil_div(p.d, kSlice));
+  p.keep = least(p.k_slices, kKeep);
+  p.idesc = p.idesc2 = tc::idesc_16(bf, false, false, kTile, kTile);
+}
+
+// A gradient's tiles.
+void grad_args(Args& p, const GradTiles& gt, bool bf, bool a_mn, int m_tiles, int64_t k, int splits) {
+  p.m_tiles = m_tiles;
+  p.n_tiles = gt.n_tiles;
+  p.n_cols = gt.n_cols;
+  p.k_slices = static_cast<int>(ceil_div(k, kSlice));
+  p.per_split = static_cast<int>(ceil_div(p.k_slices, splits));
+  p.tiles = m_tiles * gt.n_tiles * static_cast<int>(ceil_div(p.k_slices, p.per_split));
+  const int first = least(gt.n_cols, kTile);
+  p.idesc = tc::idesc_16(bf, a_mn, true, kTile, first);
+  p.idesc2 = tc::idesc_16(bf, a_mn, true, kTile, gt.n_cols > kTile ? gt.n_cols - first : first);
+}
+
+}  // namespace
+
+int64_t xent_forward_workspace(int64_t t, int64_t v, int clusters) { return ForwardPlan(nullptr, t, v, clusters).bytes; }
+
+int64_t xent_backward_workspace(int64_t t, int64_t v, int d, int clusters) {
+  return BackwardPlan(nullptr, t, v, d, clusters).bytes;
+}
+
+cudaError_t launch_xent_forward(const XentProblem& x, float* loss, float* lse, int reduction, float* total,
+                                float* divisor, void* ws, int clusters, cudaStream_t stream, int* launches) {
+  const bool bf = x.type == kElemBf16;
+  const ForwardPlan plan(ws, x.t, x.v, clusters);
+  Args p = common_args(x);
+  logits_args(p, bf, plan.m_tiles, plan.n_tiles);
+  p.part = plan.part;
+  p.lists = plan.lists;
+  p.counter = plan.counter;
+  CUtensorMap maps[3];
+  cudaError_t e = encode_rows_map(&maps[0], x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kHalf, 128);
+  if (e == cudaSuccess) e = encode_rows_map(&maps[1], x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kHalf, 128);
+  maps[2] = maps[0];  // not used
+  if (e == cudaSuccess) e = launch_role<kStats>(maps, p, bf, plan.pairs, stream);
   if (e != cudaSuccess) return e;
-  xent_join_kernel<<<static_cast<unsigned>(ceil_div(x.t, 8)), 256, 0, stream>>>(
-      w.part, 2 * p.splits, w.target_z, x.targets, x.ignore_index, x.t, x.v, loss, lse);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  JoinArgs j = {};
+  j.part = plan.part;
+  j.lists = plan.lists;
+  j.n_tiles = plan.n_tiles;
+  j.pairs = plan.pairs;
+  j.tiles = p.tiles;
+  j.q = static_cast<const uint16_t*>(x.q);
+  j.rows = static_cast<const uint16_t*>(x.rows);
+  j.ldq = x.ldq;
+  j.ldr = x.ldr;
+  j.t = x.t;
+  j.v = x.v;
+  j.d = x.d;
+  j.scale = x.scale;
+  j.bias = x.bias;
+  j.targets = x.targets;
+  j.ignore_index = x.ignore_index;
+  j.loss = loss;
+  j.lse = lse;
+  j.reduction = reduction;
+  j.total = total;
+  j.divisor = divisor;
+  j.counter = plan.counter;
+  auto join = bf ? xent_join_kernel<true> : xent_join_kernel<false>;
+  join<<<static_cast<unsigned>(ceil_div(x.t, 8)), 256, 0, stream>>>(j);
   *launches = 2;
-  if (reduction != 0) {
-    xent_total_kernel<<<1, 1024, 0, stream>>>(loss, x.targets, x.ignore_index, x.t, reduction == 2, total, divisor);
-    e = cudaGetLastError();
-    *launches = 3;
-  }
-  return e;
+  return cudaGetLastError();
 }
 
 cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const float* lse, const float* grad,
                                  int grad_stride, const float* divisor, void* dq, int64_t lddq, void* drows,
                                  int64_t lddr, void* ws, int clusters, cudaStream_t stream, int* launches) {
   const bool bf = x.type == kElemBf16;
-  const GradTiles gt(x.d);
-  const int64_t piece_max = piece_cols(x.t, x.v);
-  const int m_tiles = static_cast<int>(ceil_div(x.t, kTile));
-  const int64_t slab_rows = static_cast<int64_t>(m_tiles) * kTile;
-  const int64_t ld_slab = static_cast<int64_t>(gt.n_tiles) * gt.n_cols;
-  const int q_splits = grad_q_splits(m_tiles, gt.n_tiles, piece_max / kSlice, clusters);
-  const BackwardWs w(static_cast<char*>(ws), x.t, piece_max, q_splits, slab_rows, ld_slab);
-  xent_factors_kernel<<<1, 1024, 0, stream>>>(loss, lse, grad, grad_stride, divisor, x.targets, x.ignore_index, x.t, x.v,
-                                              x.scale, bf ? 1.0f : 16384.0f, w.lse2, w.row_factor, w.target_g,
-                                              w.out_scale);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  *launches = 1;
+  const BackwardPlan plan(ws, x.t, x.v, x.d, clusters);
+  cudaError_t e;
+  RowGrad row = {loss, lse, grad, grad, divisor, grad_stride, bf ? 1.0f : 16384.0f};
+  if (grad_stride != 0) {
+    xent_top_kernel<<<1, 1024, 0, stream>>>(grad, x.targets, x.ignore_index, x.t, x.v, plan.top);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    ++*launches;
+    row.top = plan.top;
+  }
+  Args base = common_args(x);
+  base.row = row;
+  base.q = static_cast<const uint16_t*>(x.q);
+  base.ldq = x.ldq;
 
-  Args base = {};
-  base.t = x.t;
-  base.v = x.v;
-  base.d = x.d;
-  base.targets = x.targets;
-  base.ignore_index = x.ignore_index;
-  base.c = x.scale * kLog2e;
-  base.bias = x.bias;
-  base.lse2 = w.lse2;
-  base.row_factor = w.row_factor;
-  base.target_g = w.target_g;
-  base.g = w.g;
-  base.ldg = piece_max;
-  base.out_scale = w.out_scale;
-
-  CUtensorMap weights[2];
-  e = encode_rows_map(&weights[0], x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kHalf);
-  if (e == cudaSuccess) e = encode_rows_map(&weights[1], x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kHalf);
+  CUtensorMap q_k, rows_k, q_mn, rows_mn, slab, dr;
+  e = encode_rows_map(&q_k, x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kHalf, 128);
+  if (e == cudaSuccess) e = encode_rows_map(&rows_k, x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kHalf, 128);
   // MN-major operands: boxes of 64 columns by 64 rows.
-  CUtensorMap rows_mn, q_mn;
-  if (e == cudaSuccess) e = encode_rows_map(&rows_mn, x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kSlice);
-  if (e == cudaSuccess) e = encode_rows_map(&q_mn, x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kSlice);
+  if (e == cudaSuccess) e = encode_rows_map(&rows_mn, x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kSlice, 128);
+  if (e == cudaSuccess) e = encode_rows_map(&q_mn, x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kSlice, 128);
+  // Stores: an epilogue warp's 32 rows of 64 bytes.
+  if (e == cudaSuccess)
+    e = encode_rows_map(&slab, kElemF32, plan.slab, plan.ld_slab, plan.q_splits * plan.slab_rows, plan.ld_slab * 4, 16,
+                        32, 64);
+  const bool tma_out = reinterpret_cast<uintptr_t>(drows) % 16 == 0 && lddr % 8 == 0;
+  if (e == cudaSuccess && drows != nullptr && tma_out)
+    e = encode_rows_map(&dr, x.type, drows, x.d, x.v, lddr * 2, 32, 32, 64);
+  else
+    dr = slab;  // not used
   if (e != cudaSuccess) return e;
   int splits_used = 0;
-  for (int64_t v0 = 0; v0 < x.v; v0 += piece_max) {
-    const int64_t piece = x.v - v0 < piece_max ? x.v - v0 : piece_max;
-    base.v0 = v0;
-    base.piece = piece;
-    // G of this piece.
-    Args p = base;
-    p.m_tiles = m_tiles;
-    p.n_tiles = static_cast<int>(ceil_div(piece, kTile));
-    p.n_items = p.m_tiles * p.n_tiles;
-    p.n_cols = kTile;
-    p.k_slices = static_cast<int>(ceil_div(x.d, kSlice));
-    p.idesc = tc::idesc_16(bf, false, false, kTile, kTile);
-    e = launch_role<kWeights>(weights, p, bf, clusters, stream);
+  for (int64_t v0 = 0; v0 < x.v; v0 += plan.piece) {
+    const int64_t piece = least(plan.piece, x.v - v0);
+    const int piece_n = static_cast<int>(ceil_div(piece, kTile));
+    base.v0 = static_cast<int>(v0);
+    base.piece = static_cast<int>(piece);
+    CUtensorMap g_k, g_mn, g_out;
+    e = encode_rows_map(&g_k, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kHalf, 128);
+    if (e == cudaSuccess) e = encode_rows_map(&g_mn, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kSlice, 128);
+    if (e == cudaSuccess) e = encode_rows_map(&g_out, x.type, plan.g, piece, x.t, plan.piece * 2, 32, 32, 64);
     if (e != cudaSuccess) return e;
+    Args p = base;
+    logits_args(p, bf, plan.m_tiles, piece_n);
+    CUtensorMap maps[3] = {q_k, rows_k, g_out};
+    if ((e = launch_role<kWeights>(maps, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
     ++*launches;
     if (dq != nullptr) {
       p = base;
-      p.m_tiles = m_tiles;
-      p.n_tiles = gt.n_tiles;
-      p.n_cols = gt.n_cols;
-      p.k_slices = static_cast<int>(ceil_div(piece, kSlice));
-      p.per_split = static_cast<int>(ceil_div(p.k_slices, q_splits));
-      p.splits = static_cast<int>(ceil_div(p.k_slices, p.per_split));
-      if (splits_used == 0) splits_used = p.splits;
-      p.n_items = p.m_tiles * p.n_tiles * p.splits;
-      p.idesc = tc::idesc_16(bf, false, true, kTile, gt.n_cols);
-      p.slab = w.slab;
-      p.ld_slab = ld_slab;
+      // Later pieces use no slab that the first did not write.
+      grad_args(p, plan.gt, bf, false, plan.m_tiles, piece, splits_used > 0 ? splits_used : plan.q_splits);
+      if (splits_used == 0) splits_used = p.tiles / (p.m_tiles * p.n_tiles);
       p.accumulate = v0 > 0;
-      CUtensorMap maps[2];
-      e = encode_rows_map(&maps[0], x.type, w.g, piece, x.t, piece_max * 2, kSlice, kHalf);
-      maps[1] = rows_mn;
-      if (e == cudaSuccess) e = launch_role<kGradQ>(maps, p, bf, clusters, stream);
-      if (e != cudaSuccess) return e;
+      CUtensorMap maps_q[3] = {g_k, rows_mn, slab};
+      if ((e = launch_role<kGradQ>(maps_q, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
       ++*launches;
     }
     if (drows != nullptr) {
       p = base;
-      p.m_tiles = static_cast<int>(ceil_div(piece, kTile));
-      p.n_tiles = gt.n_tiles;
-      p.n_cols = gt.n_cols;
-      p.k_slices = static_cast<int>(ceil_div(x.t, kSlice));
-      p.n_items = p.m_tiles * p.n_tiles;
-      p.idesc = tc::idesc_16(bf, true, true, kTile, gt.n_cols);
-      p.out = drows;
+      grad_args(p, plan.gt, bf, true, piece_n, x.t, 1);
+      p.out = static_cast<uint16_t*>(drows);
       p.ldo = lddr;
-      p.vec_out = reinterpret_cast<uintptr_t>(drows) % 16 == 0 && lddr % 8 == 0;
-      CUtensorMap maps[2];
-      e = encode_rows_map(&maps[0], x.type, w.g, piece, x.t, piece_max * 2, kSlice, kSlice);
-      maps[1] = q_mn;
-      if (e == cudaSuccess) e = launch_role<kGradRows>(maps, p, bf, clusters, stream);
-      if (e != cudaSuccess) return e;
+      p.tma_out = tma_out;
+      CUtensorMap maps_r[3] = {g_mn, q_mn, dr};
+      if ((e = launch_role<kGradRows>(maps_r, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
       ++*launches;
     }
   }
   if (dq != nullptr) {
-    const int64_t work = x.t * ceil_div(x.d, 4);
+    GradQArgs a = {plan.slab, splits_used, plan.slab_rows, plan.ld_slab, x.t, x.v, x.d, row, x.targets, x.ignore_index,
+                   static_cast<const uint16_t*>(x.rows), x.ldr, x.scale, static_cast<uint16_t*>(dq), lddq};
     auto kern = bf ? xent_grad_q_kernel<true> : xent_grad_q_kernel<false>;
-    kern<<<static_cast<unsigned>(ceil_div(work, 256)), 256, 0, stream>>>(w.slab, splits_used, slab_rows, ld_slab, x.t, x.d,
-                                                                         w.out_scale, static_cast<uint16_t*>(dq), lddq);
+    kern<<<static_cast<unsigned>(ceil_div(x.t * ceil_div(x.d, 4), 256)), 256, 0, stream>>>(a);
     e = cudaGetLastError();
     ++*launches;
   }

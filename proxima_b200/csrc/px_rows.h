@@ -14,7 +14,7 @@ enum ElemType { kElemF32 = 0, kElemF16 = 1, kElemBf16 = 2, kElemS8 = 3 };  // 0-
 
 // k_gemm.cu
 cudaError_t encode_rows_map(CUtensorMap* map, ElemType type, const void* base, int64_t cols, int64_t rows,
-                            int64_t pitch, int box_cols, int box_rows);
+                            int64_t pitch, int box_cols, int box_rows, int swizzle);
 
 // ---- 8-bit rows (k_quant.cu) -----------------------------------------------
 cudaError_t launch_quantize_rows(const void* x, ElemType type, int64_t n, int d, int64_t ldx, int8_t* codes,

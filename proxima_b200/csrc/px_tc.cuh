@@ -216,6 +216,17 @@ __host__ __device__ constexpr uint32_t idesc_tf32(int m, int n) {
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // ---- CTA pairs (cluster of 2, tcgen05 cta_group::2) -----------------------
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
