@@ -340,7 +340,7 @@ PX_API px_status px_softmax_xent_device(int32_t device, const void* queries, int
  * forward's. Queries that are ignored, or whose target is no row, add nothing
  * (but queries and rows are multiplied with a weight of zero, so they must be
  * finite). G takes the operands' 16 bits, in pieces of the base of at most
- * 160 MB or 1024 columns. Results do not change from run to run. */
+ * 256 MB or 1024 columns. Results do not change from run to run. */
 PX_API px_status px_softmax_xent_backward_device(int32_t device, const void* queries, int64_t ldq, int64_t t,
                                                  const void* rows, int64_t ldr, int64_t v, int32_t dim, int32_t type,
                                                  const int64_t* targets, int64_t ignore_index, float scale,

@@ -907,8 +907,8 @@ cudaError_t encode_bf16_map(CUtensorMap* map, const void* plane, int64_t rows, i
 
 // A row-major array of `rows` rows of `cols` values, `pitch` bytes apart, as a
 // TMA tensor with boxes of box_cols (`swizzle` bytes of them: 64 or 128, and
-// that swizzle) by box_rows. Values past the last column or row read as zeros
-// and are not written.
+// that swizzle) by box_rows. Values past the last column or row read as zeros;
+// a store writes whole 16-byte pieces of a row, none past its last row.
 cudaError_t encode_rows_map(CUtensorMap* map, ElemType type, const void* base, int64_t cols, int64_t rows,
                             int64_t pitch, int box_cols, int box_rows, int swizzle) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = get_encode_fn();

@@ -49,7 +49,8 @@ constexpr int kGroups = 4;        // epilogue warps per TMEM quarter
 constexpr int kEpiWarps = 4 * kGroups;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kWarpScales = 256 / kGroups;  // query scales an epilogue warp needs
-constexpr int kBars = 2 * kMaxStages + 2 + 2 + 2 + 2;  // one spare: the scales after them stay 16-byte aligned
+constexpr int kMaxAccs = 8;
+constexpr int kBars = 2 * kMaxStages + 2 * kMaxAccs + 4;  // one spare: the scales after them stay 16-byte aligned
 constexpr size_t kFixed = 1024 + kBars * 8 + 16 + kEpiWarps * kWarpScales * 4;
 constexpr size_t kSmemLimit = 232448;  // 227 KB
 
@@ -65,6 +66,7 @@ struct Params {
   int kc;          // slices
   int resident;    // queries stay in shared memory
   int stages, stage_bytes;
+  int accs;        // accumulators, 512 / accs columns each
 };
 
 template <typename T>
@@ -182,17 +184,17 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   auto full_bar = [&](int s) { return tc::smem_addr(&bars[s]); };
   auto empty_bar = [&](int s) { return tc::smem_addr(&bars[kMaxStages + s]); };
   auto tfull_bar = [&](int a) { return tc::smem_addr(&bars[2 * kMaxStages + a]); };
-  auto tempty_bar = [&](int a) { return tc::smem_addr(&bars[2 * kMaxStages + 2 + a]); };
-  const uint32_t bfull_bar = tc::smem_addr(&bars[2 * kMaxStages + 4]);   // resident queries loaded
-  const uint32_t bempty_bar = tc::smem_addr(&bars[2 * kMaxStages + 5]);  // and no longer read
-  const uint32_t done_bar = tc::smem_addr(&bars[2 * kMaxStages + 6]);
+  auto tempty_bar = [&](int a) { return tc::smem_addr(&bars[2 * kMaxStages + kMaxAccs + a]); };
+  const uint32_t bfull_bar = tc::smem_addr(&bars[2 * kMaxStages + 2 * kMaxAccs]);       // resident queries loaded
+  const uint32_t bempty_bar = tc::smem_addr(&bars[2 * kMaxStages + 2 * kMaxAccs + 1]);  // and no longer read
+  const uint32_t done_bar = tc::smem_addr(&bars[2 * kMaxStages + 2 * kMaxAccs + 2]);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       tc::mbar_init(full_bar(s), 1);
       tc::mbar_init(empty_bar(s), 1);
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < p.accs; ++a) {
       tc::mbar_init(tfull_bar(a), 1);
       tc::mbar_init(tempty_bar(a), 2 * kEpiWarps);
     }
@@ -215,6 +217,9 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   tc::cluster_sync();
   tc::tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
+  const int acc_cols = 512 / p.accs;
+  wait_for_previous();
+  let_next_start();
   const int64_t cluster = tc::cluster_id_x();
   const int64_t nclusters = tc::nclusters_x();
   const int t0 = static_cast<int>(p.tiles * cluster / nclusters);
@@ -302,7 +307,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
           fresh = false;
           ++groups;
         }
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * acc_cols);
         for (int kc = 0; kc < p.kc; ++kc) {
           if (!wait(full_bar(stage), phase)) {
             ok = false;
@@ -332,7 +337,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
           if (issuer && p.resident && t + 1 < t1) tc::mma_commit_pair_both(bempty_bar);
         }
         __syncwarp();
-        if (++acc == 2) {
+        if (++acc == p.accs) {
           acc = 0;
           acc_phase ^= 1;
         }
@@ -352,6 +357,13 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     int qg = group0, bt = base0;
     bool fresh = true;  // the queries changed
     bool lost = false;  // a wait gave up: the scores that remain are NaN
+    float next_xs, next_bias;
+    auto load_row = [&](int tile) {
+      const int64_t r = static_cast<int64_t>(tile) * (2 * kRows) + rank * kRows + quarter * 32 + lane;
+      next_xs = r < p.n ? __ldg(p.x_scale + r) : 0.0f;
+      next_bias = r < p.n && p.bias != nullptr ? __ldg(p.bias + r) : 0.0f;
+    };
+    load_row(bt);
     for (int t = t0; t < t1; ++t) {
       const int64_t q0 = static_cast<int64_t>(qg) * p.n_cols;
       const int64_t row = static_cast<int64_t>(bt) * (2 * kRows) + rank * kRows + quarter * 32 + lane;
@@ -365,24 +377,31 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         __syncwarp();
         fresh = false;
       }
-      float xs = 0.0f, bias = 0.0f;
-      if (row < p.n) {
-        xs = __ldg(p.x_scale + row);
-        if (p.bias != nullptr) bias = __ldg(p.bias + row);
-      }
+      float xs = next_xs;
+      const float bias = next_bias;
+      // The next tile's, one tile ahead of its use.
+      load_row(bt + 1 == p.base_tiles ? 0 : bt + 1);
       if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
       if (lost) xs = __int_as_float(0x7fc00000);
       tc::tc_fence_after();
       const int64_t row_warp = row - lane;
-      for (int b = grp; b * 32 < p.n_cols; b += kGroups) {
-        const int64_t qb = q0 + b * 32;
-        if (qb >= p.m || row_warp >= p.n) break;  // warp-uniform
+      // This warp's blocks: grp, grp + 4 of the tile's that hold queries.
+      const int queries = p.m - q0 < p.n_cols ? static_cast<int>(p.m - q0) : p.n_cols;
+      const int blocks = row_warp < p.n ? (queries + 31) / 32 : 0;
+      for (int b = grp; b < blocks; b += kGroups) {
         __syncwarp();
         uint32_t v[32];
-        tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * 256 + b * 32), v);
+        tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * acc_cols + b * 32), v);
         tc::tmem_ld_wait();
+        if (b + kGroups >= blocks) {
+          // The warp's last columns are in registers: the accumulator is free.
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+        }
+        const int64_t qb = q0 + b * 32;
         const float* qs = scale + b / kGroups * 32;
-        const int count = p.m - qb < 32 ? static_cast<int>(p.m - qb) : 32;
+        const int count = queries - b * 32 < 32 ? queries - b * 32 : 32;
         // Lanes 2i and 2i + 1 trade 16-bit scores when these leave in pairs:
         // the even one stores both rows' of query j, the odd one of j + 1.
         const int odd = PAIR ? lane & 1 : 0;
@@ -397,13 +416,16 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
           // The last base rows. keep: this lane's pair exists (2), or its
           // first row alone (1: the last of an odd count), or nothing (0).
           const int64_t left = p.n - (row - odd);
-          store_ragged<OT, PAIR>(v, qs, xs, bias, o, p.ldo, odd, count, left >= 2 ? 2 : left < 0 ? 0 : static_cast<int>(left));
+          store_ragged<OT, PAIR>(v, qs, xs, bias, o, p.ldo, odd, count,
+                                 left >= 2 ? 2 : left < 0 ? 0 : static_cast<int>(left));
         }
       }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
-      if (++acc == 2) {
+      if (grp >= blocks) {  // nothing to read in this tile
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+      }
+      if (++acc == p.accs) {
         acc = 0;
         acc_phase ^= 1;
       }
@@ -429,8 +451,7 @@ cudaError_t launch_typed(const CUtensorMap* maps, const Params& p, int clusters,
   auto kern = int8_scores_kernel<OT, PAIR>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  kern<<<2 * clusters, kThreads, smem, stream>>>(maps[0], maps[1], p);
-  return cudaGetLastError();
+  return launch_after(kern, 2 * clusters, kThreads, smem, stream, maps[0], maps[1], p);
 }
 
 }  // namespace
@@ -448,6 +469,9 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   const int64_t groups = (a.m + 255) / 256;
   p.n_cols = static_cast<int>(((a.m + groups - 1) / groups + 31) / 32 * 32);
   p.base_tiles = static_cast<int>((a.n + 2 * kRows - 1) / (2 * kRows));
+  // As many accumulators as fit: a tile of few queries is short, and what its
+  // hand-overs take is hidden only by the tiles in flight.
+  p.accs = p.n_cols <= 64 ? 8 : p.n_cols <= 128 ? 4 : 2;
   if (groups * p.base_tiles > 0x7fffffff) return cudaErrorInvalidValue;
   p.tiles = static_cast<int>(groups * p.base_tiles);
   p.kc = (a.d + kSlice - 1) / kSlice;

@@ -21,6 +21,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "px_rows.cuh"
 #include "px_rows.h"
 
 namespace px {
@@ -85,6 +86,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
                                                                  float* __restrict__ scales, int group, bool vec_out) {
   constexpr int VE = VB / static_cast<int>(sizeof(T));
   using W = typename Word<VB>::type;
+  wait_for_previous();
+  let_next_start();
   const int lane = threadIdx.x & (group - 1);
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
   const bool live = row < n;  // a dead group still takes part in the shuffles
@@ -141,6 +144,8 @@ __global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* _
                                                                       int64_t ldx, int8_t* __restrict__ codes,
                                                                       int64_t ldc, float* __restrict__ scales) {
   __shared__ uint32_t s_peak[kThreads / 32];
+  wait_for_previous();
+  let_next_start();
   for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
     const T* xr = x + row * ldx;
     uint32_t peak = 0;
@@ -167,6 +172,8 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const int8_t*
                                                                    T* __restrict__ out, int64_t ldo, int group) {
   using C = typename Word<VE>::type;
   using W = typename Word<VE * static_cast<int>(sizeof(T))>::type;
+  wait_for_previous();
+  let_next_start();
   const int lane = threadIdx.x & (group - 1);
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
   if (row >= n) return;
@@ -208,16 +215,14 @@ cudaError_t quantize_vec(const T* x, int64_t n, int d, int64_t ldx, int8_t* code
   const int64_t nvec = (d + VE - 1) / VE;
   if (nvec > 32 * kMost) {
     const int64_t grid = n < 65536 ? n : 65536;
-    quantize_long_rows_kernel<T><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(x, n, d, ldx, codes, ldc, scales);
-    return cudaGetLastError();
+    return launch_after(quantize_long_rows_kernel<T>, grid, kThreads, 0, stream, x, n, d, ldx, codes, ldc, scales);
   }
   const int group = group_for(nvec, 4);
   const int64_t blocks = (n * group + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
   auto kern = nvec <= 4 * group ? quantize_rows_kernel<T, VB, 4> : quantize_rows_kernel<T, VB, kMost>;
-  kern<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(x, n, d, ldx, codes, ldc, scales, group,
-                                                               aligned(codes, ldc, VE));
-  return cudaGetLastError();
+  return launch_after(kern, blocks, kThreads, 0, stream, x, n, d, ldx, codes, ldc, scales, group,
+                      aligned(codes, ldc, VE));
 }
 
 template <typename T>
@@ -236,9 +241,8 @@ cudaError_t dequantize_vec(const int8_t* codes, int64_t ldc, const float* scales
   const int group = group_for((d + VE - 1) / VE, 4);
   const int64_t blocks = (n * group + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  dequantize_rows_kernel<T, VE><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(codes, ldc, scales, n, d, out,
-                                                                                        ldo, group);
-  return cudaGetLastError();
+  return launch_after(dequantize_rows_kernel<T, VE>, blocks, kThreads, 0, stream, codes, ldc, scales, n, d, out, ldo,
+                      group);
 }
 
 template <typename T>

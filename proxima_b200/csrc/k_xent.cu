@@ -23,7 +23,7 @@
 // entry, as the outputs' own. Of thousands of probabilities it averages out;
 // the target's entry, which alone makes up most of a gradient, would carry it
 // into the result whole, so its rounding error is added back in fp32 (in dq
-// always, in dr for the first kHits queries that share a target). Entries are
+// always, in dr where at most kHits queries share a target). Entries are
 // relative to the largest |g_i|, times 2^14 for fp16, whose smallest normal
 // would otherwise lie above the probabilities of a large base.
 //
@@ -73,8 +73,7 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kOutBuf = 2048;  // staging of an epilogue warp's stores: 32 rows of 64 bytes
 constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 1;
 constexpr size_t kSmem = 1024 + kSlots * kSlot + kEpiWarps * kOutBuf + kBars * 8 + 16;
-constexpr int kHits = 4;     // queries per base row whose target entry is corrected in dr
-constexpr int kAhead = 8;    // blocks of 32 targets looked through at a time
+constexpr int kHits = 4;     // most queries that share a target for its correction in dr
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
@@ -119,6 +118,10 @@ struct Args {
   float2* part;          // kStats: [t][lists] (max, sum), log2 units
   unsigned* counter;     // kStats: cleared for the joining kernel
   RowGrad row;           // kWeights, kGradRows
+  float* rest;           // kWeights writes, kGradRows reads: [t] what rounding took from the target's entry
+  int* hits;             // [piece] how many queries have the base row as target (or null)
+  int4* hit_list;        // [piece] the first kHits of them
+  int* next_hits;        // kGradRows: cleared for the next piece
   const uint16_t* q;     // kGradRows
   int64_t ldq;
   int accumulate;        // kGradQ
@@ -221,24 +224,6 @@ __device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, i
   }
 }
 
-// One 2-D tile store (or fp32 add) from shared memory, 64-byte swizzle; what
-// lies past the array is left out.
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(src), "r"(c0), "r"(c1)
-               : "memory");
-}
-__device__ __forceinline__ void tma_add(const CUtensorMap* map, uint32_t src, int c0, int c1) {
-  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(src), "r"(c0), "r"(c1)
-               : "memory");
-}
-__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
 // A warp's 32 rows x 64 bytes into its staging buffer, as 64-byte swizzle
 // lays them out (16-byte piece p of row r at p ^ (r / 2 % 4): eight
 // consecutive lanes cover all banks), then one store by lane 0. The caller's
@@ -254,6 +239,54 @@ __device__ __forceinline__ void stage_row(uint32_t buf, int lane, const uint32_t
                  : "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
+}
+
+// The same block by plain stores, for an array that TMA cannot address (rows
+// that begin or end off 16-byte boundaries): half a warp per row where its pairs of values lie on
+// 4-byte boundaries, else a warp per row.
+__device__ __forceinline__ void store_staged(uint32_t buf, int lane, uint16_t* out, int64_t ldo, int rows, int cols) {
+  const bool words = (reinterpret_cast<uintptr_t>(out) & 3) == 0 && (ldo & 1) == 0;
+  const int per = words ? 2 : 1;  // rows at a time
+  const int c = words ? (lane & 15) * 2 : lane;
+#pragma unroll 4
+  for (int r0 = 0; r0 < 32; r0 += per) {
+    const int r = words ? r0 + (lane >> 4) : r0;
+    const uint32_t at = buf + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2;
+    if (r >= rows || c >= cols) continue;
+    uint16_t* o = out + r * ldo + c;
+    if (words && c + 1 < cols) {
+      uint32_t x;
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at));
+      *reinterpret_cast<uint32_t*>(o) = x;
+    } else {
+      uint16_t x;
+      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(at));
+      *o = x;
+    }
+  }
+}
+
+// The first n of four query numbers in ascending order, the others -1: fp32
+// additions in an order of their own, whatever order the queries came in.
+__device__ __forceinline__ int4 in_order(int4 a, int n) {
+  constexpr int kNone = 0x7fffffff;
+  if (n < 4) a.w = kNone;
+  if (n < 3) a.z = kNone;
+  if (n < 2) a.y = kNone;
+  auto order = [](int& x, int& y) {
+    const int lo = min(x, y), hi = max(x, y);
+    x = lo;
+    y = hi;
+  };
+  order(a.x, a.y);
+  order(a.z, a.w);
+  order(a.x, a.z);
+  order(a.y, a.w);
+  order(a.y, a.z);
+  if (a.y == kNone) a.y = -1;
+  if (a.z == kNone) a.z = -1;
+  if (a.w == kNone) a.w = -1;
+  return a;
 }
 
 // Gradient item i: M tile, N tile, K slices [k0, k1).
@@ -320,7 +353,6 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     tc::mbar_init(done_bar, 1);
     *s_abort = 0;
     tc::fence_mbarrier_init_cluster();
-    if (ROLE == kStats && blockIdx.x == 0) *p.counter = 0;
   }
   if (warp == 0 && lane == 0) {
     tc::prefetch_tmap(&tm_a);
@@ -336,6 +368,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   tc::cluster_sync();
   tc::tc_fence_after();
   const uint32_t tmem_base = *s_tmem;
+  wait_for_previous();
+  let_next_start();
+  if (ROLE == kStats && blockIdx.x == 0 && threadIdx.x == 0) *p.counter = 0;
   const int cluster = static_cast<int>(tc::cluster_id_x());
   const int nclusters = static_cast<int>(tc::nclusters_x());
   // This pair's tiles: a run (logits), or every nclusters-th item (gradients).
@@ -575,39 +610,19 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         }
       }
       float final_scale = 0.0f;
-      int hits[kHits];  // kGradRows: queries whose target this base row is
+      int4 hits = make_int4(-1, -1, -1, -1);  // kGradRows: the queries whose target this base row is
       int n_hits = 0;
       if (ROLE == kGradRows) {
         final_scale = out_scale(p.row, p.scale);
-        // Collected while the products run. Every lane looks for its own row
-        // among 32 * kAhead targets at a time.
-#pragma unroll
-        for (int h = 0; h < kHits; ++h) hits[h] = -1;
-        const int64_t lo = p.v0 + row_warp;
-        for (int64_t t0 = 0; t0 < p.t; t0 += 32 * kAhead) {
-          int rel[kAhead];
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) {  // loads in flight together
-            const int64_t t = t0 + 32 * u + lane;
-            const int64_t y = t < p.t ? __ldg(p.targets + t) : -1;
-            rel[u] = counts(y, p.ignore_index, p.v) && t < p.t && y >= lo && y < lo + 32 ? static_cast<int>(y - lo) : -1;
-          }
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
-            unsigned some = __ballot_sync(0xffffffffu, rel[u] >= 0);
-            while (some != 0) {
-              const int j = __ffs(some) - 1;
-              some &= some - 1;
-              if (__shfl_sync(0xffffffffu, rel[u], j) == lane) {
-#pragma unroll
-                for (int h = 0; h < kHits; ++h)
-                  if (h == n_hits) hits[h] = static_cast<int>(t0) + 32 * u + j;
-                ++n_hits;
-              }
-            }
-          }
+        if (row < p.piece) {
+          n_hits = p.hits[row];
+          // A row with more is left as it is: their errors average out, and
+          // which of them came first is chance.
+          if (n_hits > kHits) n_hits = 0;
+          if (n_hits > 0) hits = in_order(p.hit_list[row], n_hits);
+          p.next_hits[row] = 0;
         }
-        n_hits = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(min(n_hits, kHits)));
+        n_hits = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n_hits));
       }
       if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
       tc::tc_fence_after();
@@ -670,6 +685,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
               w[j] = pack2<BF>(x, y);
             }
             if (at >= 0 && at < 32) {
+              p.rest[row] = at_target - rounded<BF>(at_target);
+              if (p.hits != nullptr) {
+                const int slot = atomicAdd(p.hits + target, 1);
+                if (slot < kHits) reinterpret_cast<int*>(p.hit_list + target)[slot] = static_cast<int>(row);
+              }
               const uint32_t e = pack2<BF>(at_target, at_target);
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
@@ -703,13 +723,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           }
           if (ROLE == kGradRows) {
             for (int h = 0; h < n_hits; ++h) {
-              int t = -1;
-#pragma unroll
-              for (int k = 0; k < kHits; ++k)
-                if (k == h) t = hits[k];
+              const int t = h == 0 ? hits.x : h == 1 ? hits.y : h == 2 ? hits.z : hits.w;
               if (t >= 0) {
-                const float entry = target_entry(p.row, t, row_factor(p.row, true, t));
-                const float rest = entry - rounded<BF>(entry);
+                const float rest = __ldg(p.rest + t);
                 const uint16_t* q = p.q + t * p.ldq + col;
                 if (col + 32 <= p.d) {
                   const uint4* q4 = reinterpret_cast<const uint4*>(q);
@@ -736,19 +752,16 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
 #pragma unroll
             for (int j = 0; j < 16; ++j)
               w[j] = pack2<BF>(__uint_as_float(v[2 * j]) * final_scale, __uint_as_float(v[2 * j + 1]) * final_scale);
+            stage_row(out_buf, lane, w);
             if (p.tma_out) {
-              stage_row(out_buf, lane, w);
               if (lane == 0) {
                 tma_store(&tm_out, out_buf, col, p.v0 + static_cast<int>(row_warp));
                 store_commit();
               }
-            } else if (row < p.piece) {
-              uint16_t* o = p.out + (p.v0 + row) * p.ldo + col;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                if (col + 2 * j < p.d) o[2 * j] = static_cast<uint16_t>(w[j]);
-                if (col + 2 * j + 1 < p.d) o[2 * j + 1] = static_cast<uint16_t>(w[j] >> 16);
-              }
+            } else {
+              store_staged(out_buf, lane, p.out + (p.v0 + row_warp) * p.ldo + col, p.ldo,
+                           static_cast<int>(p.piece - row_warp), p.d - col);
+              __syncwarp();
             }
           }
         }
@@ -823,6 +836,8 @@ template <bool BF>
 __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  wait_for_previous();
+  let_next_start();
   if (row < p.t) {
     const int64_t m = row / kTile;
     const int used = kGroups * (run_of(p.tiles, (m + 1) * p.n_tiles - 1, p.pairs) - run_of(p.tiles, m * p.n_tiles, p.pairs) + 1);
@@ -871,11 +886,13 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
   __shared__ long long s_count[8];
   double sum = 0.0;
   long long count = 0;
-  for (int64_t i = threadIdx.x; i < p.t; i += 256)
-    if (p.targets[i] != p.ignore_index) {
-      sum += __ldcg(p.loss + i);
-      ++count;
-    }
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < p.t; i += 256) {
+    const bool in = __ldg(p.targets + i) != p.ignore_index;
+    const float l = __ldcg(p.loss + i);
+    sum += in ? l : 0.0f;
+    count += in;
+  }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, s);
@@ -903,6 +920,8 @@ __global__ void __launch_bounds__(1024) xent_top_kernel(const float* __restrict_
                                                         int64_t t, int64_t v, float* __restrict__ out) {
   __shared__ float s_top[32];
   float top = 0.0f;
+  wait_for_previous();
+  let_next_start();
   for (int64_t i = threadIdx.x; i < t; i += 1024)
     if (counts(targets[i], ignore_index, v)) top = fmaxf(top, fabsf(grad[i]));
 #pragma unroll
@@ -921,6 +940,7 @@ struct GradQArgs {
   int64_t slab_rows, ld_slab, t, v;
   int d;
   RowGrad row;
+  const float* rest;
   const int64_t* targets;
   int64_t ignore_index;
   const uint16_t* rows;
@@ -928,48 +948,64 @@ struct GradQArgs {
   float scale;
   uint16_t* out;
   int64_t ldo;
+  int rows_per_block;
 };
 
 // The sum of dq's slabs plus what the target's entry lost when it was rounded,
-// scaled and rounded to the queries' type.
+// scaled and rounded to the queries' type. A block takes rows_per_block rows,
+// four columns per thread.
 template <bool BF>
 __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  wait_for_previous();
+  let_next_start();
   const int quads = (p.d + 3) / 4;
-  if (i >= p.t * quads) return;
-  const int64_t row = i / quads;
-  const int col = static_cast<int>(i - row * quads) * 4;
-  const float4* s = reinterpret_cast<const float4*>(p.slab + row * p.ld_slab + col);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_block;
+  const int work = p.rows_per_block * quads;
   const int64_t step = p.slab_rows * p.ld_slab / 4;
-  float4 sum = s[0];
-#pragma unroll 4
-  for (int k = 1; k < p.splits; ++k) {
-    const float4 w = s[k * step];
-    sum.x += w.x;
-    sum.y += w.y;
-    sum.z += w.z;
-    sum.w += w.w;
-  }
-  float r[4] = {sum.x, sum.y, sum.z, sum.w};
-  const int64_t y = __ldg(p.targets + row);
-  if (counts(y, p.ignore_index, p.v)) {
-    const float entry = target_entry(p.row, row, row_factor(p.row, true, row));
-    const float rest = entry - rounded<BF>(entry);
-    const uint16_t* x = p.rows + y * p.ldr + col;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (col + j < p.d) r[j] = fmaf(rest, widen2<BF>(__ldg(x + j)).x, r[j]);
-  }
   const float f = out_scale(p.row, p.scale);
-  const uint32_t lo = pack2<BF>(r[0] * f, r[1] * f), hi = pack2<BF>(r[2] * f, r[3] * f);
-  uint16_t* o = p.out + row * p.ldo + col;
-  if (col + 4 <= p.d && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
-    *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
-  } else {
-    o[0] = static_cast<uint16_t>(lo);
-    if (col + 1 < p.d) o[1] = static_cast<uint16_t>(lo >> 16);
-    if (col + 2 < p.d) o[2] = static_cast<uint16_t>(hi);
-    if (col + 3 < p.d) o[3] = static_cast<uint16_t>(hi >> 16);
+  for (int i = threadIdx.x; i < work; i += 256) {
+    const int r_in = i / quads;
+    const int64_t row = row0 + r_in;
+    if (row >= p.t) break;
+    const int col = (i - r_in * quads) * 4;
+    const float4* s = reinterpret_cast<const float4*>(p.slab + row * p.ld_slab + col);
+    const int64_t y = __ldg(p.targets + row);
+    float4 sum = __ldcs(s);
+#pragma unroll 6
+    for (int k = 1; k < p.splits; ++k) {
+      const float4 w = __ldcs(s + k * step);
+      sum.x += w.x;
+      sum.y += w.y;
+      sum.z += w.z;
+      sum.w += w.w;
+    }
+    float r[4] = {sum.x, sum.y, sum.z, sum.w};
+    if (counts(y, p.ignore_index, p.v)) {
+      const float rest = __ldg(p.rest + row);
+      const uint16_t* x = p.rows + y * p.ldr + col;
+      if (col + 4 <= p.d) {  // rows start on 16-byte boundaries
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(x));
+        const float2 a = widen2<BF>(u.x), b = widen2<BF>(u.y);
+        r[0] = fmaf(rest, a.x, r[0]);
+        r[1] = fmaf(rest, a.y, r[1]);
+        r[2] = fmaf(rest, b.x, r[2]);
+        r[3] = fmaf(rest, b.y, r[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < p.d) r[j] = fmaf(rest, widen2<BF>(__ldg(x + j)).x, r[j]);
+      }
+    }
+    const uint32_t lo = pack2<BF>(r[0] * f, r[1] * f), hi = pack2<BF>(r[2] * f, r[3] * f);
+    uint16_t* o = p.out + row * p.ldo + col;
+    if (col + 4 <= p.d && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+    } else {
+      o[0] = static_cast<uint16_t>(lo);
+      if (col + 1 < p.d) o[1] = static_cast<uint16_t>(lo >> 16);
+      if (col + 2 < p.d) o[2] = static_cast<uint16_t>(hi);
+      if (col + 3 < p.d) o[3] = static_cast<uint16_t>(hi >> 16);
+    }
   }
 }
 
@@ -981,8 +1017,7 @@ cudaError_t launch_role(const CUtensorMap* maps, const Args& p, bool bf, int clu
                  : (bias ? xent_gemm_kernel<ROLE, false, kB> : xent_gemm_kernel<ROLE, false, false>);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
   if (e != cudaSuccess) return e;
-  kern<<<2 * clusters, kThreads, kSmem, stream>>>(maps[0], maps[1], maps[2], p);
-  return cudaGetLastError();
+  return launch_after(kern, 2 * clusters, kThreads, kSmem, stream, maps[0], maps[1], maps[2], p);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1022,22 +1057,20 @@ struct GradTiles {
 };
 
 // Base tiles (of 256 columns) per piece of the backward. A piece's G is at
-// most kPieceBytes; among the sizes that fit, the one whose waves of logits
-// and dr tiles take least, counted in slices of K per pair, with a price per
-// piece for its three launches and the add into dq's slabs (about 16 us) and one for what does not stay in
-// L2 (written once, read twice at the rate of HBM).
-constexpr int64_t kPieceBytes = int64_t(160) << 20;
-constexpr int64_t kCacheBytes = int64_t(80) << 20;
+// most kPieceBytes (larger than L2: at d >= 256 the products take longer than G's
+// way through HBM, and fewer pieces save more); among the sizes that fit, the
+// one whose waves of logits and dr tiles take least, with a price per piece for
+// its three launches and the adds into dq's slabs (about 16 us).
+constexpr int64_t kPieceBytes = int64_t(256) << 20;
 int64_t piece_tiles(int64_t t, int64_t v, int d, int clusters) {
   const GradTiles gt(d);
   const int64_t all = ceil_div(v, kTile), m_tiles = ceil_div(t, kTile);
   const int64_t per_tile = t * kTile * 2;  // bytes of G
   const int64_t fit = least(all, kPieceBytes / per_tile > 4 ? kPieceBytes / per_tile : int64_t(4));
-  const double logits = ceil_div(d, kSlice) * 512.0, dr = ceil_div(t, kSlice) * 2.0 * gt.n_cols;  // clocks per tile
+  // Clocks of a tile of each product; its bytes of G cross HBM meanwhile.
+  const double logits = ceil_div(d, kSlice) * 512.0, dr = ceil_div(t, kSlice) * 2.0 * gt.n_cols;
   auto cost = [&](int64_t tiles) {
-    double c = 30000.0 + logits * ceil_div(tiles * m_tiles, clusters) + dr * ceil_div(tiles * gt.n_tiles, clusters);
-    const double over = static_cast<double>(tiles * per_tile - kCacheBytes);
-    return over > 0 ? c + 3 * over / 3400.0 : c;  // bytes per clock of HBM
+    return 30000.0 + logits * ceil_div(tiles * m_tiles, clusters) + dr * ceil_div(tiles * gt.n_tiles, clusters);
   };
   int64_t best = fit;
   double best_cost = 0;
@@ -1095,7 +1128,9 @@ struct BackwardPlan {
   GradTiles gt;
   int m_tiles, q_splits;
   int64_t piece, slab_rows, ld_slab;  // columns of a piece
-  float *top, *slab;
+  float *top, *rest, *slab;
+  int* hits;  // two of `piece`: this piece's, and the next one's being cleared
+  int4* hit_list;
   uint16_t* g;
   int64_t bytes;
   BackwardPlan(void* ws, int64_t t, int64_t v, int d, int clusters) : gt(d) {
@@ -1106,6 +1141,9 @@ struct BackwardPlan {
     ld_slab = static_cast<int64_t>(gt.n_tiles) * gt.n_cols;
     Carve c{static_cast<char*>(ws)};
     top = c.take<float>(1);
+    rest = c.take<float>(t);
+    hits = c.take<int>(2 * piece);
+    hit_list = c.take<int4>(piece);
     slab = c.take<float>(q_splits * slab_rows * ld_slab);
     g = c.take<uint16_t>(t * piece);
     bytes = c.used;
@@ -1196,9 +1234,8 @@ cudaError_t launch_xent_forward(const XentProblem& x, float* loss, float* lse, i
   j.divisor = divisor;
   j.counter = plan.counter;
   auto join = bf ? xent_join_kernel<true> : xent_join_kernel<false>;
-  join<<<static_cast<unsigned>(ceil_div(x.t, 8)), 256, 0, stream>>>(j);
   *launches = 2;
-  return cudaGetLastError();
+  return launch_after(join, ceil_div(x.t, 8), 256, 0, stream, j);
 }
 
 cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const float* lse, const float* grad,
@@ -1209,8 +1246,8 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
   cudaError_t e;
   RowGrad row = {loss, lse, grad, grad, divisor, grad_stride, bf ? 1.0f : 16384.0f};
   if (grad_stride != 0) {
-    xent_top_kernel<<<1, 1024, 0, stream>>>(grad, x.targets, x.ignore_index, x.t, x.v, plan.top);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = launch_after(xent_top_kernel, 1, 1024, 0, stream, grad, x.targets, x.ignore_index, x.t, x.v, plan.top);
+    if (e != cudaSuccess) return e;
     ++*launches;
     row.top = plan.top;
   }
@@ -1229,18 +1266,30 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
   if (e == cudaSuccess)
     e = encode_rows_map(&slab, kElemF32, plan.slab, plan.ld_slab, plan.q_splits * plan.slab_rows, plan.ld_slab * 4, 16,
                         32, 64);
-  const bool tma_out = reinterpret_cast<uintptr_t>(drows) % 16 == 0 && lddr % 8 == 0;
+  // TMA stores whole 16-byte pieces: a row that ends inside one would take what
+  // lies behind it along.
+  const bool tma_out = reinterpret_cast<uintptr_t>(drows) % 16 == 0 && lddr % 8 == 0 && x.d % 8 == 0;
   if (e == cudaSuccess && drows != nullptr && tma_out)
     e = encode_rows_map(&dr, x.type, drows, x.d, x.v, lddr * 2, 32, 32, 64);
   else
     dr = slab;  // not used
   if (e != cudaSuccess) return e;
+  base.rest = plan.rest;
+  base.hit_list = plan.hit_list;
+  if (drows != nullptr) {
+    e = cudaMemsetAsync(plan.hits, 0, sizeof(int) * static_cast<size_t>(plan.piece), stream);
+    if (e != cudaSuccess) return e;
+  }
   int splits_used = 0;
+  int turn = 0;
   for (int64_t v0 = 0; v0 < x.v; v0 += plan.piece) {
     const int64_t piece = least(plan.piece, x.v - v0);
     const int piece_n = static_cast<int>(ceil_div(piece, kTile));
     base.v0 = static_cast<int>(v0);
     base.piece = static_cast<int>(piece);
+    base.hits = drows != nullptr ? plan.hits + turn * plan.piece : nullptr;
+    base.next_hits = plan.hits + (turn ^ 1) * plan.piece;
+    turn ^= 1;
     CUtensorMap g_k, g_mn, g_out;
     e = encode_rows_map(&g_k, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kHalf, 128);
     if (e == cudaSuccess) e = encode_rows_map(&g_mn, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kSlice, 128);
@@ -1273,11 +1322,13 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
     }
   }
   if (dq != nullptr) {
-    GradQArgs a = {plan.slab, splits_used, plan.slab_rows, plan.ld_slab, x.t, x.v, x.d, row, x.targets, x.ignore_index,
-                   static_cast<const uint16_t*>(x.rows), x.ldr, x.scale, static_cast<uint16_t*>(dq), lddq};
-    auto kern = bf ? xent_grad_q_kernel<true> : xent_grad_q_kernel<false>;
-    kern<<<static_cast<unsigned>(ceil_div(x.t * ceil_div(x.d, 4), 256)), 256, 0, stream>>>(a);
-    e = cudaGetLastError();
+    const int quads = static_cast<int>(ceil_div(x.d, 4));
+    const int rows_per_block = quads >= 256 ? 1 : 256 / quads;
+    GradQArgs a = {plan.slab, splits_used, plan.slab_rows, plan.ld_slab, x.t, x.v, x.d, row, plan.rest, x.targets,
+                   x.ignore_index, static_cast<const uint16_t*>(x.rows), x.ldr, x.scale, static_cast<uint16_t*>(dq),
+                   lddq, rows_per_block};
+    e = launch_after(bf ? xent_grad_q_kernel<true> : xent_grad_q_kernel<false>, ceil_div(x.t, rows_per_block), 256, 0,
+                     stream, a);
     ++*launches;
   }
   return e;

@@ -366,6 +366,52 @@ def test_softmax_unpitched_and_strided_operands(px):
     _check_xent(px, q2, rt, y, odd)
 
 
+@pytest.mark.parametrize("d", [1, 50, 65, 100])
+def test_padding_is_neither_read_nor_written(px, d):
+    """What lies behind the columns of a padded row, and behind the last row:
+    NaN there reaches no result, and stays."""
+    t, v = 140, 300
+    q, r, y, b = _xent_case(t, v, d, torch.bfloat16, 35, bias=True)
+    width = (d + 7) // 8 * 8 + 8
+
+    def padded(a, rows):
+        buf = torch.full((rows + 1, width), math.nan, dtype=a.dtype, device="cuda")
+        buf[:rows, :d] = a
+        return buf, buf[:rows, :d]
+
+    (qb, q2), (rb, r2) = padded(q, t), padded(r, v)
+    _check_xent(px, q2, r2, y, b)
+    # The gradients into padded arrays, through the C ABI.
+    lib, L = px._lib.load(), px._lib
+    loss, lse = torch.empty(t, device="cuda"), torch.empty(t, device="cuda")
+    ws = torch.empty(max(lib.px_softmax_xent_workspace_bytes(0, t, v, d, k) for k in (0, 1)), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    common = (0, q2.data_ptr(), width, t, r2.data_ptr(), width, v, d, 2, y.data_ptr(), -100, 1.5, b.data_ptr())
+    L.check(lib.px_softmax_xent_device(*common, 0, loss.data_ptr(), lse.data_ptr(), None, None, ws.data_ptr(), ws.numel(), stream))
+    one = torch.ones(1, device="cuda")
+    outs = [padded(torch.zeros_like(q), t), padded(torch.zeros_like(r), v)]
+    L.check(lib.px_softmax_xent_backward_device(
+        *common, loss.data_ptr(), lse.data_ptr(), one.data_ptr(), 0, None, outs[0][1].data_ptr(), width,
+        outs[1][1].data_ptr(), width, ws.data_ptr(), ws.numel(), stream))
+    q1, r1 = q.detach().requires_grad_(), r.detach().requires_grad_()
+    want = torch.autograd.grad(px.softmax_cross_entropy(q1, r1, y, scale=1.5, bias=b, reduction="sum"), (q1, r1))
+    for (buf, view), w, rows in zip(outs, want, (t, v)):
+        assert torch.equal(view, w)
+        assert buf[:, d:].isnan().all() and buf[rows].isnan().all()
+    # Codes: padding that would change the sums.
+    c1, s1, c2, s2, _ = _scores_case(t, v, d, 36, False)
+    bufs = [torch.full((rows + 1, (d + 15) // 16 * 16 + 16), 99, dtype=torch.int8, device="cuda") for rows in (t, v)]
+    for buf, c in zip(bufs, (c1, c2)):
+        buf[:-1, :d] = c
+    got = px.int8_scores(bufs[0][:-1, :d], s1, bufs[1][:-1, :d], s2)
+    assert torch.equal(got, px.int8_scores(c1.contiguous(), s1, c2.contiguous(), s2))
+    x, codes = torch.full((5, 40), math.nan, device="cuda"), torch.full((5, 48), 77, dtype=torch.int8, device="cuda")
+    x[:, :33] = 1.0
+    scales = torch.empty(5, device="cuda")
+    L.check(lib.px_quantize_rows_device(0, x.data_ptr(), 0, 5, 33, 40, codes.data_ptr(), 48, scales.data_ptr(), stream))
+    assert (codes[:, :33] == 127).all() and (codes[:, 33:] == 77).all() and (scales == np.float32(1) / np.float32(127)).all()
+
+
 def test_softmax_confident_targets(px):
     # The target holds nearly the whole softmax: the loss is far below an fp32
     # step of the logits, which subtracting them would lose.
