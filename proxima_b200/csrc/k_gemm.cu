@@ -906,8 +906,8 @@ cudaError_t encode_bf16_map(CUtensorMap* map, const void* plane, int64_t rows, i
 }
 
 // A row-major array of `rows` rows of `cols` values, `pitch` bytes apart, as a
-// TMA tensor with boxes of box_cols (`swizzle` bytes of them: 64 or 128, and
-// that swizzle) by box_rows. Values past the last column or row read as zeros;
+// TMA tensor with boxes of box_cols (`swizzle`: 64 or 128,
+// the bytes of them and that swizzle, or 0 for none) by box_rows. Values past the last column or row read as zeros;
 // a store writes whole 16-byte pieces of a row, none past its last row.
 cudaError_t encode_rows_map(CUtensorMap* map, ElemType type, const void* base, int64_t cols, int64_t rows,
                             int64_t pitch, int box_cols, int box_rows, int swizzle) {
@@ -922,7 +922,9 @@ cudaError_t encode_rows_map(CUtensorMap* map, ElemType type, const void* base, i
   cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                  swizzle == 64    ? CU_TENSOR_MAP_SWIZZLE_64B
+                  : swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                   : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }

@@ -17,10 +17,12 @@
 // where they fit (KC slices of N/2 rows; d <= 896 at N = 256), and only base
 // rows stream through the ring.
 //
-// Tiles are numbered query group major and dealt to the clusters in equal
-// contiguous runs, so a cluster changes its resident queries at most once more
-// than it must, and the clusters of different query groups read the same base
-// rows from L2.
+// Order. Neighbouring clusters take neighbouring base tiles of the same query
+// group, so what is written at any time is long runs of 256 rows of `out`:
+// runs of base tiles per cluster, whose writes lie 256 rows x 74 places apart,
+// reach 3.9 TB/s on a 400 MB matrix, neighbouring tiles 5-6. Where the base has
+// few tiles, clusters form teams with query groups of their own, so that the
+// resident queries are not replaced every few tiles.
 //
 // CTA roles (576 threads): warp 0 TMA producer, warp 1 TMEM owner and (even
 // CTA) MMA issuer, warps 2-17 epilogue: four per TMEM quarter, on alternate
@@ -48,6 +50,8 @@ constexpr int kMaxStages = 12;
 constexpr int kGroups = 4;        // epilogue warps per TMEM quarter
 constexpr int kEpiWarps = 4 * kGroups;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kOutBuf = 8192;     // staging of an epilogue group's stores
+constexpr int kBlocks = 256 / 32 / kGroups;  // blocks of 32 columns per epilogue warp
 constexpr int kWarpScales = 256 / kGroups;  // query scales an epilogue warp needs
 constexpr int kMaxAccs = 8;
 constexpr int kBars = 2 * kMaxStages + 2 * kMaxAccs + 4;  // one spare: the scales after them stay 16-byte aligned
@@ -60,12 +64,15 @@ struct Params {
   const float* bias;
   void* out;
   int64_t ldo, m, n;
-  int tiles;       // query groups x base tiles
+  int groups;      // query groups
   int base_tiles;
+  int teams, width;  // teams of `width` clusters; a team takes every teams-th query group
   int n_cols;      // queries per tile: a multiple of 32, at most 256
   int kc;          // slices
   int resident;    // queries stay in shared memory
+  int subs;        // groups of 256 base rows per tile: subs * n_cols <= 256
   int stages, stage_bytes;
+  int keep_base;   // base rows are read again: L2 should keep them
   int accs;        // accumulators, 512 / accs columns each
 };
 
@@ -159,18 +166,74 @@ __device__ __forceinline__ void store_ragged(const uint32_t (&v)[32], const floa
   }
 }
 
-// PAIR: 16-bit scores leave in pairs of base rows (out and its rows 4-byte
-// aligned).
-template <typename OT, bool PAIR>
+// Arrive and wait of one epilogue group's four warps.
+__device__ __forceinline__ void group_sync(int grp) {
+  asm volatile("bar.sync %0, 128;" ::"r"(grp + 1) : "memory");
+}
+
+// Stages a block's scores of the CTA's 128 base rows, with the group's other
+// three warps, and stores them by TMA: rows of 128 scores, 16 queries of fp32
+// or 32 of 16 bits at a time. Queries and base rows past the matrix are not
+// written.
+template <typename OT>
+__device__ __forceinline__ void stage_queries(const uint32_t (&v)[32], const float* qs, float xs, float bias,
+                                              uint32_t buf, int row_in_tile, int grp, int count,
+                                              const CUtensorMap* map, int row_tile, int q) {
+  const float4* qs4 = reinterpret_cast<const float4*>(qs);
+  const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
+  constexpr int kParts = sizeof(OT) / 2, kQueries = 32 / kParts;
+  const uint32_t at = buf + row_in_tile * static_cast<int>(sizeof(OT));
+#pragma unroll
+  for (int part = 0; part < kParts; ++part) {
+    if (part * kQueries >= count) break;
+    if (row_in_tile == 0) store_wait_read();
+    group_sync(grp);
+#pragma unroll
+    for (int i = 0; i < kQueries / 4; ++i) {
+      const float4 w = qs4[part * (kQueries / 4) + i];
+      const int j = part * kQueries + 4 * i;
+      float s[4];
+      unpack(two_scores(v, j, w.x, w.y, xs2, bias2), s[0], s[1]);
+      unpack(two_scores(v, j + 2, w.z, w.w, xs2, bias2), s[2], s[3]);
+      if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (4 * i + k) * (kRows * 4)), "f"(s[k]) : "memory");
+      } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t both = pack2<OT>(s[2 * k], s[2 * k + 1]);
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + (4 * i + 2 * k) * (kRows * 2)),
+                       "h"(static_cast<unsigned short>(both))
+                       : "memory");
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + (4 * i + 2 * k + 1) * (kRows * 2)),
+                       "h"(static_cast<unsigned short>(both >> 16))
+                       : "memory");
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    group_sync(grp);
+    if (row_in_tile == 0) {
+      tma_store(map, buf, row_tile, q + part * kQueries);
+      store_commit();
+    }
+  }
+}
+
+// TMA: `out` can be stored by TMA (rows of whole 16-byte pieces, on 16-byte
+// boundaries). Otherwise PAIR: 16-bit scores leave in pairs of base rows (out
+// and its rows 4-byte aligned).
+template <typename OT, bool PAIR, bool TMA>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_q,
-                   const Params p) {
+                   const __grid_constant__ CUtensorMap tm_out, const Params p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int b_slice = p.n_cols / 2 * kSlice;  // bytes of a slice of this CTA's queries
   const int b_bytes = p.resident ? p.kc * b_slice : 0;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + b_bytes + p.stages * p.stage_bytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + b_bytes + p.stages * p.stage_bytes + (TMA ? kGroups * kOutBuf : 0));
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   float* s_scale = reinterpret_cast<float*>(s_tmem + 4);
@@ -220,13 +283,24 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   const int acc_cols = 512 / p.accs;
   wait_for_previous();
   let_next_start();
-  const int64_t cluster = tc::cluster_id_x();
-  const int64_t nclusters = tc::nclusters_x();
-  const int t0 = static_cast<int>(p.tiles * cluster / nclusters);
-  const int t1 = static_cast<int>(p.tiles * (cluster + 1) / nclusters);
-  // Query group and base tile of t0; the roles count on from there.
-  const int group0 = t0 / p.base_tiles;
-  const int base0 = t0 - group0 * p.base_tiles;
+  // This cluster's tiles: numbers first, first + width, ... of its team's.
+  const int team = static_cast<int>(tc::cluster_id_x()) / p.width;
+  const int first = static_cast<int>(tc::cluster_id_x()) % p.width;
+  const int tiles = p.base_tiles * ((p.groups - team + p.teams - 1) / p.teams);
+  const int base0 = first % p.base_tiles;
+  const int group0 = team + first / p.base_tiles * p.teams;
+  // The next tile: `width` base tiles on, in the team's next query group where
+  // that passes the last; true if the queries changed.
+  auto advance = [&](int& qg, int& bt) {
+    bt += p.width;
+    bool changed = false;
+    while (bt >= p.base_tiles) {
+      bt -= p.base_tiles;
+      qg += p.teams;
+      changed = true;
+    }
+    return changed;
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -235,12 +309,13 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       int stage = 0;
       uint32_t phase = 0;
       bool fresh = true;    // the queries changed
+      const uint64_t policy = p.keep_base ? tc::l2_evict_last() : tc::l2_evict_first();
       uint32_t groups = 0;  // resident query groups loaded so far
       int qg = group0, bt = base0;
       bool ok = true;
-      for (int t = t0; ok && t < t1; ++t) {
+      for (int t = first; ok && t < tiles; t += p.width) {
         const int q0 = qg * p.n_cols + static_cast<int>(rank) * (p.n_cols / 2);
-        const int r0 = bt * (2 * kRows) + static_cast<int>(rank) * kRows;
+        const int r0 = bt * p.subs * (2 * kRows) + static_cast<int>(rank) * kRows;
         if (p.resident && fresh) {
           if (groups > 0 && !tc::mbar_wait(bempty_bar, (groups - 1) & 1, s_abort)) break;
           const uint32_t fb = tc::mapa_shared(bfull_bar, 0);
@@ -258,19 +333,16 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
           const uint32_t dst = ring + stage * p.stage_bytes;
           const uint32_t fb = tc::mapa_shared(full_bar(stage), 0);
           if (leader) tc::mbar_arrive_expect_tx(full_bar(stage), 2 * p.stage_bytes);
-          tc::tma_load_2d_pair(dst, &tm_x, fb, kc * kSlice, r0);
-          if (!p.resident) tc::tma_load_2d_pair(dst + kA, &tm_q, fb, kc * kSlice, q0);
+          for (int sub = 0; sub < p.subs; ++sub)
+            tc::tma_load_2d_pair_hint(dst + sub * kA, &tm_x, fb, kc * kSlice, r0 + sub * (2 * kRows), policy);
+          if (!p.resident) tc::tma_load_2d_pair(dst + p.subs * kA, &tm_q, fb, kc * kSlice, q0);
           ++loads;
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (++bt == p.base_tiles) {
-          bt = 0;
-          ++qg;
-          fresh = true;
-        }
+        fresh = advance(qg, bt) || fresh;
       }
       // Both CTAs' loads complete on the even CTA's barriers: it waits for
       // the last phase of each before shared memory goes away.
@@ -295,12 +367,12 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       uint32_t acc_phase = 0;
       bool fresh = true;
       uint32_t groups = 0;
-      int bt = base0;
+      int qg = group0, bt = base0;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity) {
         return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, s_abort)) != 0;
       };
-      for (int t = t0; ok && t < t1; ++t) {
+      for (int t = first; ok && t < tiles; t += p.width) {
         if (!wait(tempty_bar(acc), acc_phase ^ 1)) break;
         if (p.resident && fresh) {
           if (!wait(bfull_bar, groups & 1)) break;
@@ -315,12 +387,15 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
           }
           tc::tc_fence_after();
           const uint32_t a_addr = ring + stage * p.stage_bytes;
-          const uint64_t a_desc = kind + (a_addr >> 4);
-          const uint64_t b_desc = kind + ((p.resident ? smem_base + kc * b_slice : a_addr + kA) >> 4);
+          const uint64_t b_desc = kind + ((p.resident ? smem_base + kc * b_slice : a_addr + p.subs * kA) >> 4);
           if (issuer) {
+            for (int sub = 0; sub < p.subs; ++sub) {
+              const uint64_t a_desc = kind + ((a_addr + sub * kA) >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::mma_s8_pair(d_tmem, a_desc + 2 * kk, b_desc + 2 * kk, idesc, (kc > 0 || kk > 0) ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk)
+                tc::mma_s8_pair(d_tmem + sub * p.n_cols, a_desc + 2 * kk, b_desc + 2 * kk, idesc,
+                                (kc > 0 || kk > 0) ? 1u : 0u);
+            }
             tc::mma_commit_pair_both(empty_bar(stage));
           }
           __syncwarp();
@@ -331,10 +406,9 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         }
         if (!ok) break;
         if (issuer) tc::mma_commit_pair_both(tfull_bar(acc));
-        if (++bt == p.base_tiles) {
-          bt = 0;
+        if (advance(qg, bt)) {
           fresh = true;
-          if (issuer && p.resident && t + 1 < t1) tc::mma_commit_pair_both(bempty_bar);
+          if (issuer && p.resident && t + p.width < tiles) tc::mma_commit_pair_both(bempty_bar);
         }
         __syncwarp();
         if (++acc == p.accs) {
@@ -351,76 +425,101 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     const int quarter = warp & 3;     // TMEM lanes this warp may access
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     float* scale = s_scale + (warp - 2) * kWarpScales;
+    const uint32_t out_buf = ring + p.stages * p.stage_bytes + grp * kOutBuf;
     OT* out = static_cast<OT*>(p.out);
     int acc = 0;
     uint32_t acc_phase = 0;
     int qg = group0, bt = base0;
     bool fresh = true;  // the queries changed
     bool lost = false;  // a wait gave up: the scores that remain are NaN
-    float next_xs, next_bias;
-    auto load_row = [&](int tile) {
-      const int64_t r = static_cast<int64_t>(tile) * (2 * kRows) + rank * kRows + quarter * 32 + lane;
-      next_xs = r < p.n ? __ldg(p.x_scale + r) : 0.0f;
-      next_bias = r < p.n && p.bias != nullptr ? __ldg(p.bias + r) : 0.0f;
+    // This warp's blocks of 32 columns: grp and grp + 4 of the tile's, block b
+    // being queries b % q_blocks of base rows b / q_blocks.
+    const int q_blocks = p.n_cols / 32;
+    const int row_in_cta = quarter * 32 + lane;
+    float next_xs[kBlocks], next_bias[kBlocks];
+    auto load_rows = [&](int tile) {
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const int sub = (grp + kGroups * k) / q_blocks;
+        const int64_t r = (static_cast<int64_t>(tile) * p.subs + sub) * (2 * kRows) + rank * kRows + row_in_cta;
+        const bool live = sub < p.subs && r < p.n;
+        next_xs[k] = live ? __ldg(p.x_scale + r) : 0.0f;
+        next_bias[k] = live && p.bias != nullptr ? __ldg(p.bias + r) : 0.0f;
+      }
     };
-    load_row(bt);
-    for (int t = t0; t < t1; ++t) {
+    load_rows(bt);
+    for (int t = first; t < tiles; t += p.width) {
       const int64_t q0 = static_cast<int64_t>(qg) * p.n_cols;
-      const int64_t row = static_cast<int64_t>(bt) * (2 * kRows) + rank * kRows + quarter * 32 + lane;
       if (fresh) {
         __syncwarp();
 #pragma unroll
-        for (int b = 0; b < kWarpScales / 32; ++b) {
-          const int64_t qi = q0 + (kGroups * b + grp) * 32 + lane;
-          scale[b * 32 + lane] = qi < p.m ? __ldg(p.q_scale + qi) : 0.0f;
+        for (int k = 0; k < kBlocks; ++k) {
+          const int64_t qi = q0 + (grp + kGroups * k) % q_blocks * 32 + lane;
+          scale[k * 32 + lane] = qi < p.m ? __ldg(p.q_scale + qi) : 0.0f;
         }
         __syncwarp();
         fresh = false;
       }
-      float xs = next_xs;
-      const float bias = next_bias;
-      // The next tile's, one tile ahead of its use.
-      load_row(bt + 1 == p.base_tiles ? 0 : bt + 1);
+      float xs[kBlocks], bias[kBlocks];
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        xs[k] = next_xs[k];
+        bias[k] = next_bias[k];
+      }
+      // The next tile's, one tile ahead of their use.
+      load_rows((bt + p.width) % p.base_tiles);
       if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
-      if (lost) xs = __int_as_float(0x7fc00000);
       tc::tc_fence_after();
-      const int64_t row_warp = row - lane;
-      // This warp's blocks: grp, grp + 4 of the tile's that hold queries.
       const int queries = p.m - q0 < p.n_cols ? static_cast<int>(p.m - q0) : p.n_cols;
-      const int blocks = row_warp < p.n ? (queries + 31) / 32 : 0;
-      for (int b = grp; b < blocks; b += kGroups) {
+      bool freed = false;
+#pragma unroll
+      for (int k = 0; k < kBlocks; ++k) {
+        const int b = grp + kGroups * k;
+        const int sub = b / q_blocks, q_in = (b - sub * q_blocks) * 32;
+        const int64_t row_cta = (static_cast<int64_t>(bt) * p.subs + sub) * (2 * kRows) + rank * kRows;
+        const int64_t row = row_cta + row_in_cta, row_warp = row - lane;
+        // With TMA all four warps of a group take part, base rows or not: they
+        // meet at barriers, and TMA leaves out what lies past the matrix.
+        if (sub >= p.subs || q_in >= queries || (TMA ? row_cta >= p.n : row_warp >= p.n)) continue;  // warp-uniform
         __syncwarp();
         uint32_t v[32];
         tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * acc_cols + b * 32), v);
         tc::tmem_ld_wait();
-        if (b + kGroups >= blocks) {
+        if (k == kBlocks - 1) {
           // The warp's last columns are in registers: the accumulator is free.
           tc::tc_fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+          freed = true;
         }
-        const int64_t qb = q0 + b * 32;
-        const float* qs = scale + b / kGroups * 32;
-        const int count = queries - b * 32 < 32 ? queries - b * 32 : 32;
-        // Lanes 2i and 2i + 1 trade 16-bit scores when these leave in pairs:
-        // the even one stores both rows' of query j, the odd one of j + 1.
-        const int odd = PAIR ? lane & 1 : 0;
-        OT* o = out + (qb + odd) * p.ldo + (row - odd);
-        if (row_warp + 32 <= p.n) {
-          if (count == 32) {
-            store_queries<OT, PAIR, 0>(v, qs, xs, bias, o, p.ldo, odd, 32);
-          } else {
-            store_queries<OT, PAIR, 1>(v, qs, xs, bias, o, p.ldo, odd, count);
-          }
+        const float row_scale = lost ? __int_as_float(0x7fc00000) : xs[k];
+        const int64_t qb = q0 + q_in;
+        const float* qs = scale + k * 32;
+        const int count = queries - q_in < 32 ? queries - q_in : 32;
+        if constexpr (TMA) {
+          stage_queries<OT>(v, qs, row_scale, bias[k], out_buf, row_in_cta, grp, count, &tm_out,
+                            static_cast<int>(row_cta), static_cast<int>(qb));
         } else {
-          // The last base rows. keep: this lane's pair exists (2), or its
-          // first row alone (1: the last of an odd count), or nothing (0).
-          const int64_t left = p.n - (row - odd);
-          store_ragged<OT, PAIR>(v, qs, xs, bias, o, p.ldo, odd, count,
-                                 left >= 2 ? 2 : left < 0 ? 0 : static_cast<int>(left));
+          // Lanes 2i and 2i + 1 trade 16-bit scores when these leave in pairs:
+          // the even one stores both rows' of query j, the odd one of j + 1.
+          const int odd = PAIR ? lane & 1 : 0;
+          OT* o = out + (qb + odd) * p.ldo + (row - odd);
+          if (row_warp + 32 <= p.n) {
+            if (count == 32) {
+              store_queries<OT, PAIR, 0>(v, qs, row_scale, bias[k], o, p.ldo, odd, 32);
+            } else {
+              store_queries<OT, PAIR, 1>(v, qs, row_scale, bias[k], o, p.ldo, odd, count);
+            }
+          } else {
+            // The last base rows. keep: this lane's pair exists (2), or its
+            // first row alone (1: the last of an odd count), or nothing (0).
+            const int64_t left = p.n - (row - odd);
+            store_ragged<OT, PAIR>(v, qs, row_scale, bias[k], o, p.ldo, odd, count,
+                                   left >= 2 ? 2 : left < 0 ? 0 : static_cast<int>(left));
+          }
         }
       }
-      if (grp >= blocks) {  // nothing to read in this tile
+      if (!freed) {
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
@@ -429,12 +528,9 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         acc = 0;
         acc_phase ^= 1;
       }
-      if (++bt == p.base_tiles) {
-        bt = 0;
-        ++qg;
-        fresh = true;
-      }
+      fresh = advance(qg, bt);
     }
+    if (TMA && quarter == 0 && lane == 0) store_wait();
   }
 
   if (warp == 1 && lane == 0) quiet_wait(done_bar, 0);
@@ -446,12 +542,12 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   if (threadIdx.x == 0 && *s_abort) atomicOr(&g_int8_err, 1u);
 }
 
-template <typename OT, bool PAIR>
+template <typename OT, bool PAIR, bool TMA>
 cudaError_t launch_typed(const CUtensorMap* maps, const Params& p, int clusters, size_t smem, cudaStream_t stream) {
-  auto kern = int8_scores_kernel<OT, PAIR>;
+  auto kern = int8_scores_kernel<OT, PAIR, TMA>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  return launch_after(kern, 2 * clusters, kThreads, smem, stream, maps[0], maps[1], p);
+  return launch_after(kern, 2 * clusters, kThreads, smem, stream, maps[0], maps[1], maps[2], p);
 }
 
 }  // namespace
@@ -468,36 +564,64 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   // Query groups of equal size, a multiple of 32 (the pair's smallest N).
   const int64_t groups = (a.m + 255) / 256;
   p.n_cols = static_cast<int>(((a.m + groups - 1) / groups + 31) / 32 * 32);
-  p.base_tiles = static_cast<int>((a.n + 2 * kRows - 1) / (2 * kRows));
-  // As many accumulators as fit: a tile of few queries is short, and what its
-  // hand-overs take is hidden only by the tiles in flight.
-  p.accs = p.n_cols <= 64 ? 8 : p.n_cols <= 128 ? 4 : 2;
+  // Few queries: several groups of 256 base rows per tile, as many as still
+  // leave two tiles per cluster. Per tile of one slice and 32 queries the MMA
+  // warp's waits and commits take about 1250 clocks, HBM 690.
+  p.subs = p.n_cols <= 64 ? 4 : p.n_cols <= 128 ? 2 : 1;
+  while (p.subs > 1 && (a.n + p.subs * 2 * kRows - 1) / (p.subs * 2 * kRows) * groups < 2 * clusters) p.subs /= 2;
+  p.base_tiles = static_cast<int>((a.n + p.subs * 2 * kRows - 1) / (p.subs * 2 * kRows));
+  p.accs = p.subs * p.n_cols <= 128 ? 4 : 2;
+  // A base that several query groups read, and that L2 (126 MB) can hold beside
+  // what is being written, stays there; otherwise it goes first.
+  p.keep_base = groups > 1 && a.n * a.d <= (int64_t(96) << 20);
   if (groups * p.base_tiles > 0x7fffffff) return cudaErrorInvalidValue;
-  p.tiles = static_cast<int>(groups * p.base_tiles);
+  p.groups = static_cast<int>(groups);
+  // Teams: the most that divide the query groups and leave each cluster eight
+  // tiles or more between changes of its resident queries.
+  const int64_t most = (8 * static_cast<int64_t>(clusters) + p.base_tiles - 1) / p.base_tiles;
+  p.teams = 1;
+  for (int64_t k = 2; k <= most && k <= groups && k <= clusters; ++k)
+    if (groups % k == 0) p.teams = static_cast<int>(k);
+  const int64_t per_team = groups / p.teams * p.base_tiles;
+  p.width = clusters / p.teams;
+  if (p.width > per_team) p.width = static_cast<int>(per_team);
+  clusters = p.teams * p.width;
   p.kc = (a.d + kSlice - 1) / kSlice;
   const int b_slice = p.n_cols / 2 * kSlice;
-  // Resident queries leave at least six ring stages, as many as the bf16
-  // candidate pass has.
-  p.resident = kFixed + static_cast<size_t>(p.kc) * b_slice + 6 * kA <= kSmemLimit;
-  p.stage_bytes = p.resident ? kA : kA + b_slice;
+  const int64_t size = a.type == kElemF32 ? 4 : 2;
+  const bool tma = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo * size % 16 == 0 && a.n * size % 16 == 0 &&
+                   a.ldo * size < (int64_t(1) << 40);
+  const size_t fixed = kFixed + (tma ? kGroups * kOutBuf : 0);
+  // Resident queries leave 80 KB or more of ring: what HBM's latency times an
+  // SM's share of the bandwidth asks for and half more.
+  const int a_bytes = p.subs * kA;
+  p.resident = fixed + static_cast<size_t>(p.kc) * b_slice + (5 / p.subs + 1) * a_bytes <= kSmemLimit;
+  p.stage_bytes = p.resident ? a_bytes : a_bytes + b_slice;
   const size_t b_bytes = p.resident ? static_cast<size_t>(p.kc) * b_slice : 0;
-  const int fit = static_cast<int>((kSmemLimit - kFixed - b_bytes) / p.stage_bytes);
+  const int fit = static_cast<int>((kSmemLimit - fixed - b_bytes) / p.stage_bytes);
   p.stages = fit < kMaxStages ? fit : kMaxStages;
-  const size_t smem = kFixed + b_bytes + static_cast<size_t>(p.stages) * p.stage_bytes;
-  CUtensorMap maps[2];
+  const size_t smem = fixed + b_bytes + static_cast<size_t>(p.stages) * p.stage_bytes;
+  CUtensorMap maps[3];
   cudaError_t e = encode_rows_map(&maps[0], kElemS8, a.x, a.d, a.n, a.ldx, kSlice, kRows, 128);
   if (e == cudaSuccess) e = encode_rows_map(&maps[1], kElemS8, a.q, a.d, a.m, a.ldq, kSlice, p.n_cols / 2, 128);
+  if (e == cudaSuccess && tma)
+    e = encode_rows_map(&maps[2], a.type, a.out, a.n, a.m, a.ldo * size, kRows, size == 4 ? 16 : 32, 0);
+  else
+    maps[2] = maps[0];  // not used
   if (e != cudaSuccess) return e;
-  if (p.tiles < clusters) clusters = p.tiles;
   const bool pair = reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.ldo % 2 == 0;
   switch (a.type) {
-    case kElemF32: return launch_typed<float, false>(maps, p, clusters, smem, stream);
+    case kElemF32:
+      return tma ? launch_typed<float, false, true>(maps, p, clusters, smem, stream)
+                 : launch_typed<float, false, false>(maps, p, clusters, smem, stream);
     case kElemF16:
-      return pair ? launch_typed<__half, true>(maps, p, clusters, smem, stream)
-                  : launch_typed<__half, false>(maps, p, clusters, smem, stream);
+      return tma    ? launch_typed<__half, false, true>(maps, p, clusters, smem, stream)
+             : pair ? launch_typed<__half, true, false>(maps, p, clusters, smem, stream)
+                    : launch_typed<__half, false, false>(maps, p, clusters, smem, stream);
     case kElemBf16:
-      return pair ? launch_typed<__nv_bfloat16, true>(maps, p, clusters, smem, stream)
-                  : launch_typed<__nv_bfloat16, false>(maps, p, clusters, smem, stream);
+      return tma    ? launch_typed<__nv_bfloat16, false, true>(maps, p, clusters, smem, stream)
+             : pair ? launch_typed<__nv_bfloat16, true, false>(maps, p, clusters, smem, stream)
+                    : launch_typed<__nv_bfloat16, false, false>(maps, p, clusters, smem, stream);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -50,33 +50,64 @@ template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<2> { using type = uint16_t; };
 template <> struct Word<1> { using type = uint8_t; };
 
-// A row's scale, and what its values are multiplied by before the division:
-// 2^96 for rows so small that 1 / scale would overflow (a power of two, so
-// nothing is rounded), else 1.
+// The larger of a and |b|; NaN if either is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+
+// A row's scale, and its values' codes.
 struct RowScale {
-  float scale, lift, lifted, inverse;
-  __device__ __forceinline__ explicit RowScale(uint32_t peak_bits) {
-    if (peak_bits >= 0x7f800000u) {  // NaN or infinity in the row
+  float scale, inverse, half, lift;
+  __device__ __forceinline__ explicit RowScale(float peak) {
+    if (!(peak < __int_as_float(0x7f800000))) {  // NaN or infinity in the row
       scale = __int_as_float(0x7fc00000);
-      lift = lifted = inverse = 0.0f;
+      inverse = half = 0.0f;
+      lift = 1.0f;
       return;
     }
-    scale = __fdiv_rn(__uint_as_float(peak_bits), 127.0f);
+    scale = __fdiv_rn(peak, 127.0f);
+    // Rows so small that 1 / scale would overflow are taken times 2^96 (a power
+    // of two, so nothing is rounded).
     lift = scale < 1e-30f ? 0x1p96f : 1.0f;
-    lifted = scale * lift;
-    inverse = lifted > 0.0f ? __frcp_rn(lifted) : 0.0f;
+    inverse = scale > 0.0f ? __frcp_rn(scale * lift) : 0.0f;
+    half = 0.5f * (scale * lift);
   }
+  // x / scale rounded to a whole number, as the low byte of the result's bits
+  // (1.5 * 2^23 + the number), if `off` comes out below `half`; at or above it
+  // the exact quotient may round to a neighbour.
+  __device__ __forceinline__ float near(float x, float& off) const {
+    const float shifted = fmaf(x, inverse, 12582912.0f);
+    // |rest| <= scale * (1/2 + a few ulps): computed without rounding.
+    const float rest = fmaf(-(shifted - 12582912.0f), 2.0f * half, x);
+    off = fmaxf(off, fabsf(rest));
+    return shifted;
+  }
+  // The code itself, for any value.
   __device__ __forceinline__ int code(float x) const {
     if (inverse == 0.0f) return 0;
     const float xs = x * lift;
     float c = rintf(xs * inverse);
-    // |rest| <= scale * (1/2 + a few ulps): exact.
-    const float rest = fmaf(-c, lifted, xs);
-    const float twice = 2.0f * fabsf(rest);
-    if (twice > lifted || (twice == lifted && (__float2int_rn(c) & 1))) c += copysignf(1.0f, rest);
+    const float rest = fmaf(-c, 2.0f * half, xs);
+    const float far = fabsf(rest);
+    if (far > half || (far == half && (__float2int_rn(c) & 1))) c += copysignf(1.0f, rest);
     return __float2int_rn(fminf(fmaxf(c, -127.0f), 127.0f));
   }
 };
+
+// The codes of four values, one per byte. The common case takes an fma, an
+// addition, an fma and a maximum per value; a value at or past a half, or a
+// row that is lifted, goes through code().
+__device__ __forceinline__ uint32_t four_codes(const RowScale& r, const float* x) {
+  float off = 0.0f;
+  const uint32_t a = __float_as_uint(r.near(x[0], off)), b = __float_as_uint(r.near(x[1], off));
+  const uint32_t c = __float_as_uint(r.near(x[2], off)), d = __float_as_uint(r.near(x[3], off));
+  if (off < r.half && r.lift == 1.0f) return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+  uint32_t w = 0;
+  for (int j = 0; j < 4; ++j) w |= static_cast<uint32_t>(r.code(x[j]) & 0xff) << (8 * j);
+  return w;
+}
 
 // VB: bytes per load; NV: loads per lane. A row's values stay in registers, at
 // most 32 per lane.
@@ -94,7 +125,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
   const T* xr = x + (live ? row : 0) * ldx;
   const int nvec = (d + VE - 1) / VE;
   float v[NV][VE];
-  uint32_t peak = 0;
+  float peak = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int at = (i * group + lane) * VE;
@@ -111,8 +142,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < VE; ++j) peak = max(peak, __float_as_uint(v[i][j]) & 0x7fffffffu);
-  for (int s = group >> 1; s > 0; s >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, s));
+    for (int j = 0; j < VE; ++j) peak = max_abs(peak, v[i][j]);
+  for (int s = group >> 1; s > 0; s >>= 1) peak = max_abs(peak, __shfl_xor_sync(0xffffffffu, peak, s));
   if (!live) return;
   const RowScale r(peak);
   if (lane == 0) scales[row] = r.scale;
@@ -124,11 +155,18 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     const int at = vec * VE;
     using C = typename Word<VE>::type;
     if (vec_out && at + VE <= d) {
-      C w;
-      int8_t* e = reinterpret_cast<int8_t*>(&w);
+      if constexpr (VE >= 4) {
+        uint32_t w[VE / 4];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) e[j] = static_cast<int8_t>(r.code(v[i][j]));
-      *reinterpret_cast<C*>(out + at) = w;
+        for (int j = 0; j < VE / 4; ++j) w[j] = four_codes(r, &v[i][4 * j]);
+        *reinterpret_cast<C*>(out + at) = *reinterpret_cast<const C*>(w);
+      } else {
+        C w;
+        int8_t* e = reinterpret_cast<int8_t*>(&w);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) e[j] = static_cast<int8_t>(r.code(v[i][j]));
+        *reinterpret_cast<C*>(out + at) = w;
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < VE; ++j)
@@ -143,19 +181,19 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* __restrict__ x, int64_t n, int d,
                                                                       int64_t ldx, int8_t* __restrict__ codes,
                                                                       int64_t ldc, float* __restrict__ scales) {
-  __shared__ uint32_t s_peak[kThreads / 32];
+  __shared__ float s_peak[kThreads / 32];
   wait_for_previous();
   let_next_start();
   for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
     const T* xr = x + row * ldx;
-    uint32_t peak = 0;
+    float peak = 0.0f;
 #pragma unroll 8
-    for (int j = threadIdx.x; j < d; j += kThreads) peak = max(peak, __float_as_uint(to_f32(__ldg(xr + j))) & 0x7fffffffu);
-    peak = __reduce_max_sync(0xffffffffu, peak);
+    for (int j = threadIdx.x; j < d; j += kThreads) peak = max_abs(peak, to_f32(__ldg(xr + j)));
+    for (int s = 16; s > 0; s >>= 1) peak = max_abs(peak, __shfl_xor_sync(0xffffffffu, peak, s));
     if ((threadIdx.x & 31) == 0) s_peak[threadIdx.x >> 5] = peak;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) peak = max(peak, s_peak[w]);
+    for (int w = 0; w < kThreads / 32; ++w) peak = max_abs(peak, s_peak[w]);
     __syncthreads();
     const RowScale r(peak);
     if (threadIdx.x == 0) scales[row] = r.scale;
