@@ -25,5 +25,6 @@ _ROWS = ("quantize_rows", "dequantize_rows", "int8_scores", "softmax_cross_entro
 def __getattr__(name):
     if name in _ROWS:
         from . import rows
-        return getattr(rows, name)
+        globals().update({n: getattr(rows, n) for n in _ROWS})
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

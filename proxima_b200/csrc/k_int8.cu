@@ -17,12 +17,13 @@
 // where they fit (KC slices of N/2 rows; d <= 896 at N = 256), and only base
 // rows stream through the ring.
 //
-// Order. Neighbouring clusters take neighbouring base tiles of the same query
-// group, so what is written at any time is long runs of 256 rows of `out`:
-// runs of base tiles per cluster, whose writes lie 256 rows x 74 places apart,
-// reach 3.9 TB/s on a 400 MB matrix, neighbouring tiles 5-6. Where the base has
-// few tiles, clusters form teams with query groups of their own, so that the
-// resident queries are not replaced every few tiles.
+// Order. Clusters form teams. The clusters of a team take neighbouring base
+// tiles of one query group, so what is written at any time is long runs of 256
+// rows of `out`: with a run of base tiles per cluster, whose writes lie far
+// apart, plain stores of a 400 MB matrix reach 3.9 TB/s, with neighbouring
+// tiles 5-6. The teams take different query groups at the same base tiles, so
+// that they share what is read from HBM (10k queries against 100k x 768 in two
+// teams read the base 20 times).
 //
 // CTA roles (576 threads): warp 0 TMA producer, warp 1 TMEM owner and (even
 // CTA) MMA issuer, warps 2-17 epilogue: four per TMEM quarter, on alternate
@@ -576,13 +577,16 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   p.keep_base = groups > 1 && a.n * a.d <= (int64_t(96) << 20);
   if (groups * p.base_tiles > 0x7fffffff) return cudaErrorInvalidValue;
   p.groups = static_cast<int>(groups);
-  // Teams: the most that divide the query groups and leave each cluster eight
-  // tiles or more between changes of its resident queries.
-  const int64_t most = (8 * static_cast<int64_t>(clusters) + p.base_tiles - 1) / p.base_tiles;
+  // Teams read the same base tiles at about the same time, so that the base
+  // comes from HBM once per `teams` query groups; teams of eight clusters or
+  // more write runs of 4 KB and more. The most of them that leave 95% of the
+  // clusters busy.
   p.teams = 1;
-  for (int64_t k = 2; k <= most && k <= groups && k <= clusters; ++k)
-    if (groups % k == 0) p.teams = static_cast<int>(k);
-  const int64_t per_team = groups / p.teams * p.base_tiles;
+  for (int64_t k = 2; k <= groups && 8 * k <= clusters; ++k) {
+    const int64_t turns = (groups + k - 1) / k;
+    if (groups * (clusters / k * k) * 100 >= 95 * turns * k * clusters) p.teams = static_cast<int>(k);
+  }
+  const int64_t per_team = (groups + p.teams - 1) / p.teams * p.base_tiles;
   p.width = clusters / p.teams;
   if (p.width > per_team) p.width = static_cast<int>(per_team);
   clusters = p.teams * p.width;
@@ -595,7 +599,7 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   // Resident queries leave 80 KB or more of ring: what HBM's latency times an
   // SM's share of the bandwidth asks for and half more.
   const int a_bytes = p.subs * kA;
-  p.resident = fixed + static_cast<size_t>(p.kc) * b_slice + (5 / p.subs + 1) * a_bytes <= kSmemLimit;
+  p.resident = fixed + static_cast<size_t>(p.kc) * b_slice + ((4 + p.subs) / p.subs) * a_bytes <= kSmemLimit;
   p.stage_bytes = p.resident ? a_bytes : a_bytes + b_slice;
   const size_t b_bytes = p.resident ? static_cast<size_t>(p.kc) * b_slice : 0;
   const int fit = static_cast<int>((kSmemLimit - fixed - b_bytes) / p.stage_bytes);

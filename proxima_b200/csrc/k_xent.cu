@@ -4,8 +4,8 @@
 //     loss_i = log sum_j exp z_ij - z_i,y(i)
 //     G_ij = g_i (exp(z_ij - lse_i) - [j = y(i)]),  dq = scale * G r,  dr = scale * G^T q
 //
-// Forward: one pass over the products, whose epilogue keeps a running maximum
-// and sum per query over the other rows; a second kernel joins them. The
+// Forward: one pass over the products, whose epilogue keeps a running sum of
+// exponentials per query, with its scale, over the other rows; a second kernel joins them. The
 // target's own logit stays out of the sum, so the loss is
 //     softplus(log sum_{j != y} exp z_ij - z_iy),
 // which does not cancel when the target holds nearly all of the softmax. z_iy
@@ -47,7 +47,9 @@
 // Bound: the tensor pipe for d >= 256 or so (2 t v d operations forward, three
 // times that backward, of which the logits again are the price of not keeping
 // them); the forward at small d by the exponentials (one per logit, 16 per SM
-// and clock).
+// and clock: 2048 clocks per tile against 512 per slice of products). Computing
+// a quarter or three eighths of them by a polynomial on the FMA pipe was slower
+// (1000 x 1M x 128: 374 and 396 us against 351): issue slots run short.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -74,6 +76,10 @@ constexpr int kOutBuf = 2048;  // staging of an epilogue warp's stores: 32 rows 
 constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 1;
 constexpr size_t kSmem = 1024 + kSlots * kSlot + kEpiWarps * kOutBuf + kBars * 8 + 16;
 constexpr int kHits = 4;     // most queries that share a target for its correction in dr
+// A running sum is kept relative to 2^base, base the largest logit of the
+// first block; a block whose sum passes kRaise (or is NaN) raises it. Between,
+// no maximum is needed: fp32 holds sums of 2^60 as exactly as sums of 1.
+constexpr float kRaise = 0x1p60f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
@@ -108,14 +114,14 @@ struct Args {
   int keep;              // logits: query slices kept in shared memory
   int v0;                // first base row of the piece
   int piece;             // its columns
-  int lists;             // kStats: (max, sum) pairs per query
+  int lists;             // kStats: (base, sum) pairs per query
   uint32_t idesc, idesc2;  // of the first 256 columns, and of the rest
   float c;               // scale * log2(e)
   float scale;
   const float* bias;
   const int64_t* targets;
   int64_t ignore_index;
-  float2* part;          // kStats: [t][lists] (max, sum), log2 units
+  float2* part;          // kStats: [t][lists] (base, sum): sum * 2^base
   unsigned* counter;     // kStats: cleared for the joining kernel
   RowGrad row;           // kWeights, kGradRows
   float* rest;           // kWeights writes, kGradRows reads: [t] what rounding took from the target's entry
@@ -138,7 +144,12 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -197,25 +208,29 @@ __device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
   const float b1 = max3(a[3], a[4], a[5]);
   const float b2 = max3(a[6], a[7], a[8]);
   const float b3 = max3(a[9], __uint_as_float(v[30]), __uint_as_float(v[31]));
-  return fmaxf(max3(b0, b1, b2), b3);
+  return max2(max3(b0, b1, b2), b3);
+}
+
+// The sum of 2^(c * v - base) over a block of 32 logits.
+__device__ __forceinline__ float block_sum(const uint32_t (&v)[32], float c, float base) {
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(__uint_as_float(v[j]), c, -base));
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // Adds the bias: v becomes c * v + bias * log2(e), log2 units. Columns past
 // the base count as left out.
 __device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, int left, float c) {
-  const F2 cc = f2(c, c), le = f2(kLog2e, kLog2e);
   if (left >= 32) {
     const float4* b4 = reinterpret_cast<const float4*>(bias);
 #pragma unroll
     for (int j4 = 0; j4 < 8; ++j4) {
       const float4 b = __ldg(b4 + j4);
-      float x, y;
-      unpack(fma2(f2(__uint_as_float(v[4 * j4]), __uint_as_float(v[4 * j4 + 1])), cc, mul2(f2(b.x, b.y), le)), x, y);
-      v[4 * j4] = __float_as_uint(x);
-      v[4 * j4 + 1] = __float_as_uint(y);
-      unpack(fma2(f2(__uint_as_float(v[4 * j4 + 2]), __uint_as_float(v[4 * j4 + 3])), cc, mul2(f2(b.z, b.w), le)), x, y);
-      v[4 * j4 + 2] = __float_as_uint(x);
-      v[4 * j4 + 3] = __float_as_uint(y);
+      v[4 * j4] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4]), c, b.x * kLog2e));
+      v[4 * j4 + 1] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 1]), c, b.y * kLog2e));
+      v[4 * j4 + 2] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 2]), c, b.z * kLog2e));
+      v[4 * j4 + 3] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 3]), c, b.w * kLog2e));
     }
   } else {
 #pragma unroll
@@ -567,14 +582,14 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     int m_now = -1;
     // kStats / kWeights: the query's state.
     int target = -1;
-    float run_max = -kInf, run_sum = 0.0f;
+    float run_base = -kInf, run_sum = 0.0f;
     float lse2 = 0.0f, factor = 0.0f, at_target = 0.0f;
-    auto flush = [&]() {  // kStats: this pair's (max, sum) of query tile m_now
+    auto flush = [&]() {  // kStats: this pair's (base, sum) of query tile m_now
       const int64_t q = static_cast<int64_t>(m_now) * kTile + row_in_pair;
       if (q < p.t) {
         const int slot = cluster - run_of(p.tiles, static_cast<int64_t>(m_now) * p.n_tiles, nclusters);
         p.part[q * p.lists + slot * kGroups + group] =
-            make_float2(BIAS || run_max == -kInf ? run_max : run_max * p.c, lost ? __int_as_float(0x7fc00000) : run_sum);
+            make_float2(run_base, lost ? __int_as_float(0x7fc00000) : run_sum);
       }
     };
     for (int i = first; i < last; i += step) {
@@ -593,7 +608,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       if (S::LOGITS && m != m_now) {
         if (ROLE == kStats && m_now >= 0) flush();
         m_now = m;
-        run_max = -kInf;
+        run_base = -kInf;
         run_sum = 0.0f;
         target = -1;
         factor = 0.0f;
@@ -656,34 +671,25 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                 if (j == at) v[j] = __float_as_uint(-kInf);
             }
             const float c = BIAS ? 1.0f : p.c;
-            const float top = fmaxf(run_max, largest(v));
-            const float base = top == -kInf ? 0.0f : top * c;
-            const F2 cc = f2(c, c), minus = f2(-base, -base);
-            const float carry = run_sum * ex2(fmaf(run_max, c, -base));
-            F2 s[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float x, y;
-              unpack(fma2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), cc, minus), x, y);
-              s[(j >> 1) & 1] = add2(s[(j >> 1) & 1], f2(ex2(x), ex2(y)));
+            const float sum = block_sum(v, c, run_base);
+            if (run_base != -kInf && sum < kRaise) {
+              run_sum += sum;
+            } else {
+              const float top = largest(v) * c;
+              if (top != -kInf) {  // something takes part (or is NaN)
+                run_sum = run_sum * ex2(run_base - top) + block_sum(v, c, top);
+                run_base = top;
+              }
             }
-            float x, y;
-            unpack(add2(s[0], s[1]), x, y);
-            run_sum = carry + (x + y);
-            run_max = top;
           }
           if (ROLE == kWeights) {
             if (BIAS) add_bias(v, p.bias + p.v0 + col, static_cast<int>(p.v) - p.v0 - col, p.c);
             const float c = BIAS ? 1.0f : p.c;
-            const F2 cc = f2(c, c), minus = f2(-lse2, -lse2), ff = f2(factor, factor);
             uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float x, y;
-              unpack(fma2(f2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), cc, minus), x, y);
-              unpack(mul2(f2(ex2(x), ex2(y)), ff), x, y);
-              w[j] = pack2<BF>(x, y);
-            }
+            for (int j = 0; j < 16; ++j)
+              w[j] = pack2<BF>(ex2(fmaf(__uint_as_float(v[2 * j]), c, -lse2)) * factor,
+                               ex2(fmaf(__uint_as_float(v[2 * j + 1]), c, -lse2)) * factor);
             if (at >= 0 && at < 32) {
               p.rest[row] = at_target - rounded<BF>(at_target);
               if (p.hits != nullptr) {
@@ -829,7 +835,7 @@ struct JoinArgs {
   unsigned* counter;
 };
 
-// One warp per query: joins the pairs' (max, sum), forms the target's logit
+// One warp per query: joins the pairs' (base, sum), forms the target's logit
 // and the loss. The last block to finish sums the losses, in 64 bits and a
 // fixed order.
 template <bool BF>
@@ -1035,7 +1041,7 @@ int stats_pairs(int64_t m_tiles, int64_t n_tiles, int clusters) {
   return static_cast<int>(even * 10 >= clusters * 9 ? even : clusters);
 }
 
-// (max, sum) pairs per query: those of the most CTA pairs that share a query
+// (base, sum) pairs per query: those of the most CTA pairs that share a query
 // tile.
 int stats_lists(int64_t m_tiles, int64_t n_tiles, int pairs) {
   int most = 1;

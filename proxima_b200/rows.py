@@ -59,6 +59,8 @@ def _plain(a):
 def _empty_rows(n: int, dim: int, dtype, device):
     """An n x dim tensor whose rows start on 16-byte boundaries."""
     unit = 16 // dtype.itemsize
+    if dim % unit == 0:
+        return torch.empty((n, dim), dtype=dtype, device=device)
     return torch.empty((n, (dim + unit - 1) // unit * unit), dtype=dtype, device=device)[:, :dim]
 
 
@@ -86,8 +88,10 @@ def _ptr(a):
     return None if a is None else a.data_ptr()
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _stream(index: int) -> int:
+    """The current stream of a device (what torch.cuda.current_stream's
+    cuda_stream gives, without making a Stream object for it)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def quantize_rows(x):
@@ -98,14 +102,15 @@ def quantize_rows(x):
     boundaries, as ``int8_scores`` reads them. A row of zeros has scale 0; a
     row with a NaN or an infinity has scale NaN and codes 0."""
     _check(x, "x", 2, tuple(_TYPES))
-    n, dim = x.shape[0], _dim(x, "x")
-    x = _plain(x.detach())
-    codes = _empty_rows(n, dim, torch.int8, x.device)
-    scales = torch.empty(n, dtype=torch.float32, device=x.device)
+    n, dim, dev = x.shape[0], _dim(x, "x"), x.device
+    x = _plain(x)
+    codes = _empty_rows(n, dim, torch.int8, dev)
+    scales = torch.empty(n, dtype=torch.float32, device=dev)
     if n:
+        index = dev.index
         _lib.check(_lib.load().px_quantize_rows_device(
-            x.device.index, x.data_ptr(), _TYPES[x.dtype], n, dim, _ld(x), codes.data_ptr(), codes.stride(0),
-            scales.data_ptr(), _stream(x.device)))
+            index, x.data_ptr(), _TYPES[x.dtype], n, dim, _ld(x), codes.data_ptr(), codes.stride(0),
+            scales.data_ptr(), _stream(index)))
     return codes, scales
 
 
@@ -125,7 +130,7 @@ def dequantize_rows(codes, scales, dtype=torch.float32):
     if n:
         _lib.check(_lib.load().px_dequantize_rows_device(
             codes.device.index, codes.data_ptr(), _ld(codes), scales.data_ptr(), n, dim, _TYPES[dtype],
-            out.data_ptr(), dim, _stream(codes.device)))
+            out.data_ptr(), dim, _stream(codes.device.index)))
     return out
 
 
@@ -174,50 +179,63 @@ def int8_scores(q_codes, q_scales, codes, scales, bias=None, dtype=torch.float32
         b = None if bias is None else bias.contiguous()
         _lib.check(_lib.load().px_int8_scores_device(
             dev.index, qc.data_ptr(), ldq, qs.data_ptr(), m, xc.data_ptr(), ldx, xs.data_ptr(), n, dim, _ptr(b),
-            _TYPES[dtype], out.data_ptr(), _ld(out), _stream(dev)))
+            _TYPES[dtype], out.data_ptr(), _ld(out), _stream(dev.index)))
     return out
+
+
+def _xent_forward(queries, rows, targets, scale, bias, ignore_index, reduction):
+    """The loss, and what the backward needs: the operands as the tensor cores
+    read them, and the buffer that holds each query's loss and lse and the
+    reduction's divisor."""
+    lib, dev = _lib.load(), queries.device
+    (t, dim), v, index = queries.shape, rows.shape[0], dev.index
+    q, ldq = _tiled(queries)
+    r, ldr = _tiled(rows)
+    targets, bias = targets.contiguous(), _aligned(bias)
+    part = (4 * t + 255) // 256 * 256  # bytes of one float per query
+    need = lib.px_softmax_xent_workspace_bytes(index, t, v, dim, 0)
+    kept = torch.empty(2 * part + 256, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    out = torch.empty(() if reduction else t, dtype=torch.float32, device=dev)
+    base = kept.data_ptr()
+    loss = base if reduction else out.data_ptr()
+    _lib.check(lib.px_softmax_xent_device(
+        index, q.data_ptr(), ldq, t, r.data_ptr(), ldr, v, dim, _TYPES[q.dtype], targets.data_ptr(), ignore_index, scale,
+        _ptr(bias), reduction, loss, base + part, out.data_ptr() if reduction else None,
+        base + 2 * part if reduction else None, ws.data_ptr(), need, _stream(index)))
+    return out, (q, ldq, r, ldr, targets, bias, kept, part)
 
 
 class _SoftmaxCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, rows, targets, scale, bias, ignore_index, reduction):
-        lib, dev = _lib.load(), queries.device
-        (t, dim), v = queries.shape, rows.shape[0]
-        q, ldq = _tiled(queries)
-        r, ldr = _tiled(rows)
-        targets, bias = targets.contiguous(), _aligned(bias)
-        loss = torch.empty(t, dtype=torch.float32, device=dev)
-        lse = torch.empty_like(loss)
-        total = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
-        divisor = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
-        ws = torch.empty(lib.px_softmax_xent_workspace_bytes(dev.index, t, v, dim, 0), dtype=torch.uint8, device=dev)
-        _lib.check(lib.px_softmax_xent_device(
-            dev.index, q.data_ptr(), ldq, t, r.data_ptr(), ldr, v, dim, _TYPES[q.dtype], targets.data_ptr(),
-            ignore_index, scale, _ptr(bias), reduction, loss.data_ptr(), lse.data_ptr(), _ptr(total), _ptr(divisor),
-            ws.data_ptr(), ws.numel(), _stream(dev)))
-        ctx.save_for_backward(q, r, targets, bias, loss, lse, divisor)
-        ctx.args = (ldq, ldr, scale, ignore_index, reduction)
-        return total if reduction else loss
+        out, (q, ldq, r, ldr, targets, bias, kept, part) = _xent_forward(queries, rows, targets, scale, bias,
+                                                                         ignore_index, reduction)
+        ctx.save_for_backward(q, r, targets, bias, kept, None if reduction else out)
+        ctx.args = (ldq, ldr, part, scale, ignore_index, reduction)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         lib = _lib.load()
-        q, r, targets, bias, loss, lse, divisor = ctx.saved_tensors
-        ldq, ldr, scale, ignore_index, reduction = ctx.args
+        q, r, targets, bias, kept, out = ctx.saved_tensors
+        ldq, ldr, part, scale, ignore_index, reduction = ctx.args
         (t, dim), v, dev = q.shape, r.shape[0], q.device
+        index = dev.index
         want_q, want_r = ctx.needs_input_grad[:2]
         dq = torch.empty((t, dim), dtype=q.dtype, device=dev) if want_q else None
         dr = torch.empty((v, dim), dtype=r.dtype, device=dev) if want_r else None
         stride = 0 if reduction or (t > 1 and grad.stride(0) == 0) else 1
         if stride:
             grad = grad.contiguous()
-        ws = torch.empty(lib.px_softmax_xent_workspace_bytes(dev.index, t, v, dim, 1), dtype=torch.uint8, device=dev)
+        base = kept.data_ptr()
+        need = lib.px_softmax_xent_workspace_bytes(index, t, v, dim, 1)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _lib.check(lib.px_softmax_xent_backward_device(
-            dev.index, q.data_ptr(), ldq, t, r.data_ptr(), ldr, v, dim, _TYPES[q.dtype], targets.data_ptr(),
-            ignore_index, scale, _ptr(bias), loss.data_ptr(), lse.data_ptr(), grad.data_ptr(), stride,
-            _ptr(divisor), _ptr(dq), dim, _ptr(dr), dim, ws.data_ptr(), ws.numel(),
-            _stream(dev)))
+            index, q.data_ptr(), ldq, t, r.data_ptr(), ldr, v, dim, _TYPES[q.dtype], targets.data_ptr(), ignore_index,
+            scale, _ptr(bias), base if reduction else out.data_ptr(), base + part, grad.data_ptr(), stride,
+            base + 2 * part if reduction else None, _ptr(dq), dim, _ptr(dr), dim, ws.data_ptr(), need, _stream(index)))
         return dq, dr, None, None, None, None, None
 
 
@@ -260,7 +278,10 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
         # No query: an empty loss, or the sum or mean of one, with zero gradients.
         loss = (queries.float().sum(1) + 0.0 * rows[:1].float().sum())
         return {"none": lambda: loss, "sum": loss.sum, "mean": loss.mean}[reduction]()
-    return _SoftmaxCrossEntropy.apply(queries, rows, targets, scale, bias, int(ignore_index), _REDUCTIONS[reduction])
+    args = (queries, rows, targets, scale, bias, int(ignore_index), _REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (queries.requires_grad or rows.requires_grad):
+        return _SoftmaxCrossEntropy.apply(*args)
+    return _xent_forward(*args)[0]
 
 
 def rows_status(device=None) -> None:
@@ -268,4 +289,4 @@ def rows_status(device=None) -> None:
     a bounded device-side wait of one of these operators has given up since
     the last call; the results it left undone are NaN."""
     device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index)
-    _lib.check(_lib.load().px_rows_status_device(device.index, _stream(device)))
+    _lib.check(_lib.load().px_rows_status_device(device.index, _stream(device.index)))
