@@ -112,6 +112,7 @@ struct Args {
   int n_cols;            // N of a tile: 256 (logits), else a multiple of 32 up to 512
   int k_slices;
   int keep;              // logits: query slices kept in shared memory
+  int per_slot;          // logits: K slices of the base per ring slot, 1 or 2
   int v0;                // first base row of the piece
   int piece;             // its columns
   int lists;             // kStats: (base, sum) pairs per query
@@ -211,12 +212,24 @@ __device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
   return max2(max3(b0, b1, b2), b3);
 }
 
-// The sum of 2^(c * v - base) over a block of 32 logits.
+// The sum of 2^(c * v - base) over a block.
 __device__ __forceinline__ float block_sum(const uint32_t (&v)[32], float c, float base) {
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(__uint_as_float(v[j]), c, -base));
   return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// Logit `at`, or those from `from` on, leave a block.
+__device__ __forceinline__ void leave_out(uint32_t (&v)[32], int at) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j == at) v[j] = __float_as_uint(-kInf);
+}
+__device__ __forceinline__ void leave_out_from(uint32_t (&v)[32], int from) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j >= from) v[j] = __float_as_uint(-kInf);
 }
 
 // Adds the bias: v becomes c * v + bias * log2(e), log2 units. Columns past
@@ -395,7 +408,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   // The first `keep` slots of shared memory hold kept query slices, the rest
   // are the ring.
   const int keep = S::LOGITS ? p.keep : 0;
-  const int ring = kSlots - keep;
+  const int per = S::LOGITS ? p.per_slot : 1;  // slices per ring slot
+  const int slot_bytes = per * kSlot;
+  const int ring = (kSlots - keep) / per;
   const uint32_t ring_base = smem_base + keep * kSlot;
   // An MN-major B tile: the columns of the first MMA (up to 256) and of the
   // second, in boxes of 64 per CTA.
@@ -415,7 +430,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       // The next ring slot, armed for both CTAs' bytes; 0 when a wait gave up.
       auto next_slot = [&](uint32_t bytes, uint32_t& fb) -> uint32_t {
         if (!tc::mbar_wait(empty_bar(slot), phase ^ 1, s_abort)) return 0;
-        const uint32_t dst = ring_base + slot * kSlot;
+        const uint32_t dst = ring_base + slot * slot_bytes;
         fb = tc::mapa_shared(full_bar(slot), 0);
         if (leader) tc::mbar_arrive_expect_tx(full_bar(slot), 2 * bytes);
         ++loads;
@@ -439,13 +454,15 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             kept = m;
             ++keeps;
           }
-          for (int k = 0; k < p.k_slices; ++k) {
+          for (int k = 0; k < p.k_slices; k += per) {
             if (k >= keep) {
               if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
               tc::tma_load_2d_pair(dst, &tm_a, fb, k * kSlice, m0);
             }
-            if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
-            tc::tma_load_2d_pair(dst, &tm_b, fb, k * kSlice, n0);
+            const int count = min(per, p.k_slices - k);
+            if ((dst = next_slot(count * kSlot, fb)) == 0) { ok = false; break; }
+            for (int i2 = 0; i2 < count; ++i2)
+              tc::tma_load_2d_pair(dst + i2 * kSlot, &tm_b, fb, (k + i2) * kSlice, n0);
           }
         } else {
           const Item it = item_of<ROLE>(p, i);
@@ -525,22 +542,28 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           k1 = it.k1;
         }
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kTile);
-        for (int k = k0; k < k1; ++k) {
+        for (int k = k0; k < k1; k += per) {
           int slot_a = -1, slot_b = -1, slot_c = -1;
           const bool streamed = !S::LOGITS || k >= keep;
           if (streamed && !next_slot(slot_a)) { ok = false; break; }
           if (!next_slot(slot_b)) { ok = false; break; }
           if (n_second > 0 && !next_slot(slot_c)) { ok = false; break; }
           tc::tc_fence_after();
-          const uint32_t a_at = (streamed ? ring_base + slot_a * kSlot : smem_base + k * kSlot) >> 4;
+          const uint32_t a_at = (streamed ? ring_base + slot_a * slot_bytes : smem_base + k * kSlot) >> 4;
           const uint64_t a_desc = a_kind + a_at;
-          const uint64_t b_desc = b_kind + ((ring_base + slot_b * kSlot) >> 4);
-          const uint64_t c_desc = b_kind + ((ring_base + slot_c * kSlot) >> 4);
+          const uint64_t b_desc = b_kind + ((ring_base + slot_b * slot_bytes) >> 4);
+          const uint64_t c_desc = b_kind + ((ring_base + slot_c * slot_bytes) >> 4);
           const uint32_t more = k > k0 ? 1u : 0u;
           if (issuer) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               tc::mma_bf16_pair(d_tmem, a_desc + kk * kAStep, b_desc + kk * kBStep, p.idesc, kk > 0 ? 1u : more);
+            if (S::LOGITS && per > 1 && k + 1 < k1) {  // the slot's second slice, against the next kept one
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                tc::mma_bf16_pair(d_tmem, a_desc + (kSlot >> 4) + kk * kAStep, b_desc + (kSlot >> 4) + kk * kBStep,
+                                  p.idesc, 1u);
+            }
             if (S::B_MN && n_second > 0) {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
@@ -583,7 +606,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     // kStats / kWeights: the query's state.
     int target = -1;
     float run_base = -kInf, run_sum = 0.0f;
-    float lse2 = 0.0f, factor = 0.0f, at_target = 0.0f;
+    float shift = -kInf, factor = 0.0f, at_target = 0.0f;
     auto flush = [&]() {  // kStats: this pair's (base, sum) of query tile m_now
       const int64_t q = static_cast<int64_t>(m_now) * kTile + row_in_pair;
       if (q < p.t) {
@@ -617,9 +640,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           const bool used = counts(y, p.ignore_index, p.v);
           if (used) target = static_cast<int>(y) - p.v0;
           if (ROLE == kWeights) {
+            // G = factor * 2^(logit - lse) = +-2^(logit + shift); no row takes part
+            // where lse is -inf.
             const float l = __ldg(p.row.lse + row);
-            lse2 = l == -kInf ? kInf : l * kLog2e;
             factor = row_factor(p.row, used, row);
+            shift = l == -kInf || factor == 0.0f ? -kInf : log2f(fabsf(factor)) - l * kLog2e;
             at_target = target_entry(p.row, row, factor);
           }
         }
@@ -641,55 +666,104 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       }
       if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
       tc::tc_fence_after();
+      if (ROLE == kStats) {
+        // This warp's 64 columns.
+        const int col = n * kTile + group * 64;
+        const int left = static_cast<int>(p.v) - col;
+        const bool some = row_warp < p.t && left > 0;
+        const uint32_t at_tmem = lane_addr + static_cast<uint32_t>(acc * kTile + group * 64);
+        // The columns are in registers: the accumulator is free.
+        auto release = [&]() {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+        };
+        auto take = [&](uint32_t (&v)[32], int first_col) {
+          const int here = static_cast<int>(p.v) - first_col;
+          if (BIAS) {
+            add_bias(v, p.bias + first_col, here, p.c);
+          } else if (here < 32) {
+            leave_out_from(v, here);
+          }
+          // The target's logit stays out of the sum.
+          const int at = target - first_col;
+          if (at >= 0 && at < 32) leave_out(v, at);
+          const float c = BIAS ? 1.0f : p.c;
+          const float sum = block_sum(v, c, run_base);
+          if (run_base != -kInf && sum < kRaise) {
+            run_sum += sum;
+          } else {
+            const float top = largest(v) * c;
+            if (top != -kInf) {  // something takes part (or is NaN)
+              run_sum = run_sum * ex2(run_base - top) + block_sum(v, c, top);
+              run_base = top;
+            }
+          }
+        };
+        if (some && lost) run_sum = __int_as_float(0x7fc00000);
+        if (!some) {
+          release();
+        } else if (BIAS) {  // the bias's registers leave room for one half
+          uint32_t v[32];
+          __syncwarp();
+          tc::tmem_ld_32x32b_x32(at_tmem, v);
+          tc::tmem_ld_wait();
+          take(v, col);
+          __syncwarp();
+          tc::tmem_ld_32x32b_x32(at_tmem + 32, v);
+          tc::tmem_ld_wait();
+          release();
+          if (left > 32) take(v, col + 32);
+        } else {
+          uint32_t lo[32], hi[32];
+          __syncwarp();
+          tc::tmem_ld_32x32b_x32(at_tmem, lo);
+          tc::tmem_ld_32x32b_x32(at_tmem + 32, hi);
+          tc::tmem_ld_wait();
+          release();
+          take(lo, col);
+          if (left > 32) take(hi, col + 32);
+        }
+        if (++acc == accs) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+        continue;
+      }
       const int64_t rows = ROLE == kGradRows ? p.piece : p.t;
+      bool freed = false;
       if (row_warp < rows) {
         for (int b = group; b * 32 < p.n_cols; b += kGroups) {
           const int col = n * p.n_cols + b * 32;  // within the product
-          const int cols = ROLE == kStats ? static_cast<int>(p.v) : ROLE == kWeights ? p.piece : p.d;
+          const int cols = ROLE == kWeights ? p.piece : p.d;
           if (col >= cols) break;
           __syncwarp();
           uint32_t v[32];
           tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * kTile + b * 32), v);
           tc::tmem_ld_wait();
+          if ((b + kGroups) * 32 >= p.n_cols || col + kGroups * 32 >= cols) {
+            // The warp's last columns are in registers: the accumulator is free.
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+            freed = true;
+          }
           if (lost) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
           }
           const int at = target - col;  // the target's place in the block
-          if (ROLE == kStats) {
-            const int left = cols - col;
-            if (BIAS) {
-              add_bias(v, p.bias + col, left, p.c);
-            } else if (left < 32) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j >= left) v[j] = __float_as_uint(-kInf);
-            }
-            if (at >= 0 && at < 32) {  // the target's logit stays out of the sum
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j == at) v[j] = __float_as_uint(-kInf);
-            }
-            const float c = BIAS ? 1.0f : p.c;
-            const float sum = block_sum(v, c, run_base);
-            if (run_base != -kInf && sum < kRaise) {
-              run_sum += sum;
-            } else {
-              const float top = largest(v) * c;
-              if (top != -kInf) {  // something takes part (or is NaN)
-                run_sum = run_sum * ex2(run_base - top) + block_sum(v, c, top);
-                run_base = top;
-              }
-            }
-          }
           if (ROLE == kWeights) {
             if (BIAS) add_bias(v, p.bias + p.v0 + col, static_cast<int>(p.v) - p.v0 - col, p.c);
             const float c = BIAS ? 1.0f : p.c;
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              w[j] = pack2<BF>(ex2(fmaf(__uint_as_float(v[2 * j]), c, -lse2)) * factor,
-                               ex2(fmaf(__uint_as_float(v[2 * j + 1]), c, -lse2)) * factor);
+              w[j] = pack2<BF>(ex2(fmaf(__uint_as_float(v[2 * j]), c, shift)), ex2(fmaf(__uint_as_float(v[2 * j + 1]), c, shift)));
+            if (factor < 0.0f) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] ^= 0x80008000u;
+            }
             if (at >= 0 && at < 32) {
               p.rest[row] = at_target - rounded<BF>(at_target);
               if (p.hits != nullptr) {
@@ -772,9 +846,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           }
         }
       }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+      if (!freed) {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+      }
       if (++acc == accs) {
         acc = 0;
         acc_phase ^= 1;
@@ -1177,6 +1253,9 @@ void logits_args(Args& p, bool bf, int m_tiles, int n_tiles) {
   p.n_cols = kTile;
   p.k_slices = static_cast<int>(ceil_div(p.d, kSlice));
   p.keep = least(p.k_slices, kKeep);
+  // Two slices per slot where the ring still holds three: half the waits and
+  // commits of a short tile.
+  p.per_slot = p.k_slices <= 6 ? 2 : 1;
   p.idesc = p.idesc2 = tc::idesc_16(bf, false, false, kTile, kTile);
 }
 
