@@ -66,14 +66,15 @@ __device__ unsigned g_xent_err;
 constexpr int kHalf = 128;   // M rows per CTA (TMEM lanes)
 constexpr int kTile = 256;   // M rows per pair; N columns of a logits tile
 constexpr int kSlice = 64;   // K values per slice: 128 bytes
-constexpr int kSlots = 12;
+constexpr int kSlots = 12;       // 16 KB each; the forward stages no stores and has
+constexpr int kStatsSlots = 14;  // their 32 KB for slots too
 constexpr int kSlot = kHalf * 128;  // 16 KB
 constexpr int kKeep = 7;     // query slices kept in shared memory at most
 constexpr int kGroups = 4;   // epilogue warps per TMEM quarter
 constexpr int kEpiWarps = 4 * kGroups;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kOutBuf = 2048;  // staging of an epilogue warp's stores: 32 rows of 64 bytes
-constexpr int kBars = 2 * kSlots + 2 + 2 + 2 + 1;
+constexpr int kBars = 2 * kStatsSlots + 2 + 2 + 2 + 1;
 constexpr size_t kSmem = 1024 + kSlots * kSlot + kEpiWarps * kOutBuf + kBars * 8 + 16;
 constexpr int kHits = 4;     // most queries that share a target for its correction in dr
 // A running sum is kept relative to 2^base, base the largest logit of the
@@ -90,6 +91,7 @@ template <int ROLE> struct Shape {
   static constexpr bool LOGITS = ROLE == kStats || ROLE == kWeights;
   static constexpr bool A_MN = ROLE == kGradRows;
   static constexpr bool B_MN = !LOGITS;
+  static constexpr int SLOTS = ROLE == kStats ? kStatsSlots : kSlots;
 };
 
 // What the backward derives a query's G from.
@@ -102,6 +104,8 @@ struct RowGrad {
   int grad_stride;
   float lift;
 };
+
+static_assert(kStatsSlots * kSlot == kSlots * kSlot + kEpiWarps * kOutBuf, "one shared-memory layout");
 
 struct Args {
   int64_t t, v;
@@ -129,11 +133,13 @@ struct Args {
   int* hits;             // [piece] how many queries have the base row as target (or null)
   int4* hit_list;        // [piece] the first kHits of them
   int* next_hits;        // kGradRows: cleared for the next piece
-  const uint16_t* q;     // kGradRows
-  int64_t ldq;
-  int accumulate;        // kGradQ
-  uint16_t* out;         // kGradRows: the base's gradient, where TMA cannot store it
+  const uint16_t* other; // the gradients' other operand: the rows corrections are taken from
+  int64_t ldother;
+  int accumulate;        // kGradQ: to what its slabs hold
+  int direct;            // kGradQ: one piece in one split, so the product is the gradient
+  uint16_t* out;         // the gradient, where TMA cannot store it
   int64_t ldo;
+  int out_row0;          // its row of the product's first
   int tma_out;
 };
 
@@ -317,6 +323,30 @@ __device__ __forceinline__ int4 in_order(int4 a, int n) {
   return a;
 }
 
+// Adds f times a row of 16-bit values (32 of them, or the `left` there are) to
+// a block.
+template <bool BF>
+__device__ __forceinline__ void add_row(uint32_t (&v)[32], float f, const uint16_t* x, int left) {
+  if (left >= 32) {
+    const uint4* x4 = reinterpret_cast<const uint4*>(x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint4 a = __ldg(x4 + k);
+      const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 p = widen2<BF>(u[j]);
+        v[8 * k + 2 * j] = __float_as_uint(fmaf(f, p.x, __uint_as_float(v[8 * k + 2 * j])));
+        v[8 * k + 2 * j + 1] = __float_as_uint(fmaf(f, p.y, __uint_as_float(v[8 * k + 2 * j + 1])));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) v[j] = __float_as_uint(fmaf(f, widen2<BF>(__ldg(x + j)).x, __uint_as_float(v[j])));
+  }
+}
+
 // Gradient item i: M tile, N tile, K slices [k0, k1).
 struct Item {
   int m, n, split, k0, k1;
@@ -360,15 +390,15 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   const bool leader = rank == 0;
   const uint32_t smem_base = tc::smem_addr(smem);
   auto full_bar = [&](int s) { return tc::smem_addr(&bars[s]); };
-  auto empty_bar = [&](int s) { return tc::smem_addr(&bars[kSlots + s]); };
-  auto tfull_bar = [&](int a) { return tc::smem_addr(&bars[2 * kSlots + a]); };
-  auto tempty_bar = [&](int a) { return tc::smem_addr(&bars[2 * kSlots + 2 + a]); };
-  const uint32_t kfull_bar = tc::smem_addr(&bars[2 * kSlots + 4]);   // kept query slices loaded
-  const uint32_t kempty_bar = tc::smem_addr(&bars[2 * kSlots + 5]);  // and no longer read
-  const uint32_t done_bar = tc::smem_addr(&bars[2 * kSlots + 6]);
+  auto empty_bar = [&](int s) { return tc::smem_addr(&bars[kStatsSlots + s]); };
+  auto tfull_bar = [&](int a) { return tc::smem_addr(&bars[2 * kStatsSlots + a]); };
+  auto tempty_bar = [&](int a) { return tc::smem_addr(&bars[2 * kStatsSlots + 2 + a]); };
+  const uint32_t kfull_bar = tc::smem_addr(&bars[2 * kStatsSlots + 4]);   // kept query slices loaded
+  const uint32_t kempty_bar = tc::smem_addr(&bars[2 * kStatsSlots + 5]);  // and no longer read
+  const uint32_t done_bar = tc::smem_addr(&bars[2 * kStatsSlots + 6]);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) {
+    for (int s = 0; s < S::SLOTS; ++s) {
       tc::mbar_init(full_bar(s), 1);
       tc::mbar_init(empty_bar(s), 1);
     }
@@ -410,7 +440,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   const int keep = S::LOGITS ? p.keep : 0;
   const int per = S::LOGITS ? p.per_slot : 1;  // slices per ring slot
   const int slot_bytes = per * kSlot;
-  const int ring = (kSlots - keep) / per;
+  const int ring = (S::SLOTS - keep) / per;
   const uint32_t ring_base = smem_base + keep * kSlot;
   // An MN-major B tile: the columns of the first MMA (up to 256) and of the
   // second, in boxes of 64 per CTA.
@@ -664,6 +694,14 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         }
         n_hits = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n_hits));
       }
+      if (ROLE == kGradQ && p.direct) {
+        final_scale = out_scale(p.row, p.scale);
+        if (row < p.t) {
+          const int64_t y = __ldg(p.targets + row);
+          if (counts(y, p.ignore_index, p.v)) hits.x = static_cast<int>(y);
+        }
+        n_hits = 1;
+      }
       if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
       tc::tc_fence_after();
       if (ROLE == kStats) {
@@ -783,7 +821,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
               store_commit();
             }
           }
-          if (ROLE == kGradQ) {
+          if (ROLE == kGradQ && !p.direct) {
             // The split's slab, 16 fp32 columns at a time.
             const int slab_row = split * p.m_tiles * kTile + static_cast<int>(row_warp);
 #pragma unroll
@@ -801,31 +839,12 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
               }
             }
           }
-          if (ROLE == kGradRows) {
+          if (ROLE == kGradRows || (ROLE == kGradQ && p.direct)) {
             for (int h = 0; h < n_hits; ++h) {
               const int t = h == 0 ? hits.x : h == 1 ? hits.y : h == 2 ? hits.z : hits.w;
               if (t >= 0) {
-                const float rest = __ldg(p.rest + t);
-                const uint16_t* q = p.q + t * p.ldq + col;
-                if (col + 32 <= p.d) {
-                  const uint4* q4 = reinterpret_cast<const uint4*>(q);
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    const uint4 x = __ldg(q4 + k);
-                    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                      const float2 f = widen2<BF>(u[j]);
-                      v[8 * k + 2 * j] = __float_as_uint(fmaf(rest, f.x, __uint_as_float(v[8 * k + 2 * j])));
-                      v[8 * k + 2 * j + 1] = __float_as_uint(fmaf(rest, f.y, __uint_as_float(v[8 * k + 2 * j + 1])));
-                    }
-                  }
-                } else {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j)
-                    if (col + j < p.d)
-                      v[j] = __float_as_uint(fmaf(rest, widen2<BF>(__ldg(q + j)).x, __uint_as_float(v[j])));
-                }
+                const float rest = __ldg(p.rest + (ROLE == kGradQ ? row : t));
+                add_row<BF>(v, rest, p.other + t * p.ldother + col, p.d - col);
               }
             }
             uint32_t w[16];
@@ -835,12 +854,12 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             stage_row(out_buf, lane, w);
             if (p.tma_out) {
               if (lane == 0) {
-                tma_store(&tm_out, out_buf, col, p.v0 + static_cast<int>(row_warp));
+                tma_store(&tm_out, out_buf, col, p.out_row0 + static_cast<int>(row_warp));
                 store_commit();
               }
             } else {
-              store_staged(out_buf, lane, p.out + (p.v0 + row_warp) * p.ldo + col, p.ldo,
-                           static_cast<int>(p.piece - row_warp), p.d - col);
+              store_staged(out_buf, lane, p.out + (p.out_row0 + row_warp) * p.ldo + col, p.ldo,
+                           static_cast<int>(rows - row_warp), p.d - col);
               __syncwarp();
             }
           }
@@ -923,6 +942,13 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
   if (row < p.t) {
     const int64_t m = row / kTile;
     const int used = kGroups * (run_of(p.tiles, (m + 1) * p.n_tiles - 1, p.pairs) - run_of(p.tiles, m * p.n_tiles, p.pairs) + 1);
+    // The target's logit, before what does not depend on it.
+    const int64_t y = __ldg(p.targets + row);
+    float zt = 0.0f;
+    if (counts(y, p.ignore_index, p.v)) {
+      zt = warp_dot<BF>(p.q + row * p.ldq, p.rows + y * p.ldr, p.d, lane) * p.scale;
+      if (p.bias != nullptr) zt += __ldg(p.bias + y);
+    }
     const float2* pr = p.part + row * p.lists;
     float top = -kInf;
     for (int i = lane; i < used; i += 32) top = fmaxf(top, pr[i].x);
@@ -934,23 +960,18 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     const float others = (base + log2f(sum)) * kLn2;  // -inf where no other row takes part
-    const int64_t y = p.targets[row];
     float loss, lse = others;
     if (y == p.ignore_index) {
       loss = 0.0f;
     } else if (y < 0 || y >= p.v) {
       loss = __int_as_float(0x7fc00000);
+    } else if (zt == -kInf) {  // the target is left out
+      loss = sum == sum ? kInf : sum;
     } else {
-      float zt = warp_dot<BF>(p.q + row * p.ldq, p.rows + y * p.ldr, p.d, lane) * p.scale;
-      if (p.bias != nullptr) zt += __ldg(p.bias + y);
-      if (zt == -kInf) {  // the target is left out
-        loss = sum == sum ? kInf : sum;
-      } else {
-        const float a = others - zt;
-        const float tail = log1pf(expf(-fabsf(a)));
-        loss = fmaxf(a, 0.0f) + tail + (a != a ? a : 0.0f);
-        lse = fmaxf(others, zt) + tail;
-      }
+      const float a = others - zt;
+      const float tail = log1pf(expf(-fabsf(a)));
+      loss = fmaxf(a, 0.0f) + tail + (a != a ? a : 0.0f);
+      lse = fmaxf(others, zt) + tail;
     }
     if (lane == 0) {
       p.loss[row] = loss;
@@ -1338,10 +1359,8 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
   }
   Args base = common_args(x);
   base.row = row;
-  base.q = static_cast<const uint16_t*>(x.q);
-  base.ldq = x.ldq;
 
-  CUtensorMap q_k, rows_k, q_mn, rows_mn, slab, dr;
+  CUtensorMap q_k, rows_k, q_mn, rows_mn, slab, dr, dq_map;
   e = encode_rows_map(&q_k, x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kHalf, 128);
   if (e == cudaSuccess) e = encode_rows_map(&rows_k, x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kHalf, 128);
   // MN-major operands: boxes of 64 columns by 64 rows.
@@ -1353,11 +1372,13 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
                         32, 64);
   // TMA stores whole 16-byte pieces: a row that ends inside one would take what
   // lies behind it along.
-  const bool tma_out = reinterpret_cast<uintptr_t>(drows) % 16 == 0 && lddr % 8 == 0 && x.d % 8 == 0;
-  if (e == cudaSuccess && drows != nullptr && tma_out)
-    e = encode_rows_map(&dr, x.type, drows, x.d, x.v, lddr * 2, 32, 32, 64);
-  else
-    dr = slab;  // not used
+  auto by_tma = [&](const void* p, int64_t ld) {
+    return p != nullptr && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && x.d % 8 == 0;
+  };
+  const bool dr_tma = by_tma(drows, lddr), dq_tma = by_tma(dq, lddq);
+  dr = dq_map = slab;
+  if (e == cudaSuccess && dr_tma) e = encode_rows_map(&dr, x.type, drows, x.d, x.v, lddr * 2, 32, 32, 64);
+  if (e == cudaSuccess && dq_tma) e = encode_rows_map(&dq_map, x.type, dq, x.d, x.t, lddq * 2, 32, 32, 64);
   if (e != cudaSuccess) return e;
   base.rest = plan.rest;
   base.hit_list = plan.hit_list;
@@ -1366,6 +1387,7 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
     if (e != cudaSuccess) return e;
   }
   int splits_used = 0;
+  bool direct = false;
   int turn = 0;
   for (int64_t v0 = 0; v0 < x.v; v0 += plan.piece) {
     const int64_t piece = least(plan.piece, x.v - v0);
@@ -1391,22 +1413,32 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
       grad_args(p, plan.gt, bf, false, plan.m_tiles, piece, splits_used > 0 ? splits_used : plan.q_splits);
       if (splits_used == 0) splits_used = p.tiles / (p.m_tiles * p.n_tiles);
       p.accumulate = v0 > 0;
-      CUtensorMap maps_q[3] = {g_k, rows_mn, slab};
+      p.other = static_cast<const uint16_t*>(x.rows);
+      p.ldother = x.ldr;
+      p.direct = splits_used == 1 && piece == x.v;
+      p.out = static_cast<uint16_t*>(dq);
+      p.ldo = lddq;
+      p.tma_out = dq_tma;
+      direct = p.direct != 0;
+      CUtensorMap maps_q[3] = {g_k, rows_mn, direct ? dq_map : slab};
       if ((e = launch_role<kGradQ>(maps_q, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
       ++*launches;
     }
     if (drows != nullptr) {
       p = base;
       grad_args(p, plan.gt, bf, true, piece_n, x.t, 1);
+      p.other = static_cast<const uint16_t*>(x.q);
+      p.ldother = x.ldq;
       p.out = static_cast<uint16_t*>(drows);
       p.ldo = lddr;
-      p.tma_out = tma_out;
+      p.out_row0 = static_cast<int>(v0);
+      p.tma_out = dr_tma;
       CUtensorMap maps_r[3] = {g_mn, q_mn, dr};
       if ((e = launch_role<kGradRows>(maps_r, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
       ++*launches;
     }
   }
-  if (dq != nullptr) {
+  if (dq != nullptr && !direct) {
     const int quads = static_cast<int>(ceil_div(x.d, 4));
     const int rows_per_block = quads >= 256 ? 1 : 256 / quads;
     GradQArgs a = {plan.slab, splits_used, plan.slab_rows, plan.ld_slab, x.t, x.v, x.d, row, plan.rest, x.targets,
