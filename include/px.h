@@ -317,7 +317,8 @@ PX_API px_status px_int8_scores_device(int32_t device, const int8_t* q, int64_t 
  *   loss[i] = log sum_j exp z_ij - z_i,targets[i],  lse[i] = log sum_j exp z_ij
  * queries (t x dim) and rows (v x dim) are PX_F16 or PX_BF16 with rows on
  * 16-byte boundaries; targets are row numbers; bias (v floats, 16-byte
- * aligned) may be NULL, and -infinity in it leaves a row out of the softmax.
+ * aligned) may be NULL, and -infinity in it, or any value below -2e31, leaves
+ * a row out of the softmax.
  * A query whose target is ignore_index has loss 0 (its lse is still written);
  * one whose target is any other number outside [0, v) has loss NaN; one whose
  * target is left out, +infinity. total (2 floats) receives, for PX_REDUCE_SUM

@@ -238,6 +238,10 @@ __device__ __forceinline__ void leave_out_from(uint32_t (&v)[32], int from) {
     if (j >= from) v[j] = __float_as_uint(-kInf);
 }
 
+// A row's bias in log2 units. Below about -1.4e31 (a type's lowest value, say) it
+// is -inf: the row is left out, as with -inf itself.
+__device__ __forceinline__ float bias2(float b) { return b * (kLog2e * 0x1p24f) * 0x1p-24f; }
+
 // Adds the bias: v becomes c * v + bias * log2(e), log2 units. Columns past
 // the base count as left out.
 __device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, int left, float c) {
@@ -246,15 +250,15 @@ __device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, i
 #pragma unroll
     for (int j4 = 0; j4 < 8; ++j4) {
       const float4 b = __ldg(b4 + j4);
-      v[4 * j4] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4]), c, b.x * kLog2e));
-      v[4 * j4 + 1] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 1]), c, b.y * kLog2e));
-      v[4 * j4 + 2] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 2]), c, b.z * kLog2e));
-      v[4 * j4 + 3] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 3]), c, b.w * kLog2e));
+      v[4 * j4] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4]), c, bias2(b.x)));
+      v[4 * j4 + 1] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 1]), c, bias2(b.y)));
+      v[4 * j4 + 2] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 2]), c, bias2(b.z)));
+      v[4 * j4 + 3] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 3]), c, bias2(b.w)));
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      v[j] = __float_as_uint(j < left ? fmaf(__uint_as_float(v[j]), c, __ldg(bias + j) * kLog2e) : -kInf);
+      v[j] = __float_as_uint(j < left ? fmaf(__uint_as_float(v[j]), c, bias2(__ldg(bias + j))) : -kInf);
   }
 }
 
@@ -947,7 +951,7 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
     float zt = 0.0f;
     if (counts(y, p.ignore_index, p.v)) {
       zt = warp_dot<BF>(p.q + row * p.ldq, p.rows + y * p.ldr, p.d, lane) * p.scale;
-      if (p.bias != nullptr) zt += __ldg(p.bias + y);
+      if (p.bias != nullptr) zt += bias2(__ldg(p.bias + y)) * kLn2;
     }
     const float2* pr = p.part + row * p.lists;
     float top = -kInf;

@@ -4,6 +4,7 @@
 // call can be captured into a CUDA graph.
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "px_rows.h"
@@ -53,6 +54,21 @@ px_status check_tiled(const void* p, int64_t ld, int64_t elem, int32_t dim, cons
   return PX_OK;
 }
 
+// Pointers of whole elements.
+px_status check_aligned(std::initializer_list<const void*> ps, uintptr_t bytes, const char* what) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % bytes != 0)
+      return set_error(PX_EINVAL, std::string(what) + ": misaligned for its type");
+  return PX_OK;
+}
+
+// Tiles are numbered in 32 bits.
+px_status check_tiles(int64_t a, int64_t b, const char* what) {
+  if (((a + 255) / 256) * ((b + 255) / 256) > 0x7fffffff)
+    return set_error(PX_EUNSUPPORTED, std::string(what) + " is too large");
+  return PX_OK;
+}
+
 px_status check_xent(int64_t t, int64_t v, int32_t dim, const void* q, int64_t ldq, const void* rows, int64_t ldr,
                      int32_t type, const int64_t* targets, float scale, const float* bias) {
   px_status s = check_rows(t, dim, "t");
@@ -67,6 +83,10 @@ px_status check_xent(int64_t t, int64_t v, int32_t dim, const void* q, int64_t l
   if (s == PX_OK) s = check_tiled(rows, ldr, 2, dim, "rows");
   if (s != PX_OK) return s;
   if (targets == nullptr) return set_error(PX_EINVAL, "null buffer");
+  s = check_aligned({targets}, 8, "targets");
+  if (s == PX_OK) s = check_tiles(t, v, "t * v");
+  if (s == PX_OK) s = check_tiles(t > v ? t : v, dim, "dim");
+  if (s != PX_OK) return s;
   if (bias != nullptr && !aligned16(bias)) return set_error(PX_EINVAL, "bias must be 16-byte aligned");
   return PX_OK;
 }
@@ -101,6 +121,9 @@ PX_API px_status px_quantize_rows_device(int32_t device, const void* x, int32_t 
   if (n == 0) return PX_OK;
   if (x == nullptr || codes == nullptr || scales == nullptr) return set_error(PX_EINVAL, "null buffer");
   if (ldx < dim || ldc < dim) return set_error(PX_EINVAL, "a row stride is less than dim");
+  s = check_aligned({x}, size_of(type), "x");
+  if (s == PX_OK) s = check_aligned({scales}, 4, "scales");
+  if (s != PX_OK) return s;
   if ((s = check_device(device)) != PX_OK) return s;
   DeviceGuard dg(device);
   cudaError_t e = launch_quantize_rows(x, static_cast<ElemType>(type), n, dim, ldx, codes, ldc, scales,
@@ -118,6 +141,9 @@ PX_API px_status px_dequantize_rows_device(int32_t device, const int8_t* codes, 
   if (n == 0) return PX_OK;
   if (codes == nullptr || scales == nullptr || out == nullptr) return set_error(PX_EINVAL, "null buffer");
   if (ldc < dim || ldo < dim) return set_error(PX_EINVAL, "a row stride is less than dim");
+  s = check_aligned({out}, size_of(type), "out");
+  if (s == PX_OK) s = check_aligned({scales}, 4, "scales");
+  if (s != PX_OK) return s;
   if ((s = check_device(device)) != PX_OK) return s;
   DeviceGuard dg(device);
   cudaError_t e = launch_dequantize_rows(codes, ldc, scales, n, dim, static_cast<ElemType>(type), out, ldo,
@@ -142,7 +168,10 @@ PX_API px_status px_int8_scores_device(int32_t device, const int8_t* q, int64_t 
   if (s != PX_OK) return s;
   if (q_scales == nullptr || x_scales == nullptr || out == nullptr) return set_error(PX_EINVAL, "null buffer");
   if (ldo < n) return set_error(PX_EINVAL, "out: the row stride is less than n");
-  if (reinterpret_cast<uintptr_t>(out) % size_of(type) != 0) return set_error(PX_EINVAL, "out is misaligned");
+  s = check_aligned({out}, size_of(type), "out");
+  if (s == PX_OK) s = check_aligned({q_scales, x_scales, bias}, 4, "scales or bias");
+  if (s == PX_OK) s = check_tiles(m, n, "m * n");
+  if (s != PX_OK) return s;
   if ((s = check_device(device)) != PX_OK) return s;
   DeviceGuard dg(device);
   Int8ScoresArgs a;
@@ -166,6 +195,7 @@ PX_API px_status px_int8_scores_device(int32_t device, const int8_t* q, int64_t 
 
 PX_API int64_t px_softmax_xent_workspace_bytes(int32_t device, int64_t t, int64_t v, int32_t dim, int32_t backward) {
   if (t < 0 || v < 0 || dim <= 0 || t > kMaxRows || v > kMaxRows) return 0;
+  if (check_tiles(t, v, "t * v") != PX_OK || check_tiles(t > v ? t : v, dim, "dim") != PX_OK) return 0;
   if (t == 0 || v == 0) return 0;
   DeviceGuard dg(device);
   const int clusters = gemm_pair_clusters(device);
@@ -184,6 +214,8 @@ PX_API px_status px_softmax_xent_device(int32_t device, const void* queries, int
   if (t == 0) return PX_OK;
   if (loss == nullptr || lse == nullptr || (reduction != PX_REDUCE_NONE && (total == nullptr || divisor == nullptr)))
     return set_error(PX_EINVAL, "null buffer");
+  s = check_aligned({loss, lse, total, divisor}, 4, "an output");
+  if (s != PX_OK) return s;
   if ((s = check_device(device)) != PX_OK) return s;
   DeviceGuard dg(device);
   const int clusters = gemm_pair_clusters(device);
@@ -211,8 +243,9 @@ PX_API px_status px_softmax_xent_backward_device(int32_t device, const void* que
   if (loss == nullptr || lse == nullptr || grad == nullptr) return set_error(PX_EINVAL, "null buffer");
   if ((grad_queries != nullptr && ldgq < dim) || (grad_rows != nullptr && ldgr < dim))
     return set_error(PX_EINVAL, "a row stride is less than dim");
-  if (reinterpret_cast<uintptr_t>(grad_queries) % 2 != 0 || reinterpret_cast<uintptr_t>(grad_rows) % 2 != 0)
-    return set_error(PX_EINVAL, "a gradient is misaligned");
+  s = check_aligned({grad_queries, grad_rows}, 2, "a gradient");
+  if (s == PX_OK) s = check_aligned({loss, lse, grad, divisor}, 4, "an input");
+  if (s != PX_OK) return s;
   if ((s = check_device(device)) != PX_OK) return s;
   DeviceGuard dg(device);
   const int clusters = gemm_pair_clusters(device);

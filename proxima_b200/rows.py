@@ -141,7 +141,7 @@ def int8_scores(q_codes, q_scales, codes, scales, bias=None, dtype=torch.float32
     32-bit integers (dim <= 131071). ``bias`` (float32, n) is added to each
     base row's scores; with ``bias = -0.5 * |row|^2`` scores order rows as L2
     distance does. ``out`` receives the result if given (its rows may be
-    strided)."""
+    strided). Not differentiable."""
     _check(q_codes, "q_codes", 2, (torch.int8,))
     _check(q_scales, "q_scales", 1, (torch.float32,))
     _check(codes, "codes", 2, (torch.int8,))
@@ -249,7 +249,8 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     targets: int64, row numbers; ``ignore_index`` gives a query loss 0 and no
     gradient, any other number outside [0, v) loss NaN and no gradient. bias
     (float32, v, no gradient): added to a row's logits, for instance the
-    correction for how rows were sampled; -inf leaves a row out. scale: a
+    correction for how rows were sampled; -inf (or any value below -2e31)
+    leaves a row out. scale: a
     positive number (one over the temperature). reduction: "mean" (over the
     queries not ignored; NaN if there are none), "sum" or "none". Queries and
     rows must be finite even where ignored or left out."""
@@ -263,6 +264,9 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     scale = float(scale)
     if not scale > 0.0 or math.isinf(scale):
         raise ValueError("scale must be positive and finite")
+    ignore_index = int(ignore_index)
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index must be a 64-bit integer")
     if reduction not in _REDUCTIONS:
         raise ValueError("reduction must be 'none', 'sum' or 'mean'")
     if _dim(queries, "queries") != rows.shape[1]:
@@ -276,9 +280,9 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     _same_device(queries.device, rows=rows, targets=targets, bias=bias)
     if queries.shape[0] == 0:
         # No query: an empty loss, or the sum or mean of one, with zero gradients.
-        loss = (queries.float().sum(1) + 0.0 * rows[:1].float().sum())
+        loss = queries.float().sum(1) + rows[:0].float().sum()
         return {"none": lambda: loss, "sum": loss.sum, "mean": loss.mean}[reduction]()
-    args = (queries, rows, targets, scale, bias, int(ignore_index), _REDUCTIONS[reduction])
+    args = (queries, rows, targets, scale, bias, ignore_index, _REDUCTIONS[reduction])
     if torch.is_grad_enabled() and (queries.requires_grad or rows.requires_grad):
         return _SoftmaxCrossEntropy.apply(*args)
     return _xent_forward(*args)[0]

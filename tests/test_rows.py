@@ -30,6 +30,9 @@ def test_quantize_arguments(px, lib):
     _refused(px, f(0, VP(16), 3, 4, 8, 8, VP(16), 16, VP(16), None), L.PX_EINVAL, "type")
     _refused(px, f(0, VP(16), 0, 4, 8, 7, VP(16), 16, VP(16), None), L.PX_EINVAL, "stride")
     _refused(px, f(0, None, 0, 4, 8, 8, VP(16), 16, VP(16), None), L.PX_EINVAL, "null buffer")
+    _refused(px, f(0, VP(18), 0, 4, 8, 8, VP(16), 16, VP(16), None), L.PX_EINVAL, "x: misaligned")
+    _refused(px, f(0, VP(17), 2, 4, 8, 8, VP(16), 16, VP(16), None), L.PX_EINVAL, "x: misaligned")
+    _refused(px, f(0, VP(16), 0, 4, 8, 8, VP(16), 16, VP(18), None), L.PX_EINVAL, "scales: misaligned")
     assert f(0, None, 0, 0, 8, 8, None, 16, None, None) == L.PX_OK
     g = lib.px_dequantize_rows_device
     _refused(px, g(0, VP(16), 16, VP(16), 4, 8, 5, VP(16), 8, None), L.PX_EINVAL, "type")
@@ -51,6 +54,7 @@ def test_scores_arguments(px, lib):
     _refused(px, f(ldo=4), L.PX_EINVAL, "less than n")
     _refused(px, f(out=18), L.PX_EINVAL, "misaligned")
     _refused(px, f(type_=9), L.PX_EINVAL, "type")
+    _refused(px, f(m=1 << 30, n=1 << 30, ldo=1 << 30), L.PX_EUNSUPPORTED, "m * n is too large")
     assert f(m=0) == L.PX_OK and f(n=0, ldo=0) == L.PX_OK
 
 
@@ -73,6 +77,8 @@ def test_softmax_arguments(px, lib):
     _refused(px, f(bias=8), L.PX_EINVAL, "bias must be 16-byte aligned")
     _refused(px, f(reduction=3), L.PX_EINVAL, "reduction")
     _refused(px, f(reduction=2, total=None), L.PX_EINVAL, "null buffer")
+    _refused(px, f(targets=20), L.PX_EINVAL, "targets: misaligned")
+    _refused(px, f(t=1 << 30, v=1 << 30), L.PX_EUNSUPPORTED, "t * v is too large")
     assert f(t=0) == L.PX_OK
 
     def g(t=4, stride=0, grad=16, gq=16, ldgq=8):
@@ -170,6 +176,8 @@ def test_python_layer_refusals(px):
         px.softmax_cross_entropy(qq, rr, z(3, dtype=torch.int64))
     with pytest.raises(ValueError, match="at least one base row"):
         px.softmax_cross_entropy(qq, z(0, 8, dtype=b16), y)
+    with pytest.raises(ValueError, match="ignore_index"):
+        px.softmax_cross_entropy(qq, rr, y, ignore_index=2 ** 64)
     for scale in (0.0, -1.0, math.inf, math.nan):
         with pytest.raises(ValueError, match="scale"):
             px.softmax_cross_entropy(qq, rr, y, scale=scale)

@@ -347,10 +347,25 @@ def test_softmax_weighted_queries(px):
     _check_xent(px, q, r, y, b, weights=torch.zeros(200, device="cuda"))
 
 
-def test_softmax_several_pieces(px):
-    # A base of several pieces of the gradient's buffer, the last one ragged.
-    t, v, d = 300, 230_007, 16
+@pytest.mark.parametrize("v", [230_007, 520_009])
+def test_softmax_several_pieces(px, v):
+    # Bases of one and of several pieces of the gradient's buffer, the last ragged.
+    t, d = 300, 16
+    ws = px._lib.load().px_softmax_xent_workspace_bytes(0, t, v, d, 1)
+    assert (ws < 2 * t * v) == (v == 520_009)
     _check_xent(px, *_xent_case(t, v, d, torch.bfloat16, 21), reduction="mean")
+
+
+def test_softmax_several_pieces_with_shared_targets(px):
+    # Every third query has the same target, in the second piece; the others
+    # share theirs by twos and threes.
+    t, v, d = 300, 520_009, 16
+    q, r, y, b = _xent_case(t, v, d, torch.float16, 22, bias=True, ignored=True)
+    y[::3] = 400_001
+    y[1:40] = y[1:40] // 1000 * 1000
+    y[50:56] = 7
+    b[y[y >= 0]] = 0.25
+    _check_xent(px, q, r, y, b, weights=torch.linspace(0.5, 2, t, device="cuda"))
 
 
 def test_softmax_unpitched_and_strided_operands(px):
@@ -425,6 +440,32 @@ def test_softmax_confident_targets(px):
     want = math.log1p(49 * math.exp(-24.0))
     assert ((loss.double() - want).abs() <= want * (2.0 ** -21 + 30 * U + 8 * U * 24)).all()
     _check_xent(px, q, r, y, None)
+
+
+def test_softmax_lowest_bias_leaves_rows_out(px):
+    q, r, y, b = _xent_case(40, 300, 32, torch.bfloat16, 43, bias=True)
+    q, r = q.requires_grad_(), r.requires_grad_()
+
+    def step(bias):
+        loss = px.softmax_cross_entropy(q, r, y, bias=bias, reduction="none")
+        return (loss, *torch.autograd.grad(loss.sum(), (q, r)))
+
+    want = step(b)
+    out = b == -math.inf
+    for lowest in (torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min, -3e31):
+        assert all(torch.equal(x, w) for x, w in zip(step(b.masked_fill(out, lowest)), want))
+    assert not want[2][out].any()
+
+
+def test_softmax_common_offset_changes_nothing_much(px):
+    # Biases far from zero but alike: the softmax is that of their differences,
+    # to the accuracy of fp32 numbers of that size.
+    q, r, y, b = _xent_case(40, 300, 32, torch.bfloat16, 44)
+    off = torch.full((300,), -10_000.0, device="cuda")
+    a = px.softmax_cross_entropy(q, r, y, bias=off, reduction="none").double()
+    w = px.softmax_cross_entropy(q, r, y, reduction="none").double()
+    # Logits of 14427 in log2 units have steps of 2^-10; three roundings.
+    assert ((a - w).abs() <= 4 * 2.0 ** -10).all()
 
 
 def test_softmax_rows_left_out(px):
@@ -580,6 +621,78 @@ def test_row_operators_in_graphs(px):
             graph.replay()
             got = [o.clone() for o in out]
             assert all(torch.equal(g, w) for g, w in zip(got, step()))
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first use of each operator is a graph capture."""
+    code = """
+import torch, proxima_b200 as px
+q = torch.randn(70, 64, device='cuda').bfloat16().requires_grad_()
+r = torch.randn(900, 64, device='cuda').bfloat16().requires_grad_()
+y = torch.arange(70, device='cuda')
+def step():
+    loss = px.softmax_cross_entropy(q, r, y, reduction='sum')
+    qc, qs = px.quantize_rows(q); rc, rs = px.quantize_rows(r)
+    return (loss.detach(), *torch.autograd.grad(loss, (q, r)), px.int8_scores(qc, qs, rc, rs), px.dequantize_rows(qc, qs))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()
+got = [o.clone() for o in out]
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print('captured')
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_host_threads(px):
+    import threading
+    cases = [_xent_case(100, 5000, 48, torch.float16, 700 + k) for k in range(2)]
+
+    def step(k):
+        q, r, y, _ = cases[k]
+        q, r = q.detach().requires_grad_(), r.detach().requires_grad_()
+        loss = px.softmax_cross_entropy(q, r, y, reduction="sum")
+        qc, qs = px.quantize_rows(q)
+        rc, rs = px.quantize_rows(r)
+        return [loss.detach(), *torch.autograd.grad(loss, (q, r)), px.int8_scores(qc, qs, rc, rs)]
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = step(k)
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                    failed.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(100)
+    assert not failed and not any(th.is_alive() for th in threads)
+
+
+def test_rows_of_the_same_tensor(px):
+    # The queries are some of the rows themselves.
+    x = (_rand(200, 40, seed=5) / 6).to(torch.bfloat16).requires_grad_()
+    y = torch.arange(50, device="cuda") + 100
+    loss = px.softmax_cross_entropy(x[:50], x, y, scale=2.0, reduction="sum")
+    loss.backward()
+    q, r = x.detach()[:50].clone().requires_grad_(), x.detach().clone().requires_grad_()
+    dq, dr = torch.autograd.grad(px.softmax_cross_entropy(q, r, y, scale=2.0, reduction="sum"), (q, r))
+    dr[:50] += dq
+    assert torch.equal(x.grad, dr)
 
 
 def test_rows_status(px):
