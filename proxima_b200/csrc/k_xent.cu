@@ -279,7 +279,25 @@ __device__ __forceinline__ void stage_row(uint32_t buf, int lane, const uint32_t
   __syncwarp();
 }
 
-// The same block by plain stores, for an array that TMA cannot address (rows
+// Half a warp's 16 rows x 128 bytes likewise, as 128-byte swizzle lays them
+// out (piece p of row r at p ^ (r % 8)).
+__device__ __forceinline__ void stage_line(uint32_t buf, int lane, int half, const uint32_t (&w)[32]) {
+  if (lane == 0) store_wait_read();
+  __syncwarp();
+  if ((lane >> 4) == half) {
+    const int r = lane & 15;
+    const uint32_t row = buf + r * 128;
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((p ^ (r & 7)) << 4)), "r"(w[4 * p]),
+                   "r"(w[4 * p + 1]), "r"(w[4 * p + 2]), "r"(w[4 * p + 3])
+                   : "memory");
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// A block of stage_row's by plain stores, for an array that TMA cannot address (rows
 // that begin or end off 16-byte boundaries): half a warp per row where its pairs of values lie on
 // 4-byte boundaries, else a warp per row.
 __device__ __forceinline__ void store_staged(uint32_t buf, int lane, uint16_t* out, int64_t ldo, int rows, int cols) {
@@ -772,12 +790,81 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         }
         continue;
       }
+      if (ROLE == kWeights) {
+        // This warp's 64 columns, packed half by half.
+        const int col = n * kTile + group * 64;  // within the piece
+        const bool some = row_warp < p.t && col < p.piece;
+        const uint32_t at_tmem = lane_addr + static_cast<uint32_t>(acc * kTile + group * 64);
+        auto release = [&]() {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
+        };
+        if (some) {
+          uint32_t w[32];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v[32];
+            __syncwarp();
+            tc::tmem_ld_32x32b_x32(at_tmem + 32 * h, v);
+            tc::tmem_ld_wait();
+            // The last columns are in registers: the accumulator is free.
+            if (h == 1) release();
+            if (lost) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
+            }
+            const int col_h = col + 32 * h;
+            if (BIAS) add_bias(v, p.bias + p.v0 + col_h, static_cast<int>(p.v) - p.v0 - col_h, p.c);
+            const float c = BIAS ? 1.0f : p.c;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[16 * h + j] = pack2<BF>(ex2(fmaf(__uint_as_float(v[2 * j]), c, shift)),
+                                        ex2(fmaf(__uint_as_float(v[2 * j + 1]), c, shift)));
+          }
+          if (factor < 0.0f) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] ^= 0x80008000u;
+          }
+          const int at = target - col;  // the target's place among the columns
+          if (at >= 0 && at < 64) {
+            p.rest[row] = at_target - rounded<BF>(at_target);
+            if (p.hits != nullptr) {
+              const int slot = atomicAdd(p.hits + target, 1);
+              if (slot < kHits) reinterpret_cast<int*>(p.hit_list + target)[slot] = static_cast<int>(row);
+            }
+            const uint32_t e = pack2<BF>(at_target, at_target);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (2 * j == at) w[j] = (w[j] & 0xffff0000u) | (e & 0xffffu);
+              if (2 * j + 1 == at) w[j] = (w[j] & 0xffffu) | (e & 0xffff0000u);
+            }
+          }
+          // Sixteen rows at a time, so that a buffer half as large as the block takes
+          // rows of whole 128-byte lines (1-2% of a training step against 64-byte ones).
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            stage_line(out_buf, lane, h, w);
+            if (lane == 0) {
+              tma_store(&tm_out, out_buf, col, static_cast<int>(row_warp) + 16 * h);
+              store_commit();
+            }
+          }
+        } else {
+          release();
+        }
+        if (++acc == accs) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+        continue;
+      }
       const int64_t rows = ROLE == kGradRows ? p.piece : p.t;
       bool freed = false;
       if (row_warp < rows) {
         for (int b = group; b * 32 < p.n_cols; b += kGroups) {
           const int col = n * p.n_cols + b * 32;  // within the product
-          const int cols = ROLE == kWeights ? p.piece : p.d;
+          const int cols = p.d;
           if (col >= cols) break;
           __syncwarp();
           uint32_t v[32];
@@ -793,37 +880,6 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           if (lost) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
-          }
-          const int at = target - col;  // the target's place in the block
-          if (ROLE == kWeights) {
-            if (BIAS) add_bias(v, p.bias + p.v0 + col, static_cast<int>(p.v) - p.v0 - col, p.c);
-            const float c = BIAS ? 1.0f : p.c;
-            uint32_t w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              w[j] = pack2<BF>(ex2(fmaf(__uint_as_float(v[2 * j]), c, shift)), ex2(fmaf(__uint_as_float(v[2 * j + 1]), c, shift)));
-            if (factor < 0.0f) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] ^= 0x80008000u;
-            }
-            if (at >= 0 && at < 32) {
-              p.rest[row] = at_target - rounded<BF>(at_target);
-              if (p.hits != nullptr) {
-                const int slot = atomicAdd(p.hits + target, 1);
-                if (slot < kHits) reinterpret_cast<int*>(p.hit_list + target)[slot] = static_cast<int>(row);
-              }
-              const uint32_t e = pack2<BF>(at_target, at_target);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                if (2 * j == at) w[j] = (w[j] & 0xffff0000u) | (e & 0xffffu);
-                if (2 * j + 1 == at) w[j] = (w[j] & 0xffffu) | (e & 0xffff0000u);
-              }
-            }
-            stage_row(out_buf, lane, w);
-            if (lane == 0) {
-              tma_store(&tm_out, out_buf, col, static_cast<int>(row_warp));
-              store_commit();
-            }
           }
           if (ROLE == kGradQ && !p.direct) {
             // The split's slab, 16 fp32 columns at a time.
@@ -1404,7 +1460,7 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
     CUtensorMap g_k, g_mn, g_out;
     e = encode_rows_map(&g_k, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kHalf, 128);
     if (e == cudaSuccess) e = encode_rows_map(&g_mn, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kSlice, 128);
-    if (e == cudaSuccess) e = encode_rows_map(&g_out, x.type, plan.g, piece, x.t, plan.piece * 2, 32, 32, 64);
+    if (e == cudaSuccess) e = encode_rows_map(&g_out, x.type, plan.g, piece, x.t, plan.piece * 2, 64, 16, 128);
     if (e != cudaSuccess) return e;
     Args p = base;
     logits_args(p, bf, plan.m_tiles, piece_n);
