@@ -435,13 +435,20 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     bool lost = false;  // a wait gave up: the scores that remain are NaN
     // This warp's blocks of 32 columns: grp and grp + 4 of the tile's, block b
     // being queries b % q_blocks of base rows b / q_blocks.
+    // (Divided once: per tile, the divisions took as long as the scores.)
     const int q_blocks = p.n_cols / 32;
     const int row_in_cta = quarter * 32 + lane;
+    int sub_of[kBlocks], q_of[kBlocks];  // row group and first query of each block
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+      sub_of[k] = (grp + kGroups * k) / q_blocks;
+      q_of[k] = (grp + kGroups * k - sub_of[k] * q_blocks) * 32;
+    }
     float next_xs[kBlocks], next_bias[kBlocks];
     auto load_rows = [&](int tile) {
 #pragma unroll
       for (int k = 0; k < kBlocks; ++k) {
-        const int sub = (grp + kGroups * k) / q_blocks;
+        const int sub = sub_of[k];
         const int64_t r = (static_cast<int64_t>(tile) * p.subs + sub) * (2 * kRows) + rank * kRows + row_in_cta;
         const bool live = sub < p.subs && r < p.n;
         next_xs[k] = live ? __ldg(p.x_scale + r) : 0.0f;
@@ -451,11 +458,14 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     load_rows(bt);
     for (int t = first; t < tiles; t += p.width) {
       const int64_t q0 = static_cast<int64_t>(qg) * p.n_cols;
+      // The next tile's base rows, whichever query group's it is.
+      int wrapped = bt + p.width;
+      while (wrapped >= p.base_tiles) wrapped -= p.base_tiles;
       if (fresh) {
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
-          const int64_t qi = q0 + (grp + kGroups * k) % q_blocks * 32 + lane;
+          const int64_t qi = q0 + q_of[k] + lane;
           scale[k * 32 + lane] = qi < p.m ? __ldg(p.q_scale + qi) : 0.0f;
         }
         __syncwarp();
@@ -468,7 +478,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         bias[k] = next_bias[k];
       }
       // The next tile's, one tile ahead of their use.
-      load_rows((bt + p.width) % p.base_tiles);
+      load_rows(wrapped);
       if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
       tc::tc_fence_after();
       const int queries = p.m - q0 < p.n_cols ? static_cast<int>(p.m - q0) : p.n_cols;
@@ -476,7 +486,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
 #pragma unroll
       for (int k = 0; k < kBlocks; ++k) {
         const int b = grp + kGroups * k;
-        const int sub = b / q_blocks, q_in = (b - sub * q_blocks) * 32;
+        const int sub = sub_of[k], q_in = q_of[k];
         const int64_t row_cta = (static_cast<int64_t>(bt) * p.subs + sub) * (2 * kRows) + rank * kRows;
         const int64_t row = row_cta + row_in_cta, row_warp = row - lane;
         // With TMA all four warps of a group take part, base rows or not: they

@@ -113,6 +113,7 @@ struct Args {
   int m_tiles, n_tiles;
   int tiles;             // logits: m_tiles * n_tiles; gradients: items
   int per_split;         // kGradQ: K slices per split
+  int next_m, next_n, next_split;  // gradients: from a pair's tile to its next
   int n_cols;            // N of a tile: 256 (logits), else a multiple of 32 up to 512
   int k_slices;
   int keep;              // logits: query slices kept in shared memory
@@ -369,21 +370,63 @@ __device__ __forceinline__ void add_row(uint32_t (&v)[32], float f, const uint16
   }
 }
 
-// Gradient item i: M tile, N tile, K slices [k0, k1).
-struct Item {
-  int m, n, split, k0, k1;
+// Where a tile lies. Tiles are numbered along the base, then along the queries
+// (logits), or along M, then N, then the splits (gradients). A pair divides its
+// first tile's number once and counts on from there: an integer division uses
+// the special-function unit, and per tile, behind the exponentials, one took
+// 3500 clocks.
+struct Place {
+  int m, n, split;
 };
 
 template <int ROLE>
-__device__ __forceinline__ Item item_of(const Args& p, int i) {
-  Item it;
-  it.m = i % p.m_tiles;
-  const int rest = i / p.m_tiles;
-  it.n = rest % p.n_tiles;
-  it.split = rest / p.n_tiles;
-  it.k0 = ROLE == kGradQ ? it.split * p.per_split : 0;
-  it.k1 = ROLE == kGradQ ? min(p.k_slices, it.k0 + p.per_split) : p.k_slices;
-  return it;
+__device__ __forceinline__ Place place_of(const Args& p, int i) {
+  Place at;
+  if (Shape<ROLE>::LOGITS) {
+    at.m = i / p.n_tiles;
+    at.n = i - at.m * p.n_tiles;
+    at.split = 0;
+  } else {
+    const int rest = i / p.m_tiles;
+    at.m = i - rest * p.m_tiles;
+    at.split = rest / p.n_tiles;
+    at.n = rest - at.split * p.n_tiles;
+  }
+  return at;
+}
+
+// To the pair's next tile: the next one, or (gradients) the one `pairs` further,
+// which is (next_m, next_n, next_split) on.
+template <int ROLE>
+__device__ __forceinline__ void advance(const Args& p, Place& at) {
+  if (Shape<ROLE>::LOGITS) {
+    if (++at.n == p.n_tiles) {
+      at.n = 0;
+      ++at.m;
+    }
+  } else {
+    at.m += p.next_m;
+    at.n += p.next_n;
+    at.split += p.next_split;
+    if (at.m >= p.m_tiles) {
+      at.m -= p.m_tiles;
+      ++at.n;
+    }
+    if (at.n >= p.n_tiles) {
+      at.n -= p.n_tiles;
+      ++at.split;
+    }
+  }
+}
+
+// A gradient tile's K slices.
+template <int ROLE>
+__device__ __forceinline__ int first_slice(const Args& p, const Place& at) {
+  return ROLE == kGradQ ? at.split * p.per_split : 0;
+}
+template <int ROLE>
+__device__ __forceinline__ int last_slice(const Args& p, const Place& at) {
+  return ROLE == kGradQ ? min(p.k_slices, (at.split + 1) * p.per_split) : p.k_slices;
 }
 
 // Logits tiles [first, last) of pair `i` of `n`, and the pair that has tile x.
@@ -477,6 +520,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       int slot = 0;
       uint32_t phase = 0;
       int kept = -1;          // query tile whose slices are kept
+      Place at = place_of<ROLE>(p, first);
       uint32_t keeps = 0;
       bool ok = true;
       // The next ring slot, armed for both CTAs' bytes; 0 when a wait gave up.
@@ -494,8 +538,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       };
       for (int i = first; ok && i < last; i += step) {
         uint32_t fb, dst;
+        const int m = at.m, n = at.n;
         if (S::LOGITS) {
-          const int m = i / p.n_tiles, n = i - m * p.n_tiles;
           const int m0 = m * kTile + rank * kHalf;
           const int n0 = p.v0 + n * kTile + rank * kHalf;
           if (m != kept) {
@@ -517,11 +561,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
               tc::tma_load_2d_pair(dst + i2 * kSlot, &tm_b, fb, (k + i2) * kSlice, n0);
           }
         } else {
-          const Item it = item_of<ROLE>(p, i);
-          const int m0 = it.m * kTile + rank * kHalf;
-          const int n0 = it.n * p.n_cols;
+          const int m0 = m * kTile + rank * kHalf;
+          const int n0 = n * p.n_cols;
+          const int k0 = first_slice<ROLE>(p, at), k1 = last_slice<ROLE>(p, at);
           const int boxes1 = (n_first / 2 + 63) / 64, boxes2 = (n_second / 2 + 63) / 64;
-          for (int k = it.k0; k < it.k1; ++k) {
+          for (int k = k0; k < k1; ++k) {
             if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
             if (S::A_MN) {
               tc::tma_load_2d_pair(dst, &tm_a, fb, m0, k * kSlice);
@@ -540,6 +584,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             }
           }
         }
+        advance<ROLE>(p, at);
       }
       // Both CTAs' loads complete on the even CTA's barriers: it waits for
       // the last phase of each before shared memory goes away.
@@ -577,8 +622,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         }
         return true;
       };
-      int n_left = S::LOGITS ? p.n_tiles - first % p.n_tiles : 0;  // tiles until the queries change
-      bool fresh = true;
+      Place at = place_of<ROLE>(p, first);
+      bool fresh = true;  // the queries changed
       for (int i = first; ok && i < last; i += step) {
         if (!wait(tempty_bar(acc), acc_phase ^ 1)) break;
         int k0 = 0, k1 = p.k_slices;
@@ -589,9 +634,8 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             fresh = false;
           }
         } else {
-          const Item it = item_of<ROLE>(p, i);
-          k0 = it.k0;
-          k1 = it.k1;
+          k0 = first_slice<ROLE>(p, at);
+          k1 = last_slice<ROLE>(p, at);
         }
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kTile);
         for (int k = k0; k < k1; k += per) {
@@ -630,8 +674,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         }
         if (!ok) break;
         if (issuer) tc::mma_commit_pair_both(tfull_bar(acc));
-        if (S::LOGITS && --n_left == 0) {
-          n_left = p.n_tiles;
+        const int m = at.m;
+        advance<ROLE>(p, at);
+        if (S::LOGITS && at.m != m) {
           fresh = true;
           if (issuer && i + 1 < last) tc::mma_commit_pair_both(kempty_bar);
         }
@@ -667,17 +712,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             make_float2(run_base, lost ? __int_as_float(0x7fc00000) : run_sum);
       }
     };
+    Place place = place_of<ROLE>(p, first);
+    // What the gradients are multiplied by at the end.
+    const float final_scale =
+        ROLE == kGradRows || (ROLE == kGradQ && p.direct) ? out_scale(p.row, p.scale) : 0.0f;
     for (int i = first; i < last; i += step) {
-      int m, n, split = 0;
-      if (S::LOGITS) {
-        m = i / p.n_tiles;
-        n = i - m * p.n_tiles;
-      } else {
-        const Item it = item_of<ROLE>(p, i);
-        m = it.m;
-        n = it.n;
-        split = it.split;
-      }
+      const int m = place.m, n = place.n, split = place.split;
+      advance<ROLE>(p, place);
       const int64_t row = static_cast<int64_t>(m) * kTile + row_in_pair;
       const int64_t row_warp = row - lane;
       if (S::LOGITS && m != m_now) {
@@ -701,11 +742,9 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           }
         }
       }
-      float final_scale = 0.0f;
       int4 hits = make_int4(-1, -1, -1, -1);  // kGradRows: the queries whose target this base row is
       int n_hits = 0;
       if (ROLE == kGradRows) {
-        final_scale = out_scale(p.row, p.scale);
         if (row < p.piece) {
           n_hits = p.hits[row];
           // A row with more is left as it is: their errors average out, and
@@ -717,7 +756,6 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         n_hits = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n_hits));
       }
       if (ROLE == kGradQ && p.direct) {
-        final_scale = out_scale(p.row, p.scale);
         if (row < p.t) {
           const int64_t y = __ldg(p.targets + row);
           if (counts(y, p.ignore_index, p.v)) hits.x = static_cast<int>(y);
@@ -1173,7 +1211,10 @@ __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
 }
 
 template <int ROLE>
-cudaError_t launch_role(const CUtensorMap* maps, const Args& p, bool bf, int clusters, cudaStream_t stream) {
+cudaError_t launch_role(const CUtensorMap* maps, Args p, bool bf, int clusters, cudaStream_t stream) {
+  p.next_m = clusters % p.m_tiles;
+  p.next_n = clusters / p.m_tiles % p.n_tiles;
+  p.next_split = clusters / p.m_tiles / p.n_tiles;
   constexpr bool kB = ROLE == kStats || ROLE == kWeights;
   const bool bias = kB && p.bias != nullptr;
   auto kern = bf ? (bias ? xent_gemm_kernel<ROLE, true, kB> : xent_gemm_kernel<ROLE, true, false>)
