@@ -434,8 +434,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     bool fresh = true;  // the queries changed
     bool lost = false;  // a wait gave up: the scores that remain are NaN
     // This warp's blocks of 32 columns: grp and grp + 4 of the tile's, block b
-    // being queries b % q_blocks of base rows b / q_blocks.
-    // (Divided once: per tile, the divisions took as long as the scores.)
+    // being queries b % q_blocks of base rows b / q_blocks (divided here, once).
     const int q_blocks = p.n_cols / 32;
     const int row_in_cta = quarter * 32 + lane;
     int sub_of[kBlocks], q_of[kBlocks];  // row group and first query of each block

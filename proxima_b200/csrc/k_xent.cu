@@ -5,8 +5,8 @@
 //     G_ij = g_i (exp(z_ij - lse_i) - [j = y(i)]),  dq = scale * G r,  dr = scale * G^T q
 //
 // Forward: one pass over the products, whose epilogue keeps a running sum of
-// exponentials per query, with its scale, over the other rows; a second kernel joins them. The
-// target's own logit stays out of the sum, so the loss is
+// exponentials per query, with its scale, over the other rows; a second kernel
+// joins them. The target's own logit stays out of the sum, so the loss is
 //     softplus(log sum_{j != y} exp z_ij - z_iy),
 // which does not cancel when the target holds nearly all of the softmax. z_iy
 // is a dot product of its own in the joining kernel, in fp32 with rounding:
@@ -19,6 +19,12 @@
 // the pieces in fp32 slabs (one per split of the piece, added to in the same
 // order every time, so results do not change from run to run), dr is complete
 // per piece.
+// G lies in blocks of 64 columns, each block's rows of 128 bytes behind one
+// another: what a tile writes, and what a load of it reads, is then a run of
+// 16 to 32 KB instead of lines a row of G apart (each of the three kernels 2-4%
+// faster; 200 MB of G through HBM and L2 cost 45 of 1000 x 100k x 384's 326 us).
+// Its rows are padded with zeros to whole K slices of dr, its last block's
+// columns likewise.
 // G's rounding to 16 bits is relative 2^-9 (bf16) or 2^-12 (fp16) of each
 // entry, as the outputs' own. Of thousands of probabilities it averages out;
 // the target's entry, which alone makes up most of a gradient, would carry it
@@ -29,8 +35,11 @@
 //
 // All three products are one kernel, instantiated per role: CTA pairs
 // (tcgen05.mma cta_group::2, kind::f16), 256 M rows per pair, K slices of 64.
-// Operands stream through a ring of twelve 16 KB slots, each with its own
-// barriers. The three read their operands as they lie: G^T, the base as dq's
+// Operands stream through a ring of 16 KB slots (14 in shared memory for the
+// forward, 12 for the others, which stage stores beside them), each with its own
+// barriers. The MMA warp stays converged and one elected lane issues, so that
+// descriptors live in uniform registers: with a lone lane walking the loop the
+// tensor pipe waited for its issuer. The three read their operands as they lie: G^T, the base as dq's
 // right operand and the queries as dr's are MN-major tiles, so nothing is
 // transposed in memory.
 //   Logits (kStats, kWeights): 256 x 256 tiles, two accumulators so that the
@@ -42,7 +51,8 @@
 //   Gradients (kGradQ, kGradRows): tiles as wide as d up to 512 columns, for
 //   the same reason (53 bytes per SM and clock at 384); up to 256 columns the
 //   accumulator is doubled.
-// 16 epilogue warps: four per TMEM quarter, on alternate 32-column blocks.
+// 16 epilogue warps: four per TMEM quarter, on 64 columns each (logits) or on
+// alternate 32-column blocks (gradients).
 //
 // Bound: the tensor pipe for d >= 256 or so (2 t v d operations forward, three
 // times that backward, of which the logits again are the price of not keeping
@@ -110,6 +120,7 @@ static_assert(kStatsSlots * kSlot == kSlots * kSlot + kEpiWarps * kOutBuf, "one 
 struct Args {
   int64_t t, v;
   int d;
+  int g_rows;            // rows per block of G
   int m_tiles, n_tiles;
   int tiles;             // logits: m_tiles * n_tiles; gradients: items
   int per_split;         // kGradQ: K slices per split
@@ -372,9 +383,9 @@ __device__ __forceinline__ void add_row(uint32_t (&v)[32], float f, const uint16
 
 // Where a tile lies. Tiles are numbered along the base, then along the queries
 // (logits), or along M, then N, then the splits (gradients). A pair divides its
-// first tile's number once and counts on from there: an integer division uses
-// the special-function unit, and per tile, behind the exponentials, one took
-// 3500 clocks.
+// first tile's number once and counts on from there; dividing per tile, in the
+// epilogue's warps, costs more than it looks (1000 x 1M x 128 forward: 352
+// against 327 us), as a division takes the unit that the exponentials keep busy.
 struct Place {
   int m, n, split;
 };
@@ -568,10 +579,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           for (int k = k0; k < k1; ++k) {
             if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
             if (S::A_MN) {
-              tc::tma_load_2d_pair(dst, &tm_a, fb, m0, k * kSlice);
-              tc::tma_load_2d_pair(dst + 8192, &tm_a, fb, m0 + 64, k * kSlice);
+              const int block = m0 / kSlice;
+              tc::tma_load_2d_pair(dst, &tm_a, fb, 0, block * p.g_rows + k * kSlice);
+              tc::tma_load_2d_pair(dst + 8192, &tm_a, fb, 0, (block + 1) * p.g_rows + k * kSlice);
             } else {
-              tc::tma_load_2d_pair(dst, &tm_a, fb, k * kSlice, m0);
+              tc::tma_load_2d_pair(dst, &tm_a, fb, 0, k * p.g_rows + m0);
             }
             const int k_row = k * kSlice + (ROLE == kGradQ ? p.v0 : 0);
             if ((dst = next_slot(boxes1 * 8192, fb)) == 0) { ok = false; break; }
@@ -831,7 +843,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       if (ROLE == kWeights) {
         // This warp's 64 columns, packed half by half.
         const int col = n * kTile + group * 64;  // within the piece
-        const bool some = row_warp < p.t && col < p.piece;
+        const bool some = row_warp < p.g_rows && col < p.piece;
         const uint32_t at_tmem = lane_addr + static_cast<uint32_t>(acc * kTile + group * 64);
         auto release = [&]() {
           tc::tc_fence_before();
@@ -853,7 +865,11 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
               for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
             }
             const int col_h = col + 32 * h;
-            if (BIAS) add_bias(v, p.bias + p.v0 + col_h, static_cast<int>(p.v) - p.v0 - col_h, p.c);
+            if (BIAS) {
+              add_bias(v, p.bias + p.v0 + col_h, static_cast<int>(p.v) - p.v0 - col_h, p.c);
+            } else if (p.piece - col_h < 32) {
+              leave_out_from(v, p.piece - col_h);
+            }
             const float c = BIAS ? 1.0f : p.c;
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -884,7 +900,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           for (int h = 0; h < 2; ++h) {
             stage_line(out_buf, lane, h, w);
             if (lane == 0) {
-              tma_store(&tm_out, out_buf, col, static_cast<int>(row_warp) + 16 * h);
+              tma_store(&tm_out, out_buf, 0, col / kSlice * p.g_rows + static_cast<int>(row_warp) + 16 * h);
               store_commit();
             }
           }
@@ -1330,7 +1346,7 @@ struct ForwardPlan {
 
 struct BackwardPlan {
   GradTiles gt;
-  int m_tiles, q_splits;
+  int m_tiles, q_splits, g_rows;
   int64_t piece, slab_rows, ld_slab;  // columns of a piece
   float *top, *rest, *slab;
   int* hits;  // two of `piece`: this piece's, and the next one's being cleared
@@ -1349,7 +1365,8 @@ struct BackwardPlan {
     hits = c.take<int>(2 * piece);
     hit_list = c.take<int4>(piece);
     slab = c.take<float>(q_splits * slab_rows * ld_slab);
-    g = c.take<uint16_t>(t * piece);
+    g_rows = static_cast<int>(align_up(t, kSlice));
+    g = c.take<uint16_t>(g_rows * piece);
     bytes = c.used;
   }
 };
@@ -1482,6 +1499,7 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
   if (e == cudaSuccess && dq_tma) e = encode_rows_map(&dq_map, x.type, dq, x.d, x.t, lddq * 2, 32, 32, 64);
   if (e != cudaSuccess) return e;
   base.rest = plan.rest;
+  base.g_rows = plan.g_rows;
   base.hit_list = plan.hit_list;
   if (drows != nullptr) {
     e = cudaMemsetAsync(plan.hits, 0, sizeof(int) * static_cast<size_t>(plan.piece), stream);
@@ -1499,9 +1517,10 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
     base.next_hits = plan.hits + (turn ^ 1) * plan.piece;
     turn ^= 1;
     CUtensorMap g_k, g_mn, g_out;
-    e = encode_rows_map(&g_k, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kHalf, 128);
-    if (e == cudaSuccess) e = encode_rows_map(&g_mn, x.type, plan.g, piece, x.t, plan.piece * 2, kSlice, kSlice, 128);
-    if (e == cudaSuccess) e = encode_rows_map(&g_out, x.type, plan.g, piece, x.t, plan.piece * 2, 64, 16, 128);
+    const int64_t g_all = ceil_div(piece, kSlice) * plan.g_rows;
+    e = encode_rows_map(&g_k, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, kHalf, 128);
+    if (e == cudaSuccess) e = encode_rows_map(&g_mn, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, kSlice, 128);
+    if (e == cudaSuccess) e = encode_rows_map(&g_out, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, 16, 128);
     if (e != cudaSuccess) return e;
     Args p = base;
     logits_args(p, bf, plan.m_tiles, piece_n);

@@ -368,6 +368,35 @@ def test_softmax_several_pieces_with_shared_targets(px):
     _check_xent(px, q, r, y, b, weights=torch.linspace(0.5, 2, t, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("t,v,d", [(1, 1, 8), (5, 70, 40), (65, 250, 64), (200, 5001, 100), (333, 520_009, 16)])
+def test_softmax_results_do_not_depend_on_what_workspaces_held(px, monkeypatch, dtype, t, v, d):
+    # All logits near -1000, so that a logit of 0 past the base's end would
+    # weigh infinitely much.
+    q = _rand(t, d, seed=71, dtype=dtype) * 0.05 + 8
+    r = _rand(v, d, seed=72, dtype=dtype) * 0.05 - 1000 / 8 / d
+    y = torch.arange(t, device="cuda") * 7 % v
+    real = torch.empty
+
+    def step(bits):
+        def filled(*args, **kw):
+            x = real(*args, **kw)
+            if x.is_cuda:
+                x.fill_(bits if x.dtype == torch.uint8 else math.nan if bits else 0.0)
+            return x
+
+        monkeypatch.setattr(torch, "empty", filled)
+        a, b = q.clone().requires_grad_(), r.clone().requires_grad_()
+        loss = px.softmax_cross_entropy(a, b, y)
+        loss.backward()
+        monkeypatch.setattr(torch, "empty", real)
+        return loss, a.grad, b.grad
+
+    want = step(0)
+    assert all(x.isfinite().all() for x in want)
+    assert all(torch.equal(x, w) for x, w in zip(step(255), want))
+
+
 def test_softmax_unpitched_and_strided_operands(px):
     q, r, y, b = _xent_case(70, 300, 50, torch.bfloat16, 31, bias=True)
     q2, r2, _, _ = _xent_case(70, 300, 50, torch.bfloat16, 31, bias=True, pitch=False)  # rows of 100 bytes
