@@ -16,14 +16,19 @@
 // is what remains. So the queries are kept in shared memory across base tiles
 // where they fit (KC slices of N/2 rows; d <= 896 at N = 256), and only base
 // rows stream through the ring.
+// Measured, fp32 out: 64 x 1M x 128 in 75 us and 1000 x 100k x 384 in 98 us,
+// 0.79 and 0.69 of what their bytes take at a copy's rate; runs of 512 bytes
+// per row of `out` are what keeps the writes from more. bf16 out: 10k x 100k x
+// 768 in 800 us, 1.92 POP/s; 640 us without its stores and 544 us with no
+// epilogue at all, under the power cap (677 us when the GPU is cool), where
+// the 2 GB of scores cost energy as well as time.
 //
 // Order. Clusters form teams. The clusters of a team take neighbouring base
 // tiles of one query group, so what is written at any time is long runs of 256
 // rows of `out`: with a run of base tiles per cluster, whose writes lie far
 // apart, plain stores of a 400 MB matrix reach 3.9 TB/s, with neighbouring
 // tiles 5-6. The teams take different query groups at the same base tiles, so
-// that they share what is read from HBM (10k queries against 100k x 768 in two
-// teams read the base 20 times).
+// that they share what is read from HBM.
 //
 // CTA roles (576 threads): warp 0 TMA producer, warp 1 TMEM owner and (even
 // CTA) MMA issuer, warps 2-17 epilogue: four per TMEM quarter, on alternate
