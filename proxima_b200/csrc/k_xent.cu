@@ -1523,6 +1523,7 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
     turn ^= 1;
     CUtensorMap g_k, g_mn, g_out;
     const int64_t g_all = ceil_div(piece, kSlice) * plan.g_rows;
+    if (g_all > 0x7fffff00) return cudaErrorInvalidValue;  // TMA coordinates are 32-bit (a G of 275 GB)
     e = encode_rows_map(&g_k, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, kHalf, 128);
     if (e == cudaSuccess) e = encode_rows_map(&g_mn, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, kSlice, 128);
     if (e == cudaSuccess) e = encode_rows_map(&g_out, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, 16, 128);
