@@ -455,8 +455,8 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         const int sub = sub_of[k];
         const int64_t r = (static_cast<int64_t>(tile) * p.subs + sub) * (2 * kRows) + rank * kRows + row_in_cta;
         const bool live = sub < p.subs && r < p.n;
-        next_xs[k] = live ? __ldg(p.x_scale + r) : 0.0f;
-        next_bias[k] = live && p.bias != nullptr ? __ldg(p.bias + r) : 0.0f;
+        next_xs[k] = live ? p.x_scale[r] : 0.0f;
+        next_bias[k] = live && p.bias != nullptr ? p.bias[r] : 0.0f;
       }
     };
     load_rows(bt);
@@ -470,7 +470,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) {
           const int64_t qi = q0 + q_of[k] + lane;
-          scale[k * 32 + lane] = qi < p.m ? __ldg(p.q_scale + qi) : 0.0f;
+          scale[k * 32 + lane] = qi < p.m ? p.q_scale[qi] : 0.0f;
         }
         __syncwarp();
         fresh = false;

@@ -32,6 +32,7 @@ namespace px {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 4;  // loads in flight per thread, ahead of the stores
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
@@ -115,9 +116,9 @@ __device__ __forceinline__ uint32_t four_codes(const RowScale& r, const float* x
 // VB: bytes per load; NV: loads per lane. A row's values stay in registers, at
 // most 32 per lane.
 template <typename T, int VB, int NV>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, int64_t n, int d, int64_t ldx,
-                                                                 int8_t* __restrict__ codes, int64_t ldc,
-                                                                 float* __restrict__ scales, int group, bool vec_out) {
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* x, int64_t n, int d, int64_t ldx,
+                                                                 int8_t* codes, int64_t ldc, float* scales, int group,
+                                                                 bool vec_out) {
   constexpr int VE = VB / static_cast<int>(sizeof(T));
   using W = typename Word<VB>::type;
   wait_for_previous();
@@ -133,13 +134,13 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
   for (int i = 0; i < NV; ++i) {
     const int at = (i * group + lane) * VE;
     if (live && at + VE <= d) {
-      const W w = __ldg(reinterpret_cast<const W*>(xr + at));
+      const W w = *reinterpret_cast<const W*>(xr + at);
       const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
       for (int j = 0; j < VE; ++j) v[i][j] = to_f32(e[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < VE; ++j) v[i][j] = live && at + j < d ? to_f32(__ldg(xr + at + j)) : 0.0f;
+      for (int j = 0; j < VE; ++j) v[i][j] = live && at + j < d ? to_f32(xr[at + j]) : 0.0f;
     }
   }
 #pragma unroll
@@ -181,9 +182,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
 // Rows longer than a group's registers hold: a block per row, which reads the
 // row twice (the second time from cache).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* __restrict__ x, int64_t n, int d,
-                                                                      int64_t ldx, int8_t* __restrict__ codes,
-                                                                      int64_t ldc, float* __restrict__ scales) {
+__global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* x, int64_t n, int d, int64_t ldx,
+                                                                      int8_t* codes, int64_t ldc, float* scales) {
   __shared__ float s_peak[kThreads / 32];
   wait_for_previous();
   let_next_start();
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* _
     const T* xr = x + row * ldx;
     float peak = 0.0f;
 #pragma unroll 8
-    for (int j = threadIdx.x; j < d; j += kThreads) peak = max_abs(peak, to_f32(__ldg(xr + j)));
+    for (int j = threadIdx.x; j < d; j += kThreads) peak = max_abs(peak, to_f32(xr[j]));
     for (int s = 16; s > 0; s >>= 1) peak = max_abs(peak, __shfl_xor_sync(0xffffffffu, peak, s));
     if ((threadIdx.x & 31) == 0) s_peak[threadIdx.x >> 5] = peak;
     __syncthreads();
@@ -201,16 +201,21 @@ __global__ void __launch_bounds__(kThreads) quantize_long_rows_kernel(const T* _
     const RowScale r(peak);
     if (threadIdx.x == 0) scales[row] = r.scale;
     int8_t* out = codes + row * ldc;
-#pragma unroll 8
-    for (int j = threadIdx.x; j < d; j += kThreads) out[j] = static_cast<int8_t>(r.code(to_f32(__ldg(xr + j))));
+    for (int j0 = threadIdx.x; j0 < d; j0 += kAhead * kThreads) {
+      float v[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) v[i] = j0 + i * kThreads < d ? to_f32(xr[j0 + i * kThreads]) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (j0 + i * kThreads < d) out[j0 + i * kThreads] = static_cast<int8_t>(r.code(v[i]));
+    }
   }
 }
 
 // VE codes at a time; a group of lanes takes a row, as above.
 template <typename T, int VE>
-__global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const int8_t* __restrict__ codes, int64_t ldc,
-                                                                   const float* __restrict__ scales, int64_t n, int d,
-                                                                   T* __restrict__ out, int64_t ldo, int group) {
+__global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const int8_t* codes, int64_t ldc, const float* scales,
+                                                                   int64_t n, int d, T* out, int64_t ldo, int group) {
   using C = typename Word<VE>::type;
   using W = typename Word<VE * static_cast<int>(sizeof(T))>::type;
   wait_for_previous();
@@ -218,21 +223,28 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const int8_t*
   const int lane = threadIdx.x & (group - 1);
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
   if (row >= n) return;
-  const float s = __ldg(scales + row);
+  const float s = scales[row];
   const int8_t* c = codes + row * ldc;
   T* o = out + row * ldo;
-#pragma unroll 4
-  for (int at = lane * VE; at < d; at += group * VE) {
-    if (at + VE <= d) {
-      const C w = __ldg(reinterpret_cast<const C*>(c + at));
-      const int8_t* e = reinterpret_cast<const int8_t*>(&w);
-      W r;
-      T* p = reinterpret_cast<T*>(&r);
+  const int step = group * VE;
+  for (int at0 = lane * VE; at0 < d; at0 += kAhead * step) {
+    C w[kAhead];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) p[j] = from_f32<T>(static_cast<float>(e[j]) * s);
-      *reinterpret_cast<W*>(o + at) = r;
-    } else {
-      for (int j = at; j < d; ++j) o[j] = from_f32<T>(static_cast<float>(__ldg(c + j)) * s);
+    for (int i = 0; i < kAhead; ++i)
+      if (at0 + i * step + VE <= d) w[i] = *reinterpret_cast<const C*>(c + at0 + i * step);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = at0 + i * step;
+      if (at + VE <= d) {
+        const int8_t* e = reinterpret_cast<const int8_t*>(&w[i]);
+        W r;
+        T* p = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) p[j] = from_f32<T>(static_cast<float>(e[j]) * s);
+        *reinterpret_cast<W*>(o + at) = r;
+      } else {
+        for (int j = at; j < d; ++j) o[j] = from_f32<T>(static_cast<float>(c[j]) * s);
+      }
     }
   }
 }

@@ -206,21 +206,21 @@ __device__ __forceinline__ bool counts(int64_t y, int64_t ignore_index, int64_t 
 // A query's factor: its gradient relative to the largest, lifted; 0 for one
 // that adds nothing.
 __device__ __forceinline__ float row_factor(const RowGrad& r, bool used, int64_t t) {
-  const float top = fabsf(__ldg(r.top));
+  const float top = fabsf(*r.top);
   if (!used || top == 0.0f) return 0.0f;
-  return __ldg(r.grad + t * r.grad_stride) / top * r.lift;
+  return r.grad[t * r.grad_stride] / top * r.lift;
 }
 
 // What the products of G are multiplied by at the end.
 __device__ __forceinline__ float out_scale(const RowGrad& r, float scale) {
-  const float top = fabsf(__ldg(r.top));
-  return top * scale / r.lift / (r.divisor != nullptr ? __ldg(r.divisor) : 1.0f);
+  const float top = fabsf(*r.top);
+  return top * scale / r.lift / (r.divisor != nullptr ? *r.divisor : 1.0f);
 }
 
 // The target's entry: exp(-loss) - 1 is its share minus one, without
 // cancellation.
 __device__ __forceinline__ float target_entry(const RowGrad& r, int64_t t, float factor) {
-  return expm1f(-__ldg(r.loss + t)) * factor;
+  return expm1f(-r.loss[t]) * factor;
 }
 
 __device__ __forceinline__ float largest(const uint32_t (&v)[32]) {
@@ -266,7 +266,7 @@ __device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, i
     const float4* b4 = reinterpret_cast<const float4*>(bias);
 #pragma unroll
     for (int j4 = 0; j4 < 8; ++j4) {
-      const float4 b = __ldg(b4 + j4);
+      const float4 b = b4[j4];
       v[4 * j4] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4]), c, bias2(b.x)));
       v[4 * j4 + 1] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 1]), c, bias2(b.y)));
       v[4 * j4 + 2] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 2]), c, bias2(b.z)));
@@ -275,7 +275,7 @@ __device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, i
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      v[j] = __float_as_uint(j < left ? fmaf(__uint_as_float(v[j]), c, bias2(__ldg(bias + j))) : -kInf);
+      v[j] = __float_as_uint(j < left ? fmaf(__uint_as_float(v[j]), c, bias2(bias[j])) : -kInf);
   }
 }
 
@@ -370,7 +370,7 @@ __device__ __forceinline__ void add_row(uint32_t (&v)[32], float f, const uint16
     const uint4* x4 = reinterpret_cast<const uint4*>(x);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint4 a = __ldg(x4 + k);
+      const uint4 a = x4[k];
       const uint32_t u[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -382,7 +382,7 @@ __device__ __forceinline__ void add_row(uint32_t (&v)[32], float f, const uint16
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j < left) v[j] = __float_as_uint(fmaf(f, widen2<BF>(__ldg(x + j)).x, __uint_as_float(v[j])));
+      if (j < left) v[j] = __float_as_uint(fmaf(f, widen2<BF>(x[j]).x, __uint_as_float(v[j])));
   }
 }
 
@@ -746,13 +746,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         target = -1;
         factor = 0.0f;
         if (row < p.t) {
-          const int64_t y = __ldg(p.targets + row);
+          const int64_t y = p.targets[row];
           const bool used = counts(y, p.ignore_index, p.v);
           if (used) target = static_cast<int>(y) - p.v0;
           if (ROLE == kWeights) {
             // G = factor * 2^(logit - lse) = +-2^(logit + shift); no row takes part
             // where lse is -inf.
-            const float l = __ldg(p.row.lse + row);
+            const float l = p.row.lse[row];
             factor = row_factor(p.row, used, row);
             shift = l == -kInf || factor == 0.0f ? -kInf : log2f(fabsf(factor)) - l * kLog2e;
             at_target = target_entry(p.row, row, factor);
@@ -774,7 +774,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       }
       if (ROLE == kGradQ && p.direct) {
         if (row < p.t) {
-          const int64_t y = __ldg(p.targets + row);
+          const int64_t y = p.targets[row];
           if (counts(y, p.ignore_index, p.v)) hits.x = static_cast<int>(y);
         }
         n_hits = 1;
@@ -962,7 +962,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             for (int h = 0; h < n_hits; ++h) {
               const int t = h == 0 ? hits.x : h == 1 ? hits.y : h == 2 ? hits.z : hits.w;
               if (t >= 0) {
-                const float rest = __ldg(p.rest + (ROLE == kGradQ ? row : t));
+                const float rest = p.rest[ROLE == kGradQ ? row : t];
                 add_row<BF>(v, rest, p.other + t * p.ldother + col, p.d - col);
               }
             }
@@ -1013,8 +1013,8 @@ __device__ __forceinline__ float warp_dot(const uint16_t* q, const uint16_t* r, 
   float s = 0.0f;
   for (int at = lane * 8; at < d; at += 256) {
     if (at + 8 <= d) {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(q + at));
-      const uint4 b = __ldg(reinterpret_cast<const uint4*>(r + at));
+      const uint4 a = *reinterpret_cast<const uint4*>(q + at);
+      const uint4 b = *reinterpret_cast<const uint4*>(r + at);
       const uint32_t u[4] = {a.x, a.y, a.z, a.w}, w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -1023,7 +1023,7 @@ __device__ __forceinline__ float warp_dot(const uint16_t* q, const uint16_t* r, 
         s = fmaf(x.y, y.y, s);
       }
     } else {
-      for (int j = at; j < d; ++j) s = fmaf(widen2<BF>(__ldg(q + j)).x, widen2<BF>(__ldg(r + j)).x, s);
+      for (int j = at; j < d; ++j) s = fmaf(widen2<BF>(q[j]).x, widen2<BF>(r[j]).x, s);
     }
   }
 #pragma unroll
@@ -1062,11 +1062,11 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
     const int64_t m = row / kTile;
     const int used = kGroups * (run_of(p.tiles, (m + 1) * p.n_tiles - 1, p.pairs) - run_of(p.tiles, m * p.n_tiles, p.pairs) + 1);
     // The target's logit, before what does not depend on it.
-    const int64_t y = __ldg(p.targets + row);
+    const int64_t y = p.targets[row];
     float zt = 0.0f;
     if (counts(y, p.ignore_index, p.v)) {
       zt = warp_dot<BF>(p.q + row * p.ldq, p.rows + y * p.ldr, p.d, lane) * p.scale;
-      if (p.bias != nullptr) zt += bias2(__ldg(p.bias + y)) * kLn2;
+      if (p.bias != nullptr) zt += bias2(p.bias[y]) * kLn2;
     }
     const float2* pr = p.part + row * p.lists;
     float top = -kInf;
@@ -1110,7 +1110,7 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
   long long count = 0;
 #pragma unroll 8
   for (int64_t i = threadIdx.x; i < p.t; i += 256) {
-    const bool in = __ldg(p.targets + i) != p.ignore_index;
+    const bool in = p.targets[i] != p.ignore_index;
     const float l = __ldcg(p.loss + i);
     sum += in ? l : 0.0f;
     count += in;
@@ -1137,9 +1137,8 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
 }
 
 // One block: the largest |grad| of the queries that count.
-__global__ void __launch_bounds__(1024) xent_top_kernel(const float* __restrict__ grad,
-                                                        const int64_t* __restrict__ targets, int64_t ignore_index,
-                                                        int64_t t, int64_t v, float* __restrict__ out) {
+__global__ void __launch_bounds__(1024) xent_top_kernel(const float* grad, const int64_t* targets,
+                                                        int64_t ignore_index, int64_t t, int64_t v, float* out) {
   __shared__ float s_top[32];
   float top = 0.0f;
   wait_for_previous();
@@ -1154,6 +1153,16 @@ __global__ void __launch_bounds__(1024) xent_top_kernel(const float* __restrict_
     for (int w = 1; w < 32; ++w) top = fmaxf(top, s_top[w]);
     out[0] = top;
   }
+}
+
+// Four values that nobody reads again.
+__device__ __forceinline__ float4 load_once(const float4* p) {
+  float4 r;
+  asm volatile("ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w)
+               : "l"(p)
+               : "memory");
+  return r;
 }
 
 struct GradQArgs {
@@ -1191,11 +1200,11 @@ __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
     if (row >= p.t) break;
     const int col = (i - r_in * quads) * 4;
     const float4* s = reinterpret_cast<const float4*>(p.slab + row * p.ld_slab + col);
-    const int64_t y = __ldg(p.targets + row);
-    float4 sum = __ldcs(s);
+    const int64_t y = p.targets[row];
+    float4 sum = load_once(s);
 #pragma unroll 6
     for (int k = 1; k < p.splits; ++k) {
-      const float4 w = __ldcs(s + k * step);
+      const float4 w = load_once(s + k * step);
       sum.x += w.x;
       sum.y += w.y;
       sum.z += w.z;
@@ -1203,10 +1212,10 @@ __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
     }
     float r[4] = {sum.x, sum.y, sum.z, sum.w};
     if (counts(y, p.ignore_index, p.v)) {
-      const float rest = __ldg(p.rest + row);
+      const float rest = p.rest[row];
       const uint16_t* x = p.rows + y * p.ldr + col;
       if (col + 4 <= p.d) {  // rows start on 16-byte boundaries
-        const uint2 u = __ldg(reinterpret_cast<const uint2*>(x));
+        const uint2 u = *reinterpret_cast<const uint2*>(x);
         const float2 a = widen2<BF>(u.x), b = widen2<BF>(u.y);
         r[0] = fmaf(rest, a.x, r[0]);
         r[1] = fmaf(rest, a.y, r[1]);
@@ -1215,7 +1224,7 @@ __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (col + j < p.d) r[j] = fmaf(rest, widen2<BF>(__ldg(x + j)).x, r[j]);
+          if (col + j < p.d) r[j] = fmaf(rest, widen2<BF>(x[j]).x, r[j]);
       }
     }
     const uint32_t lo = pack2<BF>(r[0] * f, r[1] * f), hi = pack2<BF>(r[2] * f, r[3] * f);

@@ -9,7 +9,10 @@ namespace px {
 // that each may start its prologue (barriers, tensor memory, descriptors)
 // while the one before it finishes; every thread passes this wait, which
 // returns when that one has completed and its writes are visible, before it
-// touches global memory.
+// touches global memory. What an earlier kernel may have written is read by
+// ordinary loads, never through the read-only path (__ldg, const __restrict__):
+// that asks for memory which does not change while the kernel is there, its
+// prologue included, and lets the compiler move a load up past the wait.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -594,6 +594,33 @@ def test_results_do_not_change_between_runs(px):
 
 # ---------------------------------------------------------------- streams, graphs, devices
 
+def test_calls_in_a_row_see_what_the_last_one_wrote(px):
+    # The same buffers with other values each time, with no wait between: each
+    # kernel starts while the one before it ends.
+    n, m, d = 20_000, 64, 128
+    bases = [_rand(n, d, seed=80 + i) * 4.0 ** i for i in range(4)]
+    q = _rand(m, d, seed=79)
+    y = torch.arange(m, device="cuda")
+
+    def step(base):
+        codes, scales = px.quantize_rows(base)
+        back = px.dequantize_rows(codes, scales)
+        qc, qs = px.quantize_rows(q)
+        scores = px.int8_scores(qc, qs, codes, scales)
+        a, b = q.bfloat16().requires_grad_(), back.bfloat16().requires_grad_()
+        loss = px.softmax_cross_entropy(a, b, y, scale=0.01)
+        return (back, scores, loss.detach(), *torch.autograd.grad(loss, (a, b)))
+
+    want = []
+    for base in bases:
+        want.append(step(base))
+        torch.cuda.synchronize()
+    for i in [1, 0, 3, 2] * 5:
+        assert all(torch.equal(x, w) for x, w in zip(step(bases[i]), want[i]))
+    # Half a scale, and two roundings (the scale's, the product's) of at most 127 scales.
+    _within(want[2][0], bases[2].double(), (0.5 + 2 * 127 * 2 * U) * bases[2].abs().amax(1, keepdim=True).double() / 127)
+
+
 def test_row_operators_on_other_streams(px):
     """Two streams at once, each with its own inputs, against the default
     stream's results."""
