@@ -7,8 +7,8 @@
 // Layout. A cluster of two CTAs computes 256 base rows x N queries per tile
 // (N <= 256) with cta_group::2: base rows are the M side, one TMEM lane each,
 // so the 32 lanes of an epilogue warp hold 32 neighbouring base rows of one
-// query and every store is a run of a row of `out` straight from registers,
-// with no transposition through shared memory. Each CTA stages its 128 base
+// query, and four warps put a query's 128 of them side by side in shared memory
+// without transposing: a run of 256 or 512 bytes of a row of `out`. Each CTA stages its 128 base
 // rows and half of the queries in slices of 128 codes (128-byte swizzle).
 //
 // What bounds it: the matrix itself. At 4 bytes a score the write takes longer
@@ -56,7 +56,8 @@ constexpr int kMaxStages = 12;
 constexpr int kGroups = 4;        // epilogue warps per TMEM quarter
 constexpr int kEpiWarps = 4 * kGroups;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kOutBuf = 8192;     // staging of an epilogue group's stores
+constexpr int kOutBuf = 8192;     // staging of an epilogue group's stores by TMA,
+constexpr int kRaggedBuf = 8704;  // or of others: two halves of 8 fp32 or 16 16-bit rows and 16 bytes each
 constexpr int kBlocks = 256 / 32 / kGroups;  // blocks of 32 columns per epilogue warp
 constexpr int kWarpScales = 256 / kGroups;  // query scales an epilogue warp needs
 constexpr int kMaxAccs = 8;
@@ -83,15 +84,6 @@ struct Params {
 };
 
 template <typename T>
-__device__ __forceinline__ T narrow(float x);
-template <>
-__device__ __forceinline__ float narrow<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
-template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
@@ -107,69 +99,6 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 __device__ __forceinline__ F2 two_scores(const uint32_t (&v)[32], int j, float w0, float w1, F2 xs, F2 bias) {
   return fma2(f2(static_cast<float>(static_cast<int>(v[j])), static_cast<float>(static_cast<int>(v[j + 1]))),
               mul2(f2(w0, w1), xs), bias);
-}
-
-// A pair's word of 16-bit scores: the even lane's both rows of query j, the
-// odd lane's of query j + 1.
-template <typename OT>
-__device__ __forceinline__ uint32_t trade(float s0, float s1, int odd) {
-  const uint32_t mine = pack2<OT>(s0, s1);
-  const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-  return __byte_perm(mine, other, odd ? 0x3276 : 0x5410);
-}
-
-// Stores a block's scores, all 32 base rows of the warp being real. SOME: only
-// the first `count` queries are. The stores evict first: the matrix is larger
-// than what L2 should keep for the base.
-template <typename OT, bool PAIR, int SOME>
-__device__ __forceinline__ void store_queries(const uint32_t (&v)[32], const float* qs, float xs, float bias, OT* o,
-                                              int64_t ldo, int odd, int count) {
-  const float4* qs4 = reinterpret_cast<const float4*>(qs);
-  const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
-#pragma unroll
-  for (int j4 = 0; j4 < 8; ++j4) {
-    if (SOME && 4 * j4 >= count) break;
-    const float4 w = qs4[j4];
-    float s[4];
-    unpack(two_scores(v, 4 * j4, w.x, w.y, xs2, bias2), s[0], s[1]);
-    unpack(two_scores(v, 4 * j4 + 2, w.z, w.w, xs2, bias2), s[2], s[3]);
-    if constexpr (PAIR) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t word = trade<OT>(s[2 * h], s[2 * h + 1], odd);
-        if (!SOME || 4 * j4 + 2 * h + odd < count) __stcs(reinterpret_cast<uint32_t*>(o), word);
-        o += 2 * ldo;
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        if (!SOME || 4 * j4 + h < count) __stcs(o, narrow<OT>(s[h]));
-        o += ldo;
-      }
-    }
-  }
-}
-
-// The same for the base's last rows.
-template <typename OT, bool PAIR>
-__device__ __forceinline__ void store_ragged(const uint32_t (&v)[32], const float* qs, float xs, float bias, OT* o,
-                                             int64_t ldo, int odd, int count, int keep) {
-  const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
-#pragma unroll
-  for (int j = 0; j < 32; j += 2) {
-    if (j >= count) break;
-    float s0, s1;
-    unpack(two_scores(v, j, qs[j], qs[j + 1], xs2, bias2), s0, s1);
-    if constexpr (PAIR) {
-      const uint32_t word = trade<OT>(s0, s1, odd);
-      if (j + odd < count && keep == 2) *reinterpret_cast<uint32_t*>(o) = word;
-      if (j + odd < count && keep == 1) *reinterpret_cast<unsigned short*>(o) = static_cast<unsigned short>(word);
-    } else {
-      if (keep > 0) *o = narrow<OT>(s0);
-      if (keep > 0 && j + 1 < count) o[ldo] = narrow<OT>(s1);
-    }
-    o += 2 * ldo;
-  }
 }
 
 // Arrive and wait of one epilogue group's four warps.
@@ -227,10 +156,128 @@ __device__ __forceinline__ void stage_queries(const uint32_t (&v)[32], const flo
   }
 }
 
+// The same for a matrix that TMA cannot address (rows that begin or end off
+// 16-byte boundaries): the warps store the rows of 128 scores themselves, in
+// aligned 16-byte pieces and single scores at either end. A row lies in the
+// buffer as far from a boundary as in `out`, so pieces are read whole. Stored
+// straight from registers, 32 scores of a query per instruction, most of a
+// row's sectors are written in two parts: fp32, 1308 x 543k x 176, 1155 us
+// against 747; bf16, 6269 x 94k x 264, 583 against 444; where little is written
+// this is slower (fp16, 2705 x 49k x 80: 100 against 114). Tiles that overlap,
+// so that a CTA stores whole sectors only, gained nothing.
+// How far rows begin past a boundary repeats every kPiece queries, so that each
+// thread works out once where its scores go and which pieces it stores.
+template <typename OT>
+struct Ragged {
+  static constexpr int kSize = static_cast<int>(sizeof(OT)), kPiece = 16 / kSize;  // scores per piece
+  static constexpr int kPitch = kRows * kSize + 16;
+  static constexpr uint32_t kHalf = kRaggedBuf / 2;
+  static constexpr int kQueries = kRaggedBuf / 2 / kPitch / 4 * 4;  // per half of the buffer
+  static constexpr int kLanes = kRows / kPiece, kAtOnce = 32 / kLanes;  // lanes per row, rows per instruction
+  static constexpr int kPerWarp = kQueries / 4 / kAtOnce;
+  static_assert(kQueries % kPiece == 0 && (32 / kQueries) % 2 == 0, "parts");
+  uint32_t place[kPiece];    // this thread's score of query j (modulo kPiece), in the buffer's first half
+  uint32_t row[kPerWarp];    // where the rows this thread stores from begin there
+  int piece[kPerWarp];       // the first score of its piece of a row
+  int edge[kPerWarp];        // and the single one it stores of a whole row, or -1
+  int in_part;               // its first row
+
+  __device__ __forceinline__ Ragged(const OT* out, int64_t ldo, uint32_t buf, int row_in_tile) {
+    const uint32_t step = static_cast<uint32_t>(ldo) * kSize;
+    const uint32_t first = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out));
+    const int lane = row_in_tile & 31, l = lane % kLanes;
+    in_part = (row_in_tile >> 5) * kPerWarp * kAtOnce + lane / kLanes;
+#pragma unroll
+    for (int j = 0; j < kPiece; ++j) place[j] = buf + row_in_tile * kSize + ((first + j * step) & 15);
+#pragma unroll
+    for (int i = 0; i < kPerWarp; ++i) {
+      const int j = in_part + i * kAtOnce;
+      const uint32_t past = (first + j * step) & 15;
+      const int head = static_cast<int>((16 - past) & 15) / kSize;  // scores before the first boundary
+      row[i] = buf + j * kPitch + past;
+      piece[i] = head + l * kPiece;
+      edge[i] = l < head ? l : l >= kPiece && l - kPiece < kPiece - head && head > 0 ? kRows - 2 * kPiece + head + l : -1;
+    }
+  }
+
+  static __device__ __forceinline__ void single(OT* to, uint32_t from) {
+    if constexpr (kSize == 4) {
+      float x;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(from));
+      *reinterpret_cast<float*>(to) = x;
+    } else {
+      unsigned short x;
+      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(from));
+      *reinterpret_cast<unsigned short*>(to) = x;
+    }
+  }
+
+  // A block's scores: `count` queries of `rows` base rows, out the first's.
+  __device__ __forceinline__ void store(const uint32_t (&v)[32], const float* qs, float xs, float bias, int grp,
+                                        int count, OT* out, int64_t ldo, int rows) const {
+    const float4* qs4 = reinterpret_cast<const float4*>(qs);
+    const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
+#pragma unroll
+    for (int part = 0; part < 32 / kQueries; ++part) {
+      if (part * kQueries >= count) {
+        // The next block begins with the first half again, which the last part read.
+        if (part & 1) group_sync(grp);
+        break;
+      }
+#pragma unroll
+      for (int i = 0; i < kQueries / 4; ++i) {
+        const int j = part * kQueries + 4 * i;
+        const float4 w = qs4[j / 4];
+        float s[4];
+        unpack(two_scores(v, j, w.x, w.y, xs2, bias2), s[0], s[1]);
+        unpack(two_scores(v, j + 2, w.z, w.w, xs2, bias2), s[2], s[3]);
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const uint32_t at0 = place[(j + k) % kPiece], at1 = place[(j + k + 1) % kPiece];
+          const uint32_t add = (part & 1) * kHalf + (4 * i + k) * kPitch;
+          if constexpr (kSize == 4) {
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at0 + add), "f"(s[k]) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at1 + add + kPitch), "f"(s[k + 1]) : "memory");
+          } else {
+            const uint32_t both = pack2<OT>(s[k], s[k + 1]);
+            asm volatile("st.shared.b16 [%0], %1;" ::"r"(at0 + add), "h"(static_cast<unsigned short>(both)) : "memory");
+            asm volatile("st.shared.b16 [%0], %1;" ::"r"(at1 + add + kPitch), "h"(static_cast<unsigned short>(both >> 16))
+                         : "memory");
+          }
+        }
+      }
+      // Also: every warp has read what the other half held.
+      group_sync(grp);
+#pragma unroll
+      for (int i = 0; i < kPerWarp; ++i) {
+        const int j = part * kQueries + in_part + i * kAtOnce;
+        if (j >= count) continue;
+        OT* to = out + j * ldo;
+        const uint32_t from = row[i] + (part & 1) * kHalf;
+        if (piece[i] + kPiece <= rows) {
+          uint4 x;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                       : "r"(from + piece[i] * kSize));
+          __stcs(reinterpret_cast<uint4*>(to + piece[i]), x);
+        }
+        if (rows == kRows) {
+          if (edge[i] >= 0) single(to + edge[i], from + edge[i] * kSize);
+        } else {
+          // The base's last rows: those before the first boundary, and past the last whole piece.
+          const int l = (threadIdx.x & 31) % kLanes, head = piece[i] - l * kPiece;
+          if (l < min(head, rows)) single(to + l, from + l * kSize);
+          if (piece[i] < rows && piece[i] + kPiece > rows)
+            for (int e = piece[i]; e < rows; ++e) single(to + e, from + e * kSize);
+        }
+      }
+    }
+  }
+};
+
 // TMA: `out` can be stored by TMA (rows of whole 16-byte pieces, on 16-byte
-// boundaries). Otherwise PAIR: 16-bit scores leave in pairs of base rows (out
-// and its rows 4-byte aligned).
-template <typename OT, bool PAIR, bool TMA>
+// boundaries).
+template <typename OT, bool TMA>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_q,
                    const __grid_constant__ CUtensorMap tm_out, const Params p) {
@@ -239,7 +286,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int b_slice = p.n_cols / 2 * kSlice;  // bytes of a slice of this CTA's queries
   const int b_bytes = p.resident ? p.kc * b_slice : 0;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + b_bytes + p.stages * p.stage_bytes + (TMA ? kGroups * kOutBuf : 0));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + b_bytes + p.stages * p.stage_bytes + kGroups * (TMA ? kOutBuf : kRaggedBuf));
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   float* s_scale = reinterpret_cast<float*>(s_tmem + 4);
@@ -432,6 +479,8 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     float* scale = s_scale + (warp - 2) * kWarpScales;
     const uint32_t out_buf = ring + p.stages * p.stage_bytes + grp * kOutBuf;
+    const uint32_t ragged_buf = ring + p.stages * p.stage_bytes + grp * kRaggedBuf;
+    const Ragged<OT> ragged(static_cast<const OT*>(p.out), p.ldo, ragged_buf, quarter * 32 + lane);
     OT* out = static_cast<OT*>(p.out);
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -492,10 +541,9 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         const int b = grp + kGroups * k;
         const int sub = sub_of[k], q_in = q_of[k];
         const int64_t row_cta = (static_cast<int64_t>(bt) * p.subs + sub) * (2 * kRows) + rank * kRows;
-        const int64_t row = row_cta + row_in_cta, row_warp = row - lane;
-        // With TMA all four warps of a group take part, base rows or not: they
-        // meet at barriers, and TMA leaves out what lies past the matrix.
-        if (sub >= p.subs || q_in >= queries || (TMA ? row_cta >= p.n : row_warp >= p.n)) continue;  // warp-uniform
+        // All four warps of a group take part, base rows or not: they meet at
+        // barriers, and what lies past the matrix is left out.
+        if (sub >= p.subs || q_in >= queries || row_cta >= p.n) continue;  // uniform in the group
         __syncwarp();
         uint32_t v[32];
         tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * acc_cols + b * 32), v);
@@ -515,23 +563,8 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
           stage_queries<OT>(v, qs, row_scale, bias[k], out_buf, row_in_cta, grp, count, &tm_out,
                             static_cast<int>(row_cta), static_cast<int>(qb));
         } else {
-          // Lanes 2i and 2i + 1 trade 16-bit scores when these leave in pairs:
-          // the even one stores both rows' of query j, the odd one of j + 1.
-          const int odd = PAIR ? lane & 1 : 0;
-          OT* o = out + (qb + odd) * p.ldo + (row - odd);
-          if (row_warp + 32 <= p.n) {
-            if (count == 32) {
-              store_queries<OT, PAIR, 0>(v, qs, row_scale, bias[k], o, p.ldo, odd, 32);
-            } else {
-              store_queries<OT, PAIR, 1>(v, qs, row_scale, bias[k], o, p.ldo, odd, count);
-            }
-          } else {
-            // The last base rows. keep: this lane's pair exists (2), or its
-            // first row alone (1: the last of an odd count), or nothing (0).
-            const int64_t left = p.n - (row - odd);
-            store_ragged<OT, PAIR>(v, qs, row_scale, bias[k], o, p.ldo, odd, count,
-                                   left >= 2 ? 2 : left < 0 ? 0 : static_cast<int>(left));
-          }
+          ragged.store(v, qs, row_scale, bias[k], grp, count, out + qb * p.ldo + row_cta, p.ldo,
+                       p.n - row_cta < kRows ? static_cast<int>(p.n - row_cta) : kRows);
         }
       }
       if (!freed) {
@@ -557,9 +590,9 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   if (threadIdx.x == 0 && *s_abort) atomicOr(&g_int8_err, 1u);
 }
 
-template <typename OT, bool PAIR, bool TMA>
+template <typename OT, bool TMA>
 cudaError_t launch_typed(const CUtensorMap* maps, const Params& p, int clusters, size_t smem, cudaStream_t stream) {
-  auto kern = int8_scores_kernel<OT, PAIR, TMA>;
+  auto kern = int8_scores_kernel<OT, TMA>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   return launch_after(kern, 2 * clusters, kThreads, smem, stream, maps[0], maps[1], maps[2], p);
@@ -583,6 +616,9 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   // leave two tiles per cluster. Per tile of one slice and 32 queries the MMA
   // warp's waits and commits take about 1250 clocks, HBM 690.
   p.subs = p.n_cols <= 64 ? 4 : p.n_cols <= 128 ? 2 : 1;
+  const int64_t size = a.type == kElemF32 ? 4 : 2;
+  const bool tma = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo * size % 16 == 0 && a.n * size % 16 == 0 &&
+                   a.ldo * size < (int64_t(1) << 40);
   while (p.subs > 1 && (a.n + p.subs * 2 * kRows - 1) / (p.subs * 2 * kRows) * groups < 2 * clusters) p.subs /= 2;
   p.base_tiles = static_cast<int>((a.n + p.subs * 2 * kRows - 1) / (p.subs * 2 * kRows));
   p.accs = p.subs * p.n_cols <= 128 ? 4 : 2;
@@ -606,10 +642,7 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   clusters = p.teams * p.width;
   p.kc = (a.d + kSlice - 1) / kSlice;
   const int b_slice = p.n_cols / 2 * kSlice;
-  const int64_t size = a.type == kElemF32 ? 4 : 2;
-  const bool tma = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo * size % 16 == 0 && a.n * size % 16 == 0 &&
-                   a.ldo * size < (int64_t(1) << 40);
-  const size_t fixed = kFixed + (tma ? kGroups * kOutBuf : 0);
+  const size_t fixed = kFixed + kGroups * (tma ? kOutBuf : kRaggedBuf);
   // Resident queries leave 80 KB or more of ring: what HBM's latency times an
   // SM's share of the bandwidth asks for and half more.
   const int a_bytes = p.subs * kA;
@@ -627,19 +660,16 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   else
     maps[2] = maps[0];  // not used
   if (e != cudaSuccess) return e;
-  const bool pair = reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.ldo % 2 == 0;
   switch (a.type) {
     case kElemF32:
-      return tma ? launch_typed<float, false, true>(maps, p, clusters, smem, stream)
-                 : launch_typed<float, false, false>(maps, p, clusters, smem, stream);
+      return tma ? launch_typed<float, true>(maps, p, clusters, smem, stream)
+                 : launch_typed<float, false>(maps, p, clusters, smem, stream);
     case kElemF16:
-      return tma    ? launch_typed<__half, false, true>(maps, p, clusters, smem, stream)
-             : pair ? launch_typed<__half, true, false>(maps, p, clusters, smem, stream)
-                    : launch_typed<__half, false, false>(maps, p, clusters, smem, stream);
+      return tma ? launch_typed<__half, true>(maps, p, clusters, smem, stream)
+                 : launch_typed<__half, false>(maps, p, clusters, smem, stream);
     case kElemBf16:
-      return tma    ? launch_typed<__nv_bfloat16, false, true>(maps, p, clusters, smem, stream)
-             : pair ? launch_typed<__nv_bfloat16, true, false>(maps, p, clusters, smem, stream)
-                    : launch_typed<__nv_bfloat16, false, false>(maps, p, clusters, smem, stream);
+      return tma ? launch_typed<__nv_bfloat16, true>(maps, p, clusters, smem, stream)
+                 : launch_typed<__nv_bfloat16, false>(maps, p, clusters, smem, stream);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -203,6 +203,34 @@ def test_int8_scores_out_and_strides(px, dtype):
     assert torch.equal(px.int8_scores(q.t().contiguous().t(), qs, odd, xs, bias=b, dtype=dtype), want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_int8_scores_ragged_ends(px, dtype):
+    # Every place of a row's two ends within and across tiles of 128, in rows
+    # that begin anywhere; what lies around them stays.
+    m, d = 19, 40
+    q, qs, x, xs, _ = _scores_case(m, 400, d, 5, False)
+    qs, want = qs / 100, px.int8_scores(q, qs / 100, x, xs, dtype=dtype)
+    _within(want, _scores64(q, qs, x, xs, None), _scores_bound(_scores64(q, qs, x, xs, None), None, dtype))
+    for n in [*range(1, 20), *range(112, 146), *range(250, 275), 391]:
+        for lead, pitch in ((0, n + 9), (1 + n % 15, 401 + n % 3)):
+            buf = torch.full((m, 432), 7.0, dtype=dtype, device="cuda").view(-1)
+            out = buf[lead:].as_strided((m, n), (pitch, 1))
+            px.int8_scores(q, qs, x[:n], xs[:n], dtype=dtype, out=out)
+            assert torch.equal(out, want[:, :n]), (n, lead)
+            out.fill_(7.0)
+            assert (buf == 7.0).all(), (n, lead)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [1, 9, 17, 32, 41, 49, 270])
+def test_int8_scores_many_ragged_tiles(px, dtype, m):
+    n, d = 100_003, 24
+    q, qs, x, xs, b = _scores_case(m, n, d, 6, True)
+    qs, b = qs / 100, b / 100
+    want = _scores64(q, qs, x, xs, b)
+    _within(px.int8_scores(q, qs, x, xs, bias=b, dtype=dtype), want, _scores_bound(want, b, dtype), "scores")
+
+
 def test_int8_scores_offsets_beyond_32_bits(px):
     # An output of more than 2^31 values, of which the last rows are checked.
     m, n, d = 2200, 1_000_003, 32
