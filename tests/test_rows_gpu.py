@@ -96,6 +96,30 @@ def test_quantize_special_rows(px):
     assert px.dequantize_rows(codes, scales)[1].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,lead", [(1, 1, 1), (5000, 1, 3), (700, 3, 1), (3001, 33, 0), (3001, 33, 5), (1200, 130, 2), (601, 619, 7),
+                                      (40, 1537, 1), (40, 2048, 0), (9, 7999, 3), (3, 16001, 1), (2, 20001, 0)])
+def test_contiguous_rows_anywhere(px, dtype, n, d, lead):
+    # Contiguous rows from any element on, short and long, and back; what lies
+    # around them is not read.
+    buf = torch.full((n * d + 32,), math.nan, dtype=dtype, device="cuda")
+    x = buf[lead:lead + n * d].view(n, d)
+    x.copy_(_rand(n, d, seed=n + d, dtype=dtype))
+    codes, scales = px.quantize_rows(x)
+    want, want_scales = _codes64(x)
+    assert torch.equal(codes, want) and torch.equal(scales, want_scales)
+    back = px.dequantize_rows(codes, scales, dtype)
+    exact = codes.double() * scales.double()[:, None]
+    _within(back, exact, (U + HALF[dtype]) * 1.001 * exact.abs() + TINY[dtype])
+    # Into an output that begins anywhere: its surroundings stay.
+    lib, out = px._lib.load(), torch.full((n * d + 32,), 7.0, dtype=dtype, device="cuda")
+    kinds = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    px._lib.check(lib.px_dequantize_rows_device(0, codes.data_ptr(), codes.stride(0), scales.data_ptr(), n, d, kinds[dtype],
+                                                out[lead:].data_ptr(), d, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(out[lead:lead + n * d].view(n, d), back)
+    assert (out[:lead] == 7.0).all() and (out[lead + n * d:] == 7.0).all()
+
+
 def test_quantize_strided_inputs(px):
     base = _rand(50, 200, seed=9)
     want = px.quantize_rows(base[:, 3:100].contiguous())
