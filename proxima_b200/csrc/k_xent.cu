@@ -319,22 +319,40 @@ __device__ __forceinline__ void stage_line(uint32_t buf, int lane, int half, con
 // 4-byte boundaries, else a warp per row.
 __device__ __forceinline__ void store_staged(uint32_t buf, int lane, uint16_t* out, int64_t ldo, int rows, int cols) {
   const bool words = (reinterpret_cast<uintptr_t>(out) & 3) == 0 && (ldo & 1) == 0;
-  const int per = words ? 2 : 1;  // rows at a time
-  const int c = words ? (lane & 15) * 2 : lane;
-#pragma unroll 4
-  for (int r0 = 0; r0 < 32; r0 += per) {
-    const int r = words ? r0 + (lane >> 4) : r0;
-    const uint32_t at = buf + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2;
-    if (r >= rows || c >= cols) continue;
-    uint16_t* o = out + r * ldo + c;
-    if (words && c + 1 < cols) {
-      uint32_t x;
-      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(at));
-      *reinterpret_cast<uint32_t*>(o) = x;
-    } else {
-      uint16_t x;
-      asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(at));
-      *o = x;
+  constexpr int kAhead = 8;  // reads ahead of the stores
+  if (words) {
+    const int c = (lane & 15) * 2, half = lane >> 4;
+    uint16_t* to = out + half * ldo + c;
+#pragma unroll 1
+    for (int r0 = half; r0 < 32; r0 += 2 * kAhead) {
+      uint32_t x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int r = r0 + 2 * i;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x[i]) : "r"(buf + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2));
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i, to += 2 * ldo) {
+        if (r0 + 2 * i >= rows) continue;
+        if (c + 1 < cols)
+          *reinterpret_cast<uint32_t*>(to) = x[i];
+        else if (c < cols)
+          *to = static_cast<uint16_t>(x[i]);
+      }
+    }
+  } else {
+    uint16_t* to = out + lane;
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += kAhead) {
+      uint16_t x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int r = r0 + i;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x[i]) : "r"(buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2));
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i, to += ldo)
+        if (r0 + i < rows && lane < cols) *to = x[i];
     }
   }
 }
