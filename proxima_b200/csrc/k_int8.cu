@@ -64,6 +64,12 @@ constexpr int kMaxAccs = 8;
 constexpr int kBars = 2 * kMaxStages + 2 * kMaxAccs + 4;  // one spare: the scales after them stay 16-byte aligned
 constexpr size_t kFixed = 1024 + kBars * 8 + 16 + kEpiWarps * kWarpScales * 4;
 constexpr size_t kSmemLimit = 232448;  // 227 KB
+// From this size on, a matrix that TMA cannot address leaves through shared
+// memory (us, from registers and staged): fp16 2705 x 49k (267 MB) 100 and 114,
+// bf16 181 x 249k (90 MB) 48 and 53, fp32 129 x 425k (219 MB) 71 and 73; but
+// fp16 210 x 969k (407 MB) 221 and 176, bf16 952 x 855k (1.6 GB) 878 and 612,
+// fp32 1308 x 543k (2.8 GB) 1155 and 747.
+constexpr int64_t kStagedBytes = int64_t(320) << 20;
 
 struct Params {
   const float* q_scale;
@@ -84,6 +90,15 @@ struct Params {
 };
 
 template <typename T>
+__device__ __forceinline__ T narrow(float x);
+template <>
+__device__ __forceinline__ float narrow<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
@@ -99,6 +114,69 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 __device__ __forceinline__ F2 two_scores(const uint32_t (&v)[32], int j, float w0, float w1, F2 xs, F2 bias) {
   return fma2(f2(static_cast<float>(static_cast<int>(v[j])), static_cast<float>(static_cast<int>(v[j + 1]))),
               mul2(f2(w0, w1), xs), bias);
+}
+
+// A pair's word of 16-bit scores: the even lane's both rows of query j, the
+// odd lane's of query j + 1.
+template <typename OT>
+__device__ __forceinline__ uint32_t trade(float s0, float s1, int odd) {
+  const uint32_t mine = pack2<OT>(s0, s1);
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+  return __byte_perm(mine, other, odd ? 0x3276 : 0x5410);
+}
+
+// Stores a block's scores, all 32 base rows of the warp being real. SOME: only
+// the first `count` queries are. The stores evict first: the matrix is larger
+// than what L2 should keep for the base.
+template <typename OT, bool PAIR, int SOME>
+__device__ __forceinline__ void store_queries(const uint32_t (&v)[32], const float* qs, float xs, float bias, OT* o,
+                                              int64_t ldo, int odd, int count) {
+  const float4* qs4 = reinterpret_cast<const float4*>(qs);
+  const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
+#pragma unroll
+  for (int j4 = 0; j4 < 8; ++j4) {
+    if (SOME && 4 * j4 >= count) break;
+    const float4 w = qs4[j4];
+    float s[4];
+    unpack(two_scores(v, 4 * j4, w.x, w.y, xs2, bias2), s[0], s[1]);
+    unpack(two_scores(v, 4 * j4 + 2, w.z, w.w, xs2, bias2), s[2], s[3]);
+    if constexpr (PAIR) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t word = trade<OT>(s[2 * h], s[2 * h + 1], odd);
+        if (!SOME || 4 * j4 + 2 * h + odd < count) __stcs(reinterpret_cast<uint32_t*>(o), word);
+        o += 2 * ldo;
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (!SOME || 4 * j4 + h < count) __stcs(o, narrow<OT>(s[h]));
+        o += ldo;
+      }
+    }
+  }
+}
+
+// The same for the base's last rows.
+template <typename OT, bool PAIR>
+__device__ __forceinline__ void store_ragged(const uint32_t (&v)[32], const float* qs, float xs, float bias, OT* o,
+                                             int64_t ldo, int odd, int count, int keep) {
+  const F2 xs2 = f2(xs, xs), bias2 = f2(bias, bias);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    if (j >= count) break;
+    float s0, s1;
+    unpack(two_scores(v, j, qs[j], qs[j + 1], xs2, bias2), s0, s1);
+    if constexpr (PAIR) {
+      const uint32_t word = trade<OT>(s0, s1, odd);
+      if (j + odd < count && keep == 2) *reinterpret_cast<uint32_t*>(o) = word;
+      if (j + odd < count && keep == 1) *reinterpret_cast<unsigned short*>(o) = static_cast<unsigned short>(word);
+    } else {
+      if (keep > 0) *o = narrow<OT>(s0);
+      if (keep > 0 && j + 1 < count) o[ldo] = narrow<OT>(s1);
+    }
+    o += 2 * ldo;
+  }
 }
 
 // Arrive and wait of one epilogue group's four warps.
@@ -156,14 +234,13 @@ __device__ __forceinline__ void stage_queries(const uint32_t (&v)[32], const flo
   }
 }
 
-// The same for a matrix that TMA cannot address (rows that begin or end off
-// 16-byte boundaries): the warps store the rows of 128 scores themselves, in
-// aligned 16-byte pieces and single scores at either end. A row lies in the
+// The same for a large matrix that TMA cannot address (rows that begin or end
+// off 16-byte boundaries): the warps store the rows of 128 scores themselves,
+// in aligned 16-byte pieces and single scores at either end. A row lies in the
 // buffer as far from a boundary as in `out`, so pieces are read whole. Stored
 // straight from registers, 32 scores of a query per instruction, most of a
-// row's sectors are written in two parts: fp32, 1308 x 543k x 176, 1155 us
-// against 747; bf16, 6269 x 94k x 264, 583 against 444; where little is written
-// this is slower (fp16, 2705 x 49k x 80: 100 against 114). Tiles that overlap,
+// row's sectors are written in two parts, which costs little while L2 joins
+// them and much past it; kStagedBytes has the measurements. Tiles that overlap,
 // so that a CTA stores whole sectors only, gained nothing.
 // How far rows begin past a boundary repeats every kPiece queries, so that each
 // thread works out once where its scores go and which pieces it stores.
@@ -275,9 +352,15 @@ struct Ragged {
   }
 };
 
-// TMA: `out` can be stored by TMA (rows of whole 16-byte pieces, on 16-byte
-// boundaries).
-template <typename OT, bool TMA>
+// How scores leave: by TMA (rows of whole 16-byte pieces, on 16-byte
+// boundaries), staged by the warps (large matrices of other rows), or straight
+// from registers, 16-bit scores in pairs of base rows where out and its rows
+// are 4-byte aligned.
+enum Way { kTma, kStaged, kPairs, kSingle };
+// Shared memory that an epilogue group stages in.
+constexpr int staging(int way) { return way == kTma ? kOutBuf : way == kStaged ? kRaggedBuf : 0; }
+
+template <typename OT, int WAY>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_q,
                    const __grid_constant__ CUtensorMap tm_out, const Params p) {
@@ -286,7 +369,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int b_slice = p.n_cols / 2 * kSlice;  // bytes of a slice of this CTA's queries
   const int b_bytes = p.resident ? p.kc * b_slice : 0;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + b_bytes + p.stages * p.stage_bytes + kGroups * (TMA ? kOutBuf : kRaggedBuf));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + b_bytes + p.stages * p.stage_bytes + kGroups * staging(WAY));
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + kBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   float* s_scale = reinterpret_cast<float*>(s_tmem + 4);
@@ -480,7 +563,8 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     float* scale = s_scale + (warp - 2) * kWarpScales;
     const uint32_t out_buf = ring + p.stages * p.stage_bytes + grp * kOutBuf;
     const uint32_t ragged_buf = ring + p.stages * p.stage_bytes + grp * kRaggedBuf;
-    const Ragged<OT> ragged(static_cast<const OT*>(p.out), p.ldo, ragged_buf, quarter * 32 + lane);
+    const Ragged<OT> ragged(WAY == kStaged ? static_cast<const OT*>(p.out) : nullptr, p.ldo, ragged_buf,
+                            quarter * 32 + lane);
     OT* out = static_cast<OT*>(p.out);
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -541,9 +625,10 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         const int b = grp + kGroups * k;
         const int sub = sub_of[k], q_in = q_of[k];
         const int64_t row_cta = (static_cast<int64_t>(bt) * p.subs + sub) * (2 * kRows) + rank * kRows;
-        // All four warps of a group take part, base rows or not: they meet at
-        // barriers, and what lies past the matrix is left out.
-        if (sub >= p.subs || q_in >= queries || row_cta >= p.n) continue;  // uniform in the group
+        const int64_t row = row_cta + row_in_cta, row_warp = row - lane;
+        // Where scores are staged, all four warps of a group take part, base rows
+        // or not: they meet at barriers, and what lies past the matrix is left out.
+        if (sub >= p.subs || q_in >= queries || (WAY <= kStaged ? row_cta >= p.n : row_warp >= p.n)) continue;  // warp-uniform
         __syncwarp();
         uint32_t v[32];
         tc::tmem_ld_32x32b_x32(lane_addr + static_cast<uint32_t>(acc * acc_cols + b * 32), v);
@@ -559,12 +644,31 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         const int64_t qb = q0 + q_in;
         const float* qs = scale + k * 32;
         const int count = queries - q_in < 32 ? queries - q_in : 32;
-        if constexpr (TMA) {
+        if constexpr (WAY == kTma) {
           stage_queries<OT>(v, qs, row_scale, bias[k], out_buf, row_in_cta, grp, count, &tm_out,
                             static_cast<int>(row_cta), static_cast<int>(qb));
-        } else {
+        } else if constexpr (WAY == kStaged) {
           ragged.store(v, qs, row_scale, bias[k], grp, count, out + qb * p.ldo + row_cta, p.ldo,
                        p.n - row_cta < kRows ? static_cast<int>(p.n - row_cta) : kRows);
+        } else {
+          constexpr bool PAIR = WAY == kPairs;
+          // Lanes 2i and 2i + 1 trade 16-bit scores when these leave in pairs:
+          // the even one stores both rows' of query j, the odd one of j + 1.
+          const int odd = PAIR ? lane & 1 : 0;
+          OT* o = out + (qb + odd) * p.ldo + (row - odd);
+          if (row_warp + 32 <= p.n) {
+            if (count == 32) {
+              store_queries<OT, PAIR, 0>(v, qs, row_scale, bias[k], o, p.ldo, odd, 32);
+            } else {
+              store_queries<OT, PAIR, 1>(v, qs, row_scale, bias[k], o, p.ldo, odd, count);
+            }
+          } else {
+            // The last base rows. keep: this lane's pair exists (2), or its
+            // first row alone (1: the last of an odd count), or nothing (0).
+            const int64_t left = p.n - (row - odd);
+            store_ragged<OT, PAIR>(v, qs, row_scale, bias[k], o, p.ldo, odd, count,
+                                   left >= 2 ? 2 : left < 0 ? 0 : static_cast<int>(left));
+          }
         }
       }
       if (!freed) {
@@ -578,7 +682,7 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
       }
       fresh = advance(qg, bt);
     }
-    if (TMA && quarter == 0 && lane == 0) store_wait();
+    if (WAY == kTma && quarter == 0 && lane == 0) store_wait();
   }
 
   if (warp == 1 && lane == 0) quiet_wait(done_bar, 0);
@@ -590,12 +694,22 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
   if (threadIdx.x == 0 && *s_abort) atomicOr(&g_int8_err, 1u);
 }
 
-template <typename OT, bool TMA>
+template <typename OT, int WAY>
 cudaError_t launch_typed(const CUtensorMap* maps, const Params& p, int clusters, size_t smem, cudaStream_t stream) {
-  auto kern = int8_scores_kernel<OT, TMA>;
+  auto kern = int8_scores_kernel<OT, WAY>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   return launch_after(kern, 2 * clusters, kThreads, smem, stream, maps[0], maps[1], maps[2], p);
+}
+
+template <typename OT>
+cudaError_t launch_16(Way way, const CUtensorMap* maps, const Params& p, int clusters, size_t smem, cudaStream_t stream) {
+  switch (way) {
+    case kTma: return launch_typed<OT, kTma>(maps, p, clusters, smem, stream);
+    case kStaged: return launch_typed<OT, kStaged>(maps, p, clusters, smem, stream);
+    case kPairs: return launch_typed<OT, kPairs>(maps, p, clusters, smem, stream);
+    default: return launch_typed<OT, kSingle>(maps, p, clusters, smem, stream);
+  }
 }
 
 }  // namespace
@@ -617,8 +731,14 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   // warp's waits and commits take about 1250 clocks, HBM 690.
   p.subs = p.n_cols <= 64 ? 4 : p.n_cols <= 128 ? 2 : 1;
   const int64_t size = a.type == kElemF32 ? 4 : 2;
-  const bool tma = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo * size % 16 == 0 && a.n * size % 16 == 0 &&
-                   a.ldo * size < (int64_t(1) << 40);
+  Way way = kSingle;
+  if (reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo * size % 16 == 0 && a.n * size % 16 == 0 &&
+      a.ldo * size < (int64_t(1) << 40))
+    way = kTma;
+  else if (a.m * a.n * size >= kStagedBytes)
+    way = kStaged;
+  else if (size == 2 && reinterpret_cast<uintptr_t>(a.out) % 4 == 0 && a.ldo % 2 == 0)
+    way = kPairs;
   while (p.subs > 1 && (a.n + p.subs * 2 * kRows - 1) / (p.subs * 2 * kRows) * groups < 2 * clusters) p.subs /= 2;
   p.base_tiles = static_cast<int>((a.n + p.subs * 2 * kRows - 1) / (p.subs * 2 * kRows));
   p.accs = p.subs * p.n_cols <= 128 ? 4 : 2;
@@ -642,7 +762,7 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   clusters = p.teams * p.width;
   p.kc = (a.d + kSlice - 1) / kSlice;
   const int b_slice = p.n_cols / 2 * kSlice;
-  const size_t fixed = kFixed + kGroups * (tma ? kOutBuf : kRaggedBuf);
+  const size_t fixed = kFixed + kGroups * staging(way);
   // Resident queries leave 80 KB or more of ring: what HBM's latency times an
   // SM's share of the bandwidth asks for and half more.
   const int a_bytes = p.subs * kA;
@@ -655,21 +775,18 @@ cudaError_t launch_int8_scores(const Int8ScoresArgs& a, int clusters, cudaStream
   CUtensorMap maps[3];
   cudaError_t e = encode_rows_map(&maps[0], kElemS8, a.x, a.d, a.n, a.ldx, kSlice, kRows, 128);
   if (e == cudaSuccess) e = encode_rows_map(&maps[1], kElemS8, a.q, a.d, a.m, a.ldq, kSlice, p.n_cols / 2, 128);
-  if (e == cudaSuccess && tma)
+  if (e == cudaSuccess && way == kTma)
     e = encode_rows_map(&maps[2], a.type, a.out, a.n, a.m, a.ldo * size, kRows, size == 4 ? 16 : 32, 0);
   else
     maps[2] = maps[0];  // not used
   if (e != cudaSuccess) return e;
   switch (a.type) {
     case kElemF32:
-      return tma ? launch_typed<float, true>(maps, p, clusters, smem, stream)
-                 : launch_typed<float, false>(maps, p, clusters, smem, stream);
-    case kElemF16:
-      return tma ? launch_typed<__half, true>(maps, p, clusters, smem, stream)
-                 : launch_typed<__half, false>(maps, p, clusters, smem, stream);
-    case kElemBf16:
-      return tma ? launch_typed<__nv_bfloat16, true>(maps, p, clusters, smem, stream)
-                 : launch_typed<__nv_bfloat16, false>(maps, p, clusters, smem, stream);
+      return way == kTma      ? launch_typed<float, kTma>(maps, p, clusters, smem, stream)
+             : way == kStaged ? launch_typed<float, kStaged>(maps, p, clusters, smem, stream)
+                              : launch_typed<float, kSingle>(maps, p, clusters, smem, stream);
+    case kElemF16: return launch_16<__half>(way, maps, p, clusters, smem, stream);
+    case kElemBf16: return launch_16<__nv_bfloat16>(way, maps, p, clusters, smem, stream);
     default: return cudaErrorInvalidValue;
   }
 }

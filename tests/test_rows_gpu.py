@@ -255,6 +255,27 @@ def test_int8_scores_many_ragged_tiles(px, dtype, m):
     _within(px.int8_scores(q, qs, x, xs, bias=b, dtype=dtype), want, _scores_bound(want, b, dtype), "scores")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [73, 81])
+def test_int8_scores_large_ragged_matrices(px, dtype, m):
+    # Matrices past 320 MB off 16-byte boundaries, which leave another way.
+    most, d = 2_400_130, 16
+    q, qs, x, xs, b = _scores_case(m, most, d, 7, True)
+    qs, b = qs / 100, b / 100
+    full = px.int8_scores(q, qs, x, xs, bias=b, dtype=dtype)
+    for i in range(0, m, 16):
+        want = _scores64(q[i:i + 16], qs[i:i + 16], x, xs, b)
+        _within(full[i:i + 16], want, _scores_bound(want, b, dtype), "scores")
+    buf = torch.full((m * (most + 16),), 7.0, dtype=dtype, device="cuda")
+    for n in [*range(2_400_000, 2_400_129, 16), 2_400_127, 2_400_129]:
+        for lead, pitch in ((0, n + 9), (1 + n % 15, n)):
+            out = buf[lead:].as_strided((m, n), (pitch, 1))
+            px.int8_scores(q, qs, x[:n], xs[:n], bias=b[:n], dtype=dtype, out=out)
+            assert torch.equal(out, full[:, :n]), (n, lead)
+            out.fill_(7.0)
+            assert (buf == 7.0).all(), (n, lead)
+
+
 def test_int8_scores_offsets_beyond_32_bits(px):
     # An output of more than 2^31 values, of which the last rows are checked.
     m, n, d = 2200, 1_000_003, 32
