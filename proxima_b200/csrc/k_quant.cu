@@ -355,8 +355,9 @@ __global__ void __launch_bounds__(kThreads) dequantize_span_kernel(const int8_t*
   }
 }
 
-// VE codes at a time; a group of lanes takes a row, as above.
-template <typename T, int VE>
+// VE codes at a time, AHEAD loads before their stores; a group of lanes takes a
+// row, as above.
+template <typename T, int VE, int AHEAD>
 __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const int8_t* codes, int64_t ldc, const float* scales,
                                                                    int64_t n, int d, T* out, int64_t ldo, int group) {
   using C = typename Word<VE>::type;
@@ -370,13 +371,13 @@ __global__ void __launch_bounds__(kThreads) dequantize_rows_kernel(const int8_t*
   const int8_t* c = codes + row * ldc;
   T* o = out + row * ldo;
   const int step = group * VE;
-  for (int at0 = lane * VE; at0 < d; at0 += kAhead * step) {
-    C w[kAhead];
+  for (int at0 = lane * VE; at0 < d; at0 += AHEAD * step) {
+    C w[AHEAD];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
+    for (int i = 0; i < AHEAD; ++i)
       if (at0 + i * step + VE <= d) w[i] = *reinterpret_cast<const C*>(c + at0 + i * step);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < AHEAD; ++i) {
       const int at = at0 + i * step;
       if (at + VE <= d) {
         const int8_t* e = reinterpret_cast<const int8_t*>(&w[i]);
@@ -441,7 +442,10 @@ cudaError_t quantize_typed(const T* x, int64_t n, int d, int64_t ldx, int8_t* co
   const int64_t pitch = ldx * static_cast<int64_t>(sizeof(T));
   const int group = group_for(d, 16);
   const int rows = span_rows(n, d * static_cast<int64_t>(sizeof(T)), kThreads / group);
-  if ((ldx == d || n == 1) && rows > 0 && (!aligned(x, pitch, 16) || d > 1024)) {
+  // As spans: long rows, and those of which no load takes four values (us, in
+  // vectors and as spans: fp32 1M x 33 141 and 102, 100k x 998 227 and 146, 3M x
+  // 7 91 and 132; bf16 700k x 100, four values a load, 100 and 140).
+  if ((ldx == d || n == 1) && rows > 0 && (d > 1024 || (d >= 16 && !aligned(x, pitch, 4 * sizeof(T))))) {
     const size_t smem = (static_cast<size_t>(rows) * d * sizeof(T) + 31) / 16 * 16 + static_cast<size_t>(rows) * ((d + 3) & ~3);
     const int64_t blocks = (n + rows - 1) / rows;
     if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
@@ -460,8 +464,8 @@ cudaError_t dequantize_vec(const int8_t* codes, int64_t ldc, const float* scales
   const int group = group_for((d + VE - 1) / VE, 4);
   const int64_t blocks = (n * group + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
-  return launch_after(dequantize_rows_kernel<T, VE>, blocks, kThreads, 0, stream, codes, ldc, scales, n, d, out, ldo,
-                      group);
+  auto kern = group * VE >= d ? dequantize_rows_kernel<T, VE, 1> : dequantize_rows_kernel<T, VE, kAhead>;
+  return launch_after(kern, blocks, kThreads, 0, stream, codes, ldc, scales, n, d, out, ldo, group);
 }
 
 template <typename T>
@@ -471,6 +475,9 @@ cudaError_t dequantize_typed(const int8_t* codes, int64_t ldc, const float* scal
   const int64_t pitch = ldo * static_cast<int64_t>(sizeof(T));
   if (aligned(codes, ldc, VE) && aligned(out, pitch, 16))
     return dequantize_vec<T, VE>(codes, ldc, scales, n, d, out, ldo, stream);
+  if (aligned(codes, ldc, 2) && aligned(out, pitch, 2 * static_cast<int>(sizeof(T))))
+    return dequantize_vec<T, 2>(codes, ldc, scales, n, d, out, ldo, stream);
+  // 1M x 33: 72 us, value by value 99.
   const int rows = span_rows(n, d * static_cast<int64_t>(sizeof(T)), 1);
   if ((ldo == d || n == 1) && rows > 0) {
     const int64_t blocks = (n + rows - 1) / rows;
@@ -478,8 +485,6 @@ cudaError_t dequantize_typed(const int8_t* codes, int64_t ldc, const float* scal
     return launch_after(dequantize_span_kernel<T>, blocks, kThreads, 0, stream, codes, ldc, scales, n, d, out, rows,
                         aligned(codes, ldc, 4));
   }
-  if (aligned(codes, ldc, 2) && aligned(out, pitch, 2 * static_cast<int>(sizeof(T))))
-    return dequantize_vec<T, 2>(codes, ldc, scales, n, d, out, ldo, stream);
   return dequantize_vec<T, 1>(codes, ldc, scales, n, d, out, ldo, stream);
 }
 
