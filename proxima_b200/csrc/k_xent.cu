@@ -264,13 +264,16 @@ __device__ __forceinline__ float bias2(float b) { return b * (kLog2e * 0x1p24f) 
 __device__ __forceinline__ void add_bias(uint32_t (&v)[32], const float* bias, int left, float c) {
   if (left >= 32) {
     const float4* b4 = reinterpret_cast<const float4*>(bias);
+    const F2 up = f2(kLog2e * 0x1p24f, kLog2e * 0x1p24f), down = f2(0x1p-24f, 0x1p-24f), c2 = f2(c, c);
 #pragma unroll
-    for (int j4 = 0; j4 < 8; ++j4) {
-      const float4 b = b4[j4];
-      v[4 * j4] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4]), c, bias2(b.x)));
-      v[4 * j4 + 1] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 1]), c, bias2(b.y)));
-      v[4 * j4 + 2] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 2]), c, bias2(b.z)));
-      v[4 * j4 + 3] = __float_as_uint(fmaf(__uint_as_float(v[4 * j4 + 3]), c, bias2(b.w)));
+    for (int j = 0; j < 32; j += 4) {
+      const float4 b = b4[j / 4];
+      float x[4];
+      // bias2, two at a time.
+      unpack(fma2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), c2, mul2(mul2(f2(b.x, b.y), up), down)), x[0], x[1]);
+      unpack(fma2(f2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), c2, mul2(mul2(f2(b.z, b.w), up), down)), x[2], x[3]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[j + k] = __float_as_uint(x[k]);
     }
   } else {
 #pragma unroll
