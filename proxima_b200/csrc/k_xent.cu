@@ -800,6 +800,12 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         }
         n_hits = 1;
       }
+      if (S::LOGITS && BIAS) {
+        // This warp's 64 biases come near while the tile is awaited (loss of 1000
+        // x 500k x 128: 247 -> 227 us).
+        const int64_t b = static_cast<int64_t>(p.v0) + n * kTile + group * 64 + lane * 32;
+        if (lane < 2 && b < p.v) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.bias + b));
+      }
       if (!lost && !__all_sync(0xffffffffu, tc::mbar_wait(tfull_bar(acc), acc_phase, s_abort))) lost = true;
       tc::tc_fence_after();
       if (ROLE == kStats) {
