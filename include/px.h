@@ -340,8 +340,12 @@ PX_API px_status px_softmax_xent_device(int32_t device, const void* queries, int
  * its one gradient with stride 0 and the forward's divisor. loss and lse are the
  * forward's. Queries that are ignored, or whose target is no row, add nothing
  * (but queries and rows are multiplied with a weight of zero, so they must be
- * finite). G takes the operands' 16 bits, in pieces of the base of at most
- * 256 MB or 1024 columns. Results do not change from run to run. */
+ * finite). G takes the operands' 16 bits; an entry above 2^-9 of |g_i| is the
+ * sum of two such numbers, within 2^-16 (bf16) or 2^-22 (fp16) of itself. With
+ * fp16, entries are also held to no less than 2^-39 of the largest |g_i|, so
+ * gradients of one call should lie within a few orders of magnitude. G is kept
+ * in pieces of the base of at most 256 MB or 512 columns. Results do not change
+ * from run to run. */
 PX_API px_status px_softmax_xent_backward_device(int32_t device, const void* queries, int64_t ldq, int64_t t,
                                                  const void* rows, int64_t ldr, int64_t v, int32_t dim, int32_t type,
                                                  const int64_t* targets, int64_t ignore_index, float scale,

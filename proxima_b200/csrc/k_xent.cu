@@ -14,24 +14,32 @@
 // one sign that a loss near zero would show.
 //
 // Backward: the base is taken in pieces of columns. For each piece the
-// products are computed again, their epilogue writes the piece of G in the
-// operands' 16-bit type, and two more products read it: dq accumulates over
-// the pieces in fp32 slabs (one per split of the piece, added to in the same
-// order every time, so results do not change from run to run), dr is complete
-// per piece.
+// products are computed again, their epilogue writes the piece of G, and two
+// more products read it: dq accumulates over the pieces in fp32 slabs (one per
+// split of the piece, added to in the same order every time, so results do not
+// change from run to run), dr is complete per piece.
+// G is kept as the sum of two numbers of the operands' 16-bit type, an entry
+// rounded and what the rounding took, and each gradient is the sum of both
+// parts' products. One part alone is off by up to 2^-8 of an entry (bf16). The
+// entries of a query add up to zero, so where rows with large entries lie near
+// one another (a target and its hard negatives), the products cancel and the
+// rounding's errors do not: a negative that holds most of the rest, 0.03 of the
+// rows' length away from the target, left dq off by 3%. Both parts together are
+// within 2^-16 (bf16) or 2^-22 (fp16) of an entry.
+// The second part counts where entries are large, and a query has few of those:
+// it is kept for blocks of 32 queries x 64 rows with an entry above kLarge of
+// its query's gradient, and the products take it for slices with such a block.
+// Elsewhere an entry's error is at most 2^-17 of its query's gradient (bf16),
+// and the errors of many such entries average out (those of rows that are
+// alike to the last bit do not, and come to 2^-8 of what such rows hold).
+// Entries are relative to the largest |g_i|, times 2^14 for fp16, whose smallest
+// normal would otherwise lie above the probabilities of a large base; an fp16
+// entry is held to 2^-39 of the largest |g_i| at best.
 // G lies in blocks of 64 columns, each block's rows of 128 bytes behind one
-// another: what a tile writes, and what a load of it reads, is then a run of
-// 16 to 32 KB instead of lines a row of G apart (each of the three kernels 2-4%
-// faster; 200 MB of G through HBM and L2 cost 45 of 1000 x 100k x 384's 326 us).
-// Its rows are padded with zeros to whole K slices of dr, its last block's
-// columns likewise.
-// G's rounding to 16 bits is relative 2^-9 (bf16) or 2^-12 (fp16) of each
-// entry, as the outputs' own. Of thousands of probabilities it averages out;
-// the target's entry, which alone makes up most of a gradient, would carry it
-// into the result whole, so its rounding error is added back in fp32 (in dq
-// always, in dr where at most kHits queries share a target). Entries are
-// relative to the largest |g_i|, times 2^14 for fp16, whose smallest normal
-// would otherwise lie above the probabilities of a large base.
+// another, those of the second part after those of the first: what a tile
+// writes, and what a load of it reads, is then a run of 16 to 32 KB instead of
+// lines a row of G apart. Its rows are padded with zeros to whole K slices of
+// dr, its last block's columns likewise.
 //
 // All three products are one kernel, instantiated per role: CTA pairs
 // (tcgen05.mma cta_group::2, kind::f16), 256 M rows per pair, K slices of 64.
@@ -63,8 +71,9 @@
 // Measured, bf16: forward 1000 x 1M x 128 327 us (2900 clocks per tile), 4096 x
 // 100k x 384 1.53 PFLOP/s and, with the epilogue left out, 1.60; past the kept
 // slices the operands' way from L2 counts (d = 768: 1.25, 1.30). A training
-// step of 1000 x 100k x 384: 326 us, of it 55 forward, 70 G, 60 dq, 68 dr;
-// 8192 x 8192 x 768 (fp16): 400 us, 1.03 PFLOP/s over its four products.
+// step of 1000 x 100k x 384: 380 us in two pieces; 8192 x 8192 x 768 (fp16): 495
+// us with targets at random, so that four slices of G in five have a second
+// part. One part throughout: 343 and 418; two throughout: 499 and 551.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -91,7 +100,8 @@ constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr int kOutBuf = 2048;  // staging of an epilogue warp's stores: 32 rows of 64 bytes
 constexpr int kBars = 2 * kStatsSlots + 2 + 2 + 2 + 1;
 constexpr size_t kSmem = 1024 + kSlots * kSlot + kEpiWarps * kOutBuf + kBars * 8 + 16;
-constexpr int kHits = 4;     // most queries that share a target for its correction in dr
+// An entry of G above this share of its query's gradient is kept in two parts.
+constexpr float kLarge = 0x1p-9f;
 // A running sum is kept relative to 2^base, base the largest logit of the
 // first block; a block whose sum passes kRaise (or is NaN) raises it. Between,
 // no maximum is needed: fp32 holds sums of 2^60 as exactly as sums of 1.
@@ -125,7 +135,8 @@ static_assert(kStatsSlots * kSlot == kSlots * kSlot + kEpiWarps * kOutBuf, "one 
 struct Args {
   int64_t t, v;
   int d;
-  int g_rows;            // rows per block of G
+  int g_rows;            // rows of a part of a block of G
+  int g_all;             // rows of the whole array: a load from there on reads zeros
   int m_tiles, n_tiles;
   int tiles;             // logits: m_tiles * n_tiles; gradients: items
   int per_split;         // kGradQ: K slices per split
@@ -145,13 +156,10 @@ struct Args {
   int64_t ignore_index;
   float2* part;          // kStats: [t][lists] (base, sum): sum * 2^base
   unsigned* counter;     // kStats: cleared for the joining kernel
-  RowGrad row;           // kWeights, kGradRows
-  float* rest;           // kWeights writes, kGradRows reads: [t] what rounding took from the target's entry
-  int* hits;             // [piece] how many queries have the base row as target (or null)
-  int4* hit_list;        // [piece] the first kHits of them
-  int* next_hits;        // kGradRows: cleared for the next piece
-  const uint16_t* other; // the gradients' other operand: the rows corrections are taken from
-  int64_t ldother;
+  RowGrad row;           // kWeights, kGradRows, kGradQ where it is direct
+  // Which blocks of G have a second part, a byte each, in eights as the products
+  // take them: for dq of [row block][query tile], for dr of [row tile][64 queries].
+  uint8_t *parts_q, *parts_r;
   int accumulate;        // kGradQ: to what its slabs hold
   int direct;            // kGradQ: one piece in one split, so the product is the gradient
   uint16_t* out;         // the gradient, where TMA cannot store it
@@ -360,53 +368,6 @@ __device__ __forceinline__ void store_staged(uint32_t buf, int lane, uint16_t* o
   }
 }
 
-// The first n of four query numbers in ascending order, the others -1: fp32
-// additions in an order of their own, whatever order the queries came in.
-__device__ __forceinline__ int4 in_order(int4 a, int n) {
-  constexpr int kNone = 0x7fffffff;
-  if (n < 4) a.w = kNone;
-  if (n < 3) a.z = kNone;
-  if (n < 2) a.y = kNone;
-  auto order = [](int& x, int& y) {
-    const int lo = min(x, y), hi = max(x, y);
-    x = lo;
-    y = hi;
-  };
-  order(a.x, a.y);
-  order(a.z, a.w);
-  order(a.x, a.z);
-  order(a.y, a.w);
-  order(a.y, a.z);
-  if (a.y == kNone) a.y = -1;
-  if (a.z == kNone) a.z = -1;
-  if (a.w == kNone) a.w = -1;
-  return a;
-}
-
-// Adds f times a row of 16-bit values (32 of them, or the `left` there are) to
-// a block.
-template <bool BF>
-__device__ __forceinline__ void add_row(uint32_t (&v)[32], float f, const uint16_t* x, int left) {
-  if (left >= 32) {
-    const uint4* x4 = reinterpret_cast<const uint4*>(x);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint4 a = x4[k];
-      const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 p = widen2<BF>(u[j]);
-        v[8 * k + 2 * j] = __float_as_uint(fmaf(f, p.x, __uint_as_float(v[8 * k + 2 * j])));
-        v[8 * k + 2 * j + 1] = __float_as_uint(fmaf(f, p.y, __uint_as_float(v[8 * k + 2 * j + 1])));
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < left) v[j] = __float_as_uint(fmaf(f, widen2<BF>(x[j]).x, __uint_as_float(v[j])));
-  }
-}
-
 // Where a tile lies. Tiles are numbered along the base, then along the queries
 // (logits), or along M, then N, then the splits (gradients). A pair divides its
 // first tile's number once and counts on from there; dividing per tile, in the
@@ -466,6 +427,14 @@ __device__ __forceinline__ int last_slice(const Args& p, const Place& at) {
   return ROLE == kGradQ ? min(p.k_slices, (at.split + 1) * p.per_split) : p.k_slices;
 }
 
+// Which blocks of the pair's slice of G have a second part: its eight bytes.
+template <int ROLE>
+__device__ __forceinline__ uint64_t parts_of(const Args& p, const Place& at, int k) {
+  const uint8_t* bytes = ROLE == kGradQ ? p.parts_q + 8 * (static_cast<int64_t>(k) * p.m_tiles + at.m)
+                                        : p.parts_r + 8 * (static_cast<int64_t>(at.m) * p.k_slices + k);
+  return *reinterpret_cast<const uint64_t*>(bytes);
+}
+
 // Logits tiles [first, last) of pair `i` of `n`, and the pair that has tile x.
 __host__ __device__ __forceinline__ int run_begin(int64_t tiles, int i, int n) {
   return static_cast<int>(tiles * i / n);
@@ -477,7 +446,7 @@ __host__ __device__ __forceinline__ int run_of(int64_t tiles, int64_t x, int n) 
 template <int ROLE, bool BF, bool BIAS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                 const __grid_constant__ CUtensorMap tm_out, const Args p) {
+                 const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ CUtensorMap tm_part, const Args p) {
   using S = Shape<ROLE>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
@@ -518,6 +487,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     tc::prefetch_tmap(&tm_a);
     tc::prefetch_tmap(&tm_b);
     if (ROLE != kStats) tc::prefetch_tmap(&tm_out);
+    if (S::B_MN) tc::prefetch_tmap(&tm_part);
   }
   if (warp == 1) {
     tc::tmem_alloc_pair(tc::smem_addr(s_tmem), 512);
@@ -601,15 +571,28 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           const int m0 = m * kTile + rank * kHalf;
           const int n0 = n * p.n_cols;
           const int k0 = first_slice<ROLE>(p, at), k1 = last_slice<ROLE>(p, at);
+          uint64_t next_parts = parts_of<ROLE>(p, at, k0);
           const int boxes1 = (n_first / 2 + 63) / 64, boxes2 = (n_second / 2 + 63) / 64;
           for (int k = k0; k < k1; ++k) {
+            const uint64_t parts = next_parts;
+            if (k + 1 < k1) next_parts = parts_of<ROLE>(p, at, k + 1);
             if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
+            const int block = S::A_MN ? m0 / kSlice : k;
             if (S::A_MN) {
-              const int block = m0 / kSlice;
-              tc::tma_load_2d_pair(dst, &tm_a, fb, 0, block * p.g_rows + k * kSlice);
-              tc::tma_load_2d_pair(dst + 8192, &tm_a, fb, 0, (block + 1) * p.g_rows + k * kSlice);
+              tc::tma_load_2d_pair(dst, &tm_a, fb, 0, 2 * block * p.g_rows + k * kSlice);
+              tc::tma_load_2d_pair(dst + 8192, &tm_a, fb, 0, 2 * (block + 1) * p.g_rows + k * kSlice);
             } else {
-              tc::tma_load_2d_pair(dst, &tm_a, fb, 0, k * p.g_rows + m0);
+              tc::tma_load_2d_pair(dst, &tm_a, fb, 0, 2 * block * p.g_rows + m0);
+            }
+            if (parts != 0) {
+              // The second part, 32 rows of G at a time; zeros where there is none.
+              if ((dst = next_slot(kSlot, fb)) == 0) { ok = false; break; }
+              for (int i2 = 0; i2 < 4; ++i2) {
+                const bool some = (parts >> (32 * rank + 8 * i2) & 0xff) != 0;
+                const int row = S::A_MN ? (2 * (block + i2 / 2) + 1) * p.g_rows + k * kSlice + 32 * (i2 & 1)
+                                        : (2 * block + 1) * p.g_rows + m0 + 32 * i2;
+                tc::tma_load_2d_pair(dst + i2 * 4096, &tm_part, fb, 0, some ? row : p.g_all);
+              }
             }
             const int k_row = k * kSlice + (ROLE == kGradQ ? p.v0 : 0);
             if ((dst = next_slot(boxes1 * 8192, fb)) == 0) { ok = false; break; }
@@ -663,28 +646,35 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       Place at = place_of<ROLE>(p, first);
       bool fresh = true;  // the queries changed
       for (int i = first; ok && i < last; i += step) {
-        if (!wait(tempty_bar(acc), acc_phase ^ 1)) break;
         int k0 = 0, k1 = p.k_slices;
+        uint64_t next_parts = 0;
+        if (!S::LOGITS) {
+          k0 = first_slice<ROLE>(p, at);
+          k1 = last_slice<ROLE>(p, at);
+          next_parts = parts_of<ROLE>(p, at, k0);
+        }
+        if (!wait(tempty_bar(acc), acc_phase ^ 1)) break;
         if (S::LOGITS) {
           if (fresh) {
             if (!wait(kfull_bar, keeps & 1)) break;
             ++keeps;
             fresh = false;
           }
-        } else {
-          k0 = first_slice<ROLE>(p, at);
-          k1 = last_slice<ROLE>(p, at);
         }
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kTile);
         for (int k = k0; k < k1; k += per) {
-          int slot_a = -1, slot_b = -1, slot_c = -1;
+          int slot_a = -1, slot_l = -1, slot_b = -1, slot_c = -1;
           const bool streamed = !S::LOGITS || k >= keep;
           if (streamed && !next_slot(slot_a)) { ok = false; break; }
+          const bool two = S::B_MN && next_parts != 0;  // G's second part
+          if (S::B_MN && k + 1 < k1) next_parts = parts_of<ROLE>(p, at, k + 1);
+          if (two && !next_slot(slot_l)) { ok = false; break; }
           if (!next_slot(slot_b)) { ok = false; break; }
           if (n_second > 0 && !next_slot(slot_c)) { ok = false; break; }
           tc::tc_fence_after();
           const uint32_t a_at = (streamed ? ring_base + slot_a * slot_bytes : smem_base + k * kSlot) >> 4;
           const uint64_t a_desc = a_kind + a_at;
+          const uint64_t l_desc = a_kind + ((ring_base + slot_l * slot_bytes) >> 4);
           const uint64_t b_desc = b_kind + ((ring_base + slot_b * slot_bytes) >> 4);
           const uint64_t c_desc = b_kind + ((ring_base + slot_c * slot_bytes) >> 4);
           const uint32_t more = k > k0 ? 1u : 0u;
@@ -698,13 +688,24 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                 tc::mma_bf16_pair(d_tmem, a_desc + (kSlot >> 4) + kk * kAStep, b_desc + (kSlot >> 4) + kk * kBStep,
                                   p.idesc, 1u);
             }
+            if (two) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                tc::mma_bf16_pair(d_tmem, l_desc + kk * kAStep, b_desc + kk * kBStep, p.idesc, 1u);
+            }
             if (S::B_MN && n_second > 0) {
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
                 tc::mma_bf16_pair(d_tmem + kTile, a_desc + kk * kAStep, c_desc + kk * kBStep, p.idesc2,
                                   kk > 0 ? 1u : more);
+              if (two) {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                  tc::mma_bf16_pair(d_tmem + kTile, l_desc + kk * kAStep, c_desc + kk * kBStep, p.idesc2, 1u);
+              }
             }
             if (streamed) tc::mma_commit_pair_both(empty_bar(slot_a));
+            if (two) tc::mma_commit_pair_both(empty_bar(slot_l));
             tc::mma_commit_pair_both(empty_bar(slot_b));
             if (S::B_MN && n_second > 0) tc::mma_commit_pair_both(empty_bar(slot_c));
           }
@@ -779,26 +780,6 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             at_target = target_entry(p.row, row, factor);
           }
         }
-      }
-      int4 hits = make_int4(-1, -1, -1, -1);  // kGradRows: the queries whose target this base row is
-      int n_hits = 0;
-      if (ROLE == kGradRows) {
-        if (row < p.piece) {
-          n_hits = p.hits[row];
-          // A row with more is left as it is: their errors average out, and
-          // which of them came first is chance.
-          if (n_hits > kHits) n_hits = 0;
-          if (n_hits > 0) hits = in_order(p.hit_list[row], n_hits);
-          p.next_hits[row] = 0;
-        }
-        n_hits = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(n_hits));
-      }
-      if (ROLE == kGradQ && p.direct) {
-        if (row < p.t) {
-          const int64_t y = p.targets[row];
-          if (counts(y, p.ignore_index, p.v)) hits.x = static_cast<int>(y);
-        }
-        n_hits = 1;
       }
       if (S::LOGITS && BIAS) {
         // This warp's 64 biases come near while the tile is awaited (loss of 1000
@@ -882,16 +863,13 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           __syncwarp();
           if (lane == 0) tc::mbar_arrive_cluster(tc::mapa_shared(tempty_bar(acc), 0));
         };
+        bool two = false;  // the block has a second part
         if (some) {
-          uint32_t w[32];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32];
+          // |G| of half `h` of the columns; past the base and left out: 0.
+          auto entries = [&](uint32_t (&v)[32], int h) {
             __syncwarp();
             tc::tmem_ld_32x32b_x32(at_tmem + 32 * h, v);
             tc::tmem_ld_wait();
-            // The last columns are in registers: the accumulator is free.
-            if (h == 1) release();
             if (lost) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = 0x7fc00000u;
@@ -904,40 +882,73 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             }
             const float c = BIAS ? 1.0f : p.c;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              w[16 * h + j] = pack2<BF>(ex2(fmaf(__uint_as_float(v[2 * j]), c, shift)),
-                                        ex2(fmaf(__uint_as_float(v[2 * j + 1]), c, shift)));
-          }
-          if (factor < 0.0f) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) w[j] ^= 0x80008000u;
-          }
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(ex2(fmaf(__uint_as_float(v[j]), c, shift)));
+          };
+          const uint32_t sign = factor < 0.0f ? 0x80008000u : 0;
           const int at = target - col;  // the target's place among the columns
-          if (at >= 0 && at < 64) {
-            p.rest[row] = at_target - rounded<BF>(at_target);
-            if (p.hits != nullptr) {
-              const int slot = atomicAdd(p.hits + target, 1);
-              if (slot < kHits) reinterpret_cast<int*>(p.hit_list + target)[slot] = static_cast<int>(row);
-            }
-            const uint32_t e = pack2<BF>(at_target, at_target);
+          const bool mine = at >= 0 && at < 64;
+          auto put = [&](uint32_t (&w)[32], float x) {  // x as the target's entry
+            const uint32_t e = pack2<BF>(x, x);
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               if (2 * j == at) w[j] = (w[j] & 0xffff0000u) | (e & 0xffffu);
               if (2 * j + 1 == at) w[j] = (w[j] & 0xffffu) | (e & 0xffff0000u);
             }
-          }
-          // Sixteen rows at a time, so that a buffer half as large as the block takes
-          // rows of whole 128-byte lines (1-2% of a training step against 64-byte ones).
+          };
+          // A part leaves sixteen rows at a time, so that a buffer half as large as the
+          // block takes rows of whole 128-byte lines (1-2% of a training step against
+          // 64-byte ones).
+          auto leave = [&](const uint32_t (&w)[32], int part) {
+            const int g_row = (2 * (col / kSlice) + part) * p.g_rows + static_cast<int>(row_warp);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              stage_line(out_buf, lane, h, w);
+              if (lane == 0) {
+                tma_store(&tm_out, out_buf, 0, g_row + 16 * h);
+                store_commit();
+              }
+            }
+          };
+          uint32_t w[32];
+          float top = 0.0f;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            stage_line(out_buf, lane, h, w);
-            if (lane == 0) {
-              tma_store(&tm_out, out_buf, 0, col / kSlice * p.g_rows + static_cast<int>(row_warp) + 16 * h);
-              store_commit();
+            uint32_t v[32];
+            entries(v, h);
+            top = max2(top, largest(v));
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[16 * h + j] = pack2<BF>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])) ^ sign;
+          }
+          two = __any_sync(0xffffffffu, !(top <= kLarge * fabsf(factor)));
+          // The columns are in registers: the accumulator is free.
+          if (!two) release();
+          if (mine) put(w, at_target);
+          leave(w, 0);
+          if (two) {
+            // The products once more, for what the rounding took.
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t v[32];
+              entries(v, h);
+              if (h == 1) release();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float2 r = widen2<BF>(w[16 * h + j] ^ sign);
+                w[16 * h + j] = pack2<BF>(__uint_as_float(v[2 * j]) - r.x, __uint_as_float(v[2 * j + 1]) - r.y) ^ sign;
+              }
             }
+            if (mine) put(w, at_target - rounded<BF>(at_target));
+            leave(w, 1);
           }
         } else {
           release();
+        }
+        if (lane == 0) {
+          const int block = n * kGroups + group, rows32 = static_cast<int>(row_warp) / 32;
+          p.parts_q[8 * (static_cast<int64_t>(block) * p.m_tiles + m) + rank * 4 + quarter] = two;
+          if (row_warp < p.g_rows)
+            p.parts_r[8 * (static_cast<int64_t>(n) * (p.g_rows / kSlice) + rows32 / 2) + group * 2 + (rows32 & 1)] = two;
         }
         if (++acc == accs) {
           acc = 0;
@@ -986,13 +997,6 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             }
           }
           if (ROLE == kGradRows || (ROLE == kGradQ && p.direct)) {
-            for (int h = 0; h < n_hits; ++h) {
-              const int t = h == 0 ? hits.x : h == 1 ? hits.y : h == 2 ? hits.z : hits.w;
-              if (t >= 0) {
-                const float rest = p.rest[ROLE == kGradQ ? row : t];
-                add_row<BF>(v, rest, p.other + t * p.ldother + col, p.d - col);
-              }
-            }
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -1195,23 +1199,17 @@ __device__ __forceinline__ float4 load_once(const float4* p) {
 struct GradQArgs {
   const float* slab;
   int splits;
-  int64_t slab_rows, ld_slab, t, v;
+  int64_t slab_rows, ld_slab, t;
   int d;
   RowGrad row;
-  const float* rest;
-  const int64_t* targets;
-  int64_t ignore_index;
-  const uint16_t* rows;
-  int64_t ldr;
   float scale;
   uint16_t* out;
   int64_t ldo;
   int rows_per_block;
 };
 
-// The sum of dq's slabs plus what the target's entry lost when it was rounded,
-// scaled and rounded to the queries' type. A block takes rows_per_block rows,
-// four columns per thread.
+// The sum of dq's slabs, scaled and rounded to the queries' type. A block takes
+// rows_per_block rows, four columns per thread.
 template <bool BF>
 __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
   wait_for_previous();
@@ -1227,7 +1225,6 @@ __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
     if (row >= p.t) break;
     const int col = (i - r_in * quads) * 4;
     const float4* s = reinterpret_cast<const float4*>(p.slab + row * p.ld_slab + col);
-    const int64_t y = p.targets[row];
     float4 sum = load_once(s);
 #pragma unroll 6
     for (int k = 1; k < p.splits; ++k) {
@@ -1237,24 +1234,7 @@ __global__ void __launch_bounds__(256) xent_grad_q_kernel(const GradQArgs p) {
       sum.z += w.z;
       sum.w += w.w;
     }
-    float r[4] = {sum.x, sum.y, sum.z, sum.w};
-    if (counts(y, p.ignore_index, p.v)) {
-      const float rest = p.rest[row];
-      const uint16_t* x = p.rows + y * p.ldr + col;
-      if (col + 4 <= p.d) {  // rows start on 16-byte boundaries
-        const uint2 u = *reinterpret_cast<const uint2*>(x);
-        const float2 a = widen2<BF>(u.x), b = widen2<BF>(u.y);
-        r[0] = fmaf(rest, a.x, r[0]);
-        r[1] = fmaf(rest, a.y, r[1]);
-        r[2] = fmaf(rest, b.x, r[2]);
-        r[3] = fmaf(rest, b.y, r[3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < p.d) r[j] = fmaf(rest, widen2<BF>(x[j]).x, r[j]);
-      }
-    }
-    const uint32_t lo = pack2<BF>(r[0] * f, r[1] * f), hi = pack2<BF>(r[2] * f, r[3] * f);
+    const uint32_t lo = pack2<BF>(sum.x * f, sum.y * f), hi = pack2<BF>(sum.z * f, sum.w * f);
     uint16_t* o = p.out + row * p.ldo + col;
     if (col + 4 <= p.d && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
       *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
@@ -1278,7 +1258,7 @@ cudaError_t launch_role(const CUtensorMap* maps, Args p, bool bf, int clusters, 
                  : (bias ? xent_gemm_kernel<ROLE, false, kB> : xent_gemm_kernel<ROLE, false, false>);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
   if (e != cudaSuccess) return e;
-  return launch_after(kern, 2 * clusters, kThreads, kSmem, stream, maps[0], maps[1], maps[2], p);
+  return launch_after(kern, 2 * clusters, kThreads, kSmem, stream, maps[0], maps[1], maps[2], maps[3], p);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1318,18 +1298,18 @@ struct GradTiles {
 };
 
 // Base tiles (of 256 columns) per piece of the backward. A piece's G is at
-// most kPieceBytes (larger than L2: at d >= 256 the products take longer than G's
-// way through HBM, and fewer pieces save more); among the sizes that fit, the
-// one whose waves of logits and dr tiles take least, with a price per piece for
-// its three launches and the adds into dq's slabs (about 16 us).
+// most kPieceBytes, or two tiles (larger than L2: at d >= 256 the products take
+// longer than G's way through HBM, and fewer pieces save more); among the sizes
+// that fit, the one whose waves of logits and dr tiles take least, with a price
+// per piece for its three launches and the adds into dq's slabs (about 16 us).
 constexpr int64_t kPieceBytes = int64_t(256) << 20;
 int64_t piece_tiles(int64_t t, int64_t v, int d, int clusters) {
   const GradTiles gt(d);
   const int64_t all = ceil_div(v, kTile), m_tiles = ceil_div(t, kTile);
-  const int64_t per_tile = t * kTile * 2;  // bytes of G
-  const int64_t fit = least(all, kPieceBytes / per_tile > 4 ? kPieceBytes / per_tile : int64_t(4));
+  const int64_t per_tile = align_up(t, kSlice) * kTile * 4;  // bytes of G, both parts
+  const int64_t fit = least(all, kPieceBytes / per_tile > 2 ? kPieceBytes / per_tile : int64_t(2));
   // Clocks of a tile of each product; its bytes of G cross HBM meanwhile.
-  const double logits = ceil_div(d, kSlice) * 512.0, dr = ceil_div(t, kSlice) * 2.0 * gt.n_cols;
+  const double logits = ceil_div(d, kSlice) * 512.0, dr = ceil_div(t, kSlice) * 4.0 * gt.n_cols;
   auto cost = [&](int64_t tiles) {
     return 30000.0 + logits * ceil_div(tiles * m_tiles, clusters) + dr * ceil_div(tiles * gt.n_tiles, clusters);
   };
@@ -1389,10 +1369,9 @@ struct BackwardPlan {
   GradTiles gt;
   int m_tiles, q_splits, g_rows;
   int64_t piece, slab_rows, ld_slab;  // columns of a piece
-  float *top, *rest, *slab;
-  int* hits;  // two of `piece`: this piece's, and the next one's being cleared
-  int4* hit_list;
+  float *top, *slab;
   uint16_t* g;
+  uint8_t *parts_q, *parts_r;  // a byte per block of 32 rows x 64 columns of G
   int64_t bytes;
   BackwardPlan(void* ws, int64_t t, int64_t v, int d, int clusters) : gt(d) {
     m_tiles = static_cast<int>(ceil_div(t, kTile));
@@ -1402,12 +1381,11 @@ struct BackwardPlan {
     ld_slab = static_cast<int64_t>(gt.n_tiles) * gt.n_cols;
     Carve c{static_cast<char*>(ws)};
     top = c.take<float>(1);
-    rest = c.take<float>(t);
-    hits = c.take<int>(2 * piece);
-    hit_list = c.take<int4>(piece);
     slab = c.take<float>(q_splits * slab_rows * ld_slab);
     g_rows = static_cast<int>(align_up(t, kSlice));
-    g = c.take<uint16_t>(g_rows * piece);
+    g = c.take<uint16_t>(2 * piece * g_rows);
+    parts_q = c.take<uint8_t>(piece / kSlice * m_tiles * 8);
+    parts_r = c.take<uint8_t>(piece / kTile * (g_rows / kSlice) * 8);
     bytes = c.used;
   }
 };
@@ -1469,10 +1447,10 @@ cudaError_t launch_xent_forward(const XentProblem& x, float* loss, float* lse, i
   p.part = plan.part;
   p.lists = plan.lists;
   p.counter = plan.counter;
-  CUtensorMap maps[3];
+  CUtensorMap maps[4];
   cudaError_t e = encode_rows_map(&maps[0], x.type, x.q, x.d, x.t, x.ldq * 2, kSlice, kHalf, 128);
   if (e == cudaSuccess) e = encode_rows_map(&maps[1], x.type, x.rows, x.d, x.v, x.ldr * 2, kSlice, kHalf, 128);
-  maps[2] = maps[0];  // not used
+  maps[2] = maps[3] = maps[0];  // not used
   if (e == cudaSuccess) e = launch_role<kStats>(maps, p, bf, plan.pairs, stream);
   if (e != cudaSuccess) return e;
   JoinArgs j = {};
@@ -1539,34 +1517,28 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
   if (e == cudaSuccess && dr_tma) e = encode_rows_map(&dr, x.type, drows, x.d, x.v, lddr * 2, 32, 32, 64);
   if (e == cudaSuccess && dq_tma) e = encode_rows_map(&dq_map, x.type, dq, x.d, x.t, lddq * 2, 32, 32, 64);
   if (e != cudaSuccess) return e;
-  base.rest = plan.rest;
   base.g_rows = plan.g_rows;
-  base.hit_list = plan.hit_list;
-  if (drows != nullptr) {
-    e = cudaMemsetAsync(plan.hits, 0, sizeof(int) * static_cast<size_t>(plan.piece), stream);
-    if (e != cudaSuccess) return e;
-  }
+  base.parts_q = plan.parts_q;
+  base.parts_r = plan.parts_r;
   int splits_used = 0;
   bool direct = false;
-  int turn = 0;
   for (int64_t v0 = 0; v0 < x.v; v0 += plan.piece) {
     const int64_t piece = least(plan.piece, x.v - v0);
     const int piece_n = static_cast<int>(ceil_div(piece, kTile));
     base.v0 = static_cast<int>(v0);
     base.piece = static_cast<int>(piece);
-    base.hits = drows != nullptr ? plan.hits + turn * plan.piece : nullptr;
-    base.next_hits = plan.hits + (turn ^ 1) * plan.piece;
-    turn ^= 1;
-    CUtensorMap g_k, g_mn, g_out;
-    const int64_t g_all = ceil_div(piece, kSlice) * plan.g_rows;
+    CUtensorMap g_k, g_mn, g_out, g_part;
+    const int64_t g_all = 2 * ceil_div(piece, kSlice) * plan.g_rows;
     if (g_all > 0x7fffff00) return cudaErrorInvalidValue;  // TMA coordinates are 32-bit (a G of 275 GB)
     e = encode_rows_map(&g_k, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, kHalf, 128);
     if (e == cudaSuccess) e = encode_rows_map(&g_mn, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, kSlice, 128);
     if (e == cudaSuccess) e = encode_rows_map(&g_out, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, 16, 128);
+    if (e == cudaSuccess) e = encode_rows_map(&g_part, x.type, plan.g, kSlice, g_all, kSlice * 2, kSlice, 32, 128);
     if (e != cudaSuccess) return e;
+    base.g_all = static_cast<int>(g_all);
     Args p = base;
     logits_args(p, bf, plan.m_tiles, piece_n);
-    CUtensorMap maps[3] = {q_k, rows_k, g_out};
+    CUtensorMap maps[4] = {q_k, rows_k, g_out, g_out};
     if ((e = launch_role<kWeights>(maps, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
     ++*launches;
     if (dq != nullptr) {
@@ -1575,27 +1547,23 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
       grad_args(p, plan.gt, bf, false, plan.m_tiles, piece, splits_used > 0 ? splits_used : plan.q_splits);
       if (splits_used == 0) splits_used = p.tiles / (p.m_tiles * p.n_tiles);
       p.accumulate = v0 > 0;
-      p.other = static_cast<const uint16_t*>(x.rows);
-      p.ldother = x.ldr;
       p.direct = splits_used == 1 && piece == x.v;
       p.out = static_cast<uint16_t*>(dq);
       p.ldo = lddq;
       p.tma_out = dq_tma;
       direct = p.direct != 0;
-      CUtensorMap maps_q[3] = {g_k, rows_mn, direct ? dq_map : slab};
+      CUtensorMap maps_q[4] = {g_k, rows_mn, direct ? dq_map : slab, g_part};
       if ((e = launch_role<kGradQ>(maps_q, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
       ++*launches;
     }
     if (drows != nullptr) {
       p = base;
       grad_args(p, plan.gt, bf, true, piece_n, x.t, 1);
-      p.other = static_cast<const uint16_t*>(x.q);
-      p.ldother = x.ldq;
       p.out = static_cast<uint16_t*>(drows);
       p.ldo = lddr;
       p.out_row0 = static_cast<int>(v0);
       p.tma_out = dr_tma;
-      CUtensorMap maps_r[3] = {g_mn, q_mn, dr};
+      CUtensorMap maps_r[4] = {g_mn, q_mn, dr, g_part};
       if ((e = launch_role<kGradRows>(maps_r, p, bf, least(clusters, p.tiles), stream)) != cudaSuccess) return e;
       ++*launches;
     }
@@ -1603,9 +1571,8 @@ cudaError_t launch_xent_backward(const XentProblem& x, const float* loss, const 
   if (dq != nullptr && !direct) {
     const int quads = static_cast<int>(ceil_div(x.d, 4));
     const int rows_per_block = quads >= 256 ? 1 : 256 / quads;
-    GradQArgs a = {plan.slab, splits_used, plan.slab_rows, plan.ld_slab, x.t, x.v, x.d, row, plan.rest, x.targets,
-                   x.ignore_index, static_cast<const uint16_t*>(x.rows), x.ldr, x.scale, static_cast<uint16_t*>(dq),
-                   lddq, rows_per_block};
+    GradQArgs a = {plan.slab, splits_used, plan.slab_rows, plan.ld_slab, x.t, x.d, row, x.scale,
+                   static_cast<uint16_t*>(dq), lddq, rows_per_block};
     e = launch_after(bf ? xent_grad_q_kernel<true> : xent_grad_q_kernel<false>, ceil_div(x.t, rows_per_block), 256, 0,
                      stream, a);
     ++*launches;

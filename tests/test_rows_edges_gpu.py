@@ -1,0 +1,116 @@
+"""The operators on embedding rows where they can go wrong: gradients that
+cancel, gradients and batches that are not ordinary, calls from several
+threads. Bounds as in test_rows_gpu.py, evaluated per output.
+"""
+
+import math
+
+import pytest
+import torch
+
+from test_rows_gpu import ACC, HALF, TINY, U, _check_xent, _rand, _within, _xent_case
+
+pytestmark = pytest.mark.gpu
+
+HALVES = [torch.float16, torch.bfloat16]
+
+
+# ---------------------------------------------------------------- gradients that cancel
+
+def _gradients_of_exact_logits(q, r, y, b, scale):
+    """Gradients of the summed loss in 64 bits and bounds on the kernels'
+    errors, for operands whose dot products are exact in fp32 in any order, so
+    that what is left is the rounding of G (and of the outputs)."""
+    dtype = q.dtype
+    q, r = q.detach().double(), r.detach().double()
+    (t, _), v = q.shape, r.shape[0]
+    s = scale * (q @ r.T)
+    z = s if b is None else s + b.double()
+    lse = torch.logsumexp(z, 1)
+    p = torch.exp(z - lse[:, None])
+    pick = torch.arange(t, device=q.device)
+    G = p.clone()
+    G[pick, y] = -torch.where(torch.arange(v, device=q.device) == y[:, None], 0.0, p).sum(1)
+    # A logit in log2 units is a fused multiply and add: two roundings in its
+    # factor, three in the bias, one of the result; the shift by lse and by the
+    # gradient's factor (2^14 at most) has four, the lse itself six of its size:
+    # together below 16u of the magnitudes' sum. Then the sum over the rows (a
+    # chain of at most v / 64 + 200 additions) and two exponentials of 2^-22.
+    size = s.abs().amax() + lse.abs().amax() + 16
+    if b is not None:
+        size = size + torch.where(b.isinf(), 0.0, b.double()).abs().amax()
+    dp = 1.01 * (16 * U * size + 2 * 2.0 ** -22 + (v / 64 + 200) * U)
+    # G: an entry above 2^-9 as the sum of two numbers of its type, of which the
+    # second rounds what the first left, half a step of at most half a step of the
+    # entry; others as one number. fp16 entries have steps of 2^-24 at a lift of
+    # 2^14 above the largest gradient, here 1.
+    held = torch.where(G.abs() > 1.001 * 2.0 ** -9, HALF[dtype] ** 2, HALF[dtype])
+    dG = G.abs() * (1.01 * held + dp + 4 * U) + (2.0 ** -39 if dtype == torch.float16 else 0.0)
+    terms = 2 * int((G != 0).sum(1).max()), 2 * int((G != 0).sum(0).max())
+    dq, dr = scale * G @ r, scale * G.T @ q
+    half = 1.01 * HALF[dtype] + 4 * U
+    bq = scale * (dG + ACC * (terms[0] + 2) * G.abs()) @ r.abs() + half * dq.abs() + TINY[dtype]
+    br = scale * (dG + ACC * (terms[1] + 2) * G.abs()).T @ q.abs() + half * dr.abs() + TINY[dtype]
+    return (dq, bq), (dr, br)
+
+
+def _check_gradients(px, q, r, y, b, scale):
+    q, r = q.detach().requires_grad_(), r.detach().requires_grad_()
+    got = torch.autograd.grad(px.softmax_cross_entropy(q, r, y, scale=scale, bias=b, reduction="sum"), (q, r))
+    for x, (want, bound), name in zip(got, _gradients_of_exact_logits(q, r, y, b, scale), ("queries", "rows")):
+        _within(x, want, bound, "grad of " + name)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,v,d", [(1, 2, 64), (40, 300, 64), (200, 5000, 200), (33, 66, 520), (70, 1000, 19), (300, 260_009, 64)])
+def test_softmax_hard_negatives(px, dtype, t, v, d):
+    # Each query is its own row, and one other row differs from that in one
+    # place by a little: both hold about half of the softmax, and in all other
+    # places their parts of dq cancel. The values are whole sixteenths.
+    g = torch.Generator(device="cuda").manual_seed(t + v + d)
+    r = torch.randint(-16, 17, (v, d), device="cuda", generator=g).double() / 16
+    order = torch.randperm(v, device="cuda", generator=g)
+    y, near = order[:t], order[t:2 * t]
+    r[near] = r[y]
+    place = torch.randint(0, d, (t,), device="cuda", generator=g)
+    r[near, place] += torch.where(r[y, place] > 0, -1, 1) * torch.randint(1, 5, (t,), device="cuda", generator=g) / 16
+    q = r[y]
+    scale = 2.0 ** round(math.log2(24 / float(q.square().sum(1).mean())))
+    b = torch.full((v,), -24.0, device="cuda")
+    b[order[:2 * t]] = 0.0
+    unit = 8 * ((d + 7) // 8)
+    qx, rx = (torch.zeros(n, unit, dtype=dtype, device="cuda")[:, :d] for n in (t, v))
+    _check_gradients(px, qx.copy_(q), rx.copy_(r), y, b, scale)
+
+
+@pytest.mark.parametrize("dtype,mine,others", [(torch.bfloat16, 25, 9), (torch.bfloat16, 9, 25), (torch.float16, 32, 6), (torch.float16, 6, 32)])
+@pytest.mark.parametrize("v", [2, 700])
+def test_softmax_rows_with_many_queries(px, dtype, mine, others, v):
+    # All queries alike, of two rows that hold the softmax between them: `mine`
+    # queries have the first as their target and `others` the second, in the
+    # first's share of the softmax, so both rows' gradients are nearly zero. An
+    # entry's rounding is the same for all queries of a kind.
+    t, d = mine + others, 40
+    q = _rand(1, d, seed=3).mul(4).round().div(4).expand(t, d).to(dtype)
+    r = _rand(v, d, seed=4).mul(4).round().div(4).to(dtype)
+    r[1] = r[0]
+    b = torch.full((v,), -math.inf, device="cuda")
+    b[0], b[1] = math.log(mine / others), 0.0
+    y = (torch.arange(t, device="cuda") >= mine).long()
+    _check_gradients(px, q, r, y, b, 0.5)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,v,d", [(33, 64, 24), (40, 300, 64), (257, 700, 200), (520, 900, 390), (1000, 300, 32), (300, 230_009, 16)])
+def test_softmax_large_entries_anywhere(px, dtype, t, v, d):
+    # Queries from certain of their target to far from it, in no order, so that
+    # entries of all sizes, and blocks with and without large ones, meet in all
+    # slices of the products.
+    q, r, y, _ = _xent_case(t, v, d, dtype, t + v)
+    g = torch.Generator(device="cuda").manual_seed(t)
+    sharp = torch.rand(t, device="cuda", generator=g) < 0.3
+    with torch.no_grad():
+        q[sharp] = (0.5 * q + 3.0 / d * r[y])[sharp]
+    b = torch.where(torch.rand(v, device="cuda", generator=g) < 0.01, 6.0, 0.0)
+    _check_xent(px, q, r, y, None, scale=2.0)
+    _check_xent(px, q, r, y, b, scale=0.5, weights=torch.linspace(-1, 1, t, device="cuda"))
