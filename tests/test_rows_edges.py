@@ -1,0 +1,18 @@
+"""What of the operators on embedding rows can be checked without a GPU
+beyond their argument checks."""
+
+import pytest
+
+
+@pytest.mark.parametrize("t,v,d", [(1, 10_000_000, 64), (1, 100_000_000, 8), (65, 2_000_000, 64), (1000, 100_000, 384), (5000, 60_000, 128)])
+def test_gradient_pieces_keep_their_bound(px, t, v, d):
+    # A piece of the gradient's matrix is at most 256 MB or 512 columns, with the
+    # queries padded to 64 and both 16-bit parts counted; beside it lie the fp32
+    # sums of the queries' gradients (148 tiles of 256 x 256 at most here), a byte
+    # per 32 queries and 64 columns, twice, and little else.
+    need = px._lib.load().px_softmax_xent_workspace_bytes(0, t, v, d, 1)
+    padded = (t + 63) // 64 * 64
+    piece = max(256 << 20, 512 * 4 * padded)
+    columns = piece // (4 * padded)
+    parts = 2 * (columns // 64 + 4) * ((t + 255) // 256 * 8)
+    assert 0 < need <= piece + 148 * 256 * 256 * 4 + parts + 4096
