@@ -222,7 +222,10 @@ __device__ __forceinline__ float row_factor(const RowGrad& r, bool used, int64_t
 // What the products of G are multiplied by at the end.
 __device__ __forceinline__ float out_scale(const RowGrad& r, float scale) {
   const float top = fabsf(*r.top);
-  return top * scale / r.lift / (r.divisor != nullptr ? *r.divisor : 1.0f);
+  const float divisor = r.divisor != nullptr ? *r.divisor : 1.0f;
+  // A mean over no query: nothing has a part in it, and G is zero.
+  if (divisor == 0.0f) return 0.0f;
+  return top * scale / r.lift / divisor;
 }
 
 // The target's entry: exp(-loss) - 1 is its share minus one, without

@@ -114,3 +114,19 @@ def test_softmax_large_entries_anywhere(px, dtype, t, v, d):
     b = torch.where(torch.rand(v, device="cuda", generator=g) < 0.01, 6.0, 0.0)
     _check_xent(px, q, r, y, None, scale=2.0)
     _check_xent(px, q, r, y, b, scale=0.5, weights=torch.linspace(-1, 1, t, device="cuda"))
+
+
+# ---------------------------------------------------------------- batches and gradients out of the ordinary
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,v,d", [(4, 40, 32), (300, 2000, 100), (70, 90, 600), (300, 520_009, 16)])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_softmax_all_queries_ignored(px, dtype, t, v, d, reduction):
+    # A batch of padding: the mean over nothing is NaN, and nobody's gradient.
+    q, r, y, b = _xent_case(t, v, d, dtype, 5, bias=True)
+    y.fill_(-100)
+    q, r = q.requires_grad_(), r.requires_grad_()
+    loss = px.softmax_cross_entropy(q, r, y, bias=b, reduction=reduction)
+    assert loss.isnan() if reduction == "mean" else not loss.any()
+    for x in torch.autograd.grad(loss.sum(), (q, r)):
+        assert torch.equal(x, torch.zeros_like(x))
