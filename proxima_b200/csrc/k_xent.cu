@@ -124,7 +124,7 @@ struct RowGrad {
   const float* loss;
   const float* lse;
   const float* grad;
-  const float* top;      // the largest |grad| (grad itself when grad_stride is 0)
+  const float* top;      // the largest finite |grad| (grad itself when grad_stride is 0)
   const float* divisor;  // or null
   int grad_stride;
   float lift;
@@ -211,21 +211,25 @@ __device__ __forceinline__ bool counts(int64_t y, int64_t ignore_index, int64_t 
   return y != ignore_index && y >= 0 && y < v;
 }
 
-// A query's factor: its gradient relative to the largest, lifted; 0 for one
-// that adds nothing.
-__device__ __forceinline__ float row_factor(const RowGrad& r, bool used, int64_t t) {
+// What gradients are taken relative to. Where all are zero, infinite or NaN,
+// they are taken as they are.
+__device__ __forceinline__ float top_of(const RowGrad& r) {
   const float top = fabsf(*r.top);
-  if (!used || top == 0.0f) return 0.0f;
-  return r.grad[t * r.grad_stride] / top * r.lift;
+  return top > 0.0f && top < kInf ? top : 1.0f;
+}
+
+// A query's factor: its gradient relative to the largest, lifted; 0 for one
+// that adds nothing. An infinity or a NaN stays the query's own.
+__device__ __forceinline__ float row_factor(const RowGrad& r, bool used, int64_t t) {
+  return used ? r.grad[t * r.grad_stride] / top_of(r) * r.lift : 0.0f;
 }
 
 // What the products of G are multiplied by at the end.
 __device__ __forceinline__ float out_scale(const RowGrad& r, float scale) {
-  const float top = fabsf(*r.top);
   const float divisor = r.divisor != nullptr ? *r.divisor : 1.0f;
   // A mean over no query: nothing has a part in it, and G is zero.
   if (divisor == 0.0f) return 0.0f;
-  return top * scale / r.lift / divisor;
+  return top_of(r) * scale / r.lift / divisor;
 }
 
 // The target's entry: exp(-loss) - 1 is its share minus one, without
@@ -1170,15 +1174,17 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const JoinArgs p) {
   }
 }
 
-// One block: the largest |grad| of the queries that count.
+// One block: the largest finite |grad| of the queries that count.
 __global__ void __launch_bounds__(1024) xent_top_kernel(const float* grad, const int64_t* targets,
                                                         int64_t ignore_index, int64_t t, int64_t v, float* out) {
   __shared__ float s_top[32];
   float top = 0.0f;
   wait_for_previous();
   let_next_start();
-  for (int64_t i = threadIdx.x; i < t; i += 1024)
-    if (counts(targets[i], ignore_index, v)) top = fmaxf(top, fabsf(grad[i]));
+  for (int64_t i = threadIdx.x; i < t; i += 1024) {
+    const float g = fabsf(grad[i]);
+    if (g < kInf && counts(targets[i], ignore_index, v)) top = fmaxf(top, g);
+  }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
   if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;

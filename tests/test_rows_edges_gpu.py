@@ -130,3 +130,38 @@ def test_softmax_all_queries_ignored(px, dtype, t, v, d, reduction):
     assert loss.isnan() if reduction == "mean" else not loss.any()
     for x in torch.autograd.grad(loss.sum(), (q, r)):
         assert torch.equal(x, torch.zeros_like(x))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("t,v,d", [(1, 40, 32), (70, 300, 64), (300, 5000, 100)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_softmax_gradients_that_are_not_finite(px, dtype, t, v, d, bad):
+    # One query's gradient is no number: its row of dq, and all of dr, which it
+    # has a part in; the other queries' rows are as without it.
+    q, r, y, _ = _xent_case(t, v, d, dtype, 6)
+    q, r = q.requires_grad_(), r.requires_grad_()
+
+    def gradients(w, targets=y):
+        loss = px.softmax_cross_entropy(q, r, targets, reduction="none")
+        return torch.autograd.grad(loss, (q, r), grad_outputs=w)
+
+    w = torch.linspace(0.5, 2, t, device="cuda")
+    w[t // 2] = 0.0
+    want = gradients(w)
+    w[t // 2] = bad
+    dq, dr = gradients(w)
+    others = torch.arange(t, device="cuda") != t // 2
+    assert torch.equal(dq[others], want[0][others])
+    assert not dq[t // 2].isfinite().any() and not dr.isfinite().any()
+    # An ignored query's counts for nothing, whatever it is.
+    targets = y.clone()
+    targets[t // 2] = -100
+    dq, dr = gradients(w, targets)
+    assert torch.equal(dq, want[0]) and torch.equal(dr, want[1])
+    # The gradient of a sum, and a batch with no query to count.
+    loss = px.softmax_cross_entropy(q, r, y, reduction="sum")
+    for x in torch.autograd.grad(loss * bad, (q, r)):
+        assert not x.isfinite().any()
+    loss = px.softmax_cross_entropy(q, r, torch.full_like(y, -100), reduction="sum")
+    for x in torch.autograd.grad(loss, (q, r), grad_outputs=torch.tensor(bad, device="cuda")):
+        assert torch.equal(x, torch.zeros_like(x))
