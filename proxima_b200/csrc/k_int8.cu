@@ -697,7 +697,9 @@ int8_scores_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
 template <typename OT, int WAY>
 cudaError_t launch_typed(const CUtensorMap* maps, const Params& p, int clusters, size_t smem, cudaStream_t stream) {
   auto kern = int8_scores_kernel<OT, WAY>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // The limit belongs to the kernel, not to the launch: always the most, so that
+  // a call on another thread with less shared memory leaves this one its own.
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
   if (e != cudaSuccess) return e;
   return launch_after(kern, 2 * clusters, kThreads, smem, stream, maps[0], maps[1], maps[2], p);
 }

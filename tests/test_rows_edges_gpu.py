@@ -165,3 +165,90 @@ def test_softmax_gradients_that_are_not_finite(px, dtype, t, v, d, bad):
     loss = px.softmax_cross_entropy(q, r, torch.full_like(y, -100), reduction="sum")
     for x in torch.autograd.grad(loss, (q, r), grad_outputs=torch.tensor(bad, device="cuda")):
         assert torch.equal(x, torch.zeros_like(x))
+
+
+# ---------------------------------------------------------------- several threads
+
+def _in_threads(work, count, rounds):
+    """work(k) on `count` threads with a stream each, `rounds` times; an
+    exception in any of them is raised here."""
+    import threading
+
+    done, failed, start = [0] * count, [], threading.Barrier(count)
+
+    def run(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait(60)
+                for _ in range(rounds):
+                    work(k)
+                    done[k] += 1
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,), daemon=True) for k in range(count)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(100)
+    if failed:
+        raise failed[0]
+    assert done == [rounds] * count
+
+
+def test_threads_with_scores_of_different_shapes(px):
+    # Launches of one kernel that ask for different amounts of shared memory,
+    # close behind one another: the C ABI's calls alone, their arguments made
+    # before.
+    import sys
+
+    lib, n = px._lib.load(), 64
+    shapes = [(1, 128), (256, 768), (1, 128), (256, 768), (64, 1024), (1, 128)]
+    one, calls, outs = torch.ones(256, device="cuda"), [], []
+    for m, d in shapes:
+        q, x = (torch.full((rows, d), 1, dtype=torch.int8, device="cuda") for rows in (m, n))
+        out, stream = torch.zeros(m, n, device="cuda"), torch.cuda.Stream()
+        outs.append((out, q, x, stream))
+        calls.append((0, q.data_ptr(), d, one.data_ptr(), m, x.data_ptr(), d, one.data_ptr(), n, d, None, 0, out.data_ptr(), n,
+                      stream.cuda_stream))
+    torch.cuda.synchronize()
+
+    def work(k):
+        f, args = lib.px_int8_scores_device, calls[k]
+        for _ in range(15_000):
+            status = f(*args)
+            if status:
+                px._lib.check(status)
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-5)
+    try:
+        _in_threads(work, len(shapes), 1)
+    finally:
+        sys.setswitchinterval(interval)
+        torch.cuda.synchronize()
+    for (m, d), (out, *_) in zip(shapes, outs):
+        assert (out == d).all()
+
+
+def test_threads_with_steps_of_different_shapes(px):
+    # Each thread its own operands, types and pieces; all results as alone.
+    shapes = [(100, 5000, 48, torch.float16), (300, 900, 200, torch.bfloat16), (7, 20_000, 16, torch.bfloat16)]
+    cases = [_xent_case(t, v, d, dtype, 700 + k) for k, (t, v, d, dtype) in enumerate(shapes)]
+
+    def step(k):
+        q, r, y, _ = cases[k]
+        q, r = q.detach().requires_grad_(), r.detach().requires_grad_()
+        loss = px.softmax_cross_entropy(q, r, y, reduction="sum")
+        return [loss.detach(), *torch.autograd.grad(loss, (q, r)), *px.quantize_rows(r.detach())]
+
+    want = [step(k) for k in range(len(shapes))]
+    torch.cuda.synchronize()
+
+    def work(k):
+        got = step(k)
+        torch.cuda.current_stream().synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
+
+    _in_threads(work, len(shapes), 30)
