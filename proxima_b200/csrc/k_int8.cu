@@ -110,10 +110,12 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// The scores of queries j and j + 1 and this lane's base row.
+// The scores of queries j and j + 1 and this lane's base row. The sum is taken
+// times the query's scale first: the scales' own product may leave the range of
+// fp32 where the score does not.
 __device__ __forceinline__ F2 two_scores(const uint32_t (&v)[32], int j, float w0, float w1, F2 xs, F2 bias) {
-  return fma2(f2(static_cast<float>(static_cast<int>(v[j])), static_cast<float>(static_cast<int>(v[j + 1]))),
-              mul2(f2(w0, w1), xs), bias);
+  return fma2(mul2(f2(static_cast<float>(static_cast<int>(v[j])), static_cast<float>(static_cast<int>(v[j + 1]))), f2(w0, w1)),
+              xs, bias);
 }
 
 // A pair's word of 16-bit scores: the even lane's both rows of query j, the

@@ -8,7 +8,8 @@ import math
 import pytest
 import torch
 
-from test_rows_gpu import ACC, HALF, TINY, U, _check_xent, _rand, _within, _xent_case
+from test_rows_gpu import (ACC, HALF, TINY, TYPES, U, _check_xent, _rand, _scores64, _scores_bound, _scores_case, _within,
+                           _xent_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -252,3 +253,32 @@ def test_threads_with_steps_of_different_shapes(px):
         assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
 
     _in_threads(work, len(shapes), 30)
+
+
+# ---------------------------------------------------------------- scores
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [256, 301])
+@pytest.mark.parametrize("small,large", [(2.0 ** -70, 2.0 ** -65), (2.0 ** -100, 2.0 ** -40), (2.0 ** 80, 2.0 ** -120)])
+def test_int8_scores_of_scales_far_from_one(px, dtype, n, small, large):
+    # Scores within fp32's range whose two scales' product is below its normal
+    # numbers, or whose scales lie far apart.
+    q, qs, x, xs, _ = _scores_case(40, n, 500, 3, False)
+    for a, b in ((small, large), (large, small)):
+        if a * 2 ** 23 > 2.0 ** 127:
+            continue
+        want = _scores64(q, qs * a, x, xs * b, None)
+        _within(px.int8_scores(q, qs * a, x, xs * b, dtype=dtype), want, _scores_bound(want, None, dtype) + TINY[torch.float32])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [256, 301])
+def test_int8_scores_of_zero_sums(px, dtype, n):
+    # Rows at right angles, and rows of zeros, score 0 whatever their lengths.
+    q = torch.zeros(33, 64, dtype=torch.int8, device="cuda")
+    x = torch.zeros(n, 64, dtype=torch.int8, device="cuda")
+    q[:, 0], x[1:, 1] = 127, 127
+    qs, xs = torch.full((33,), 1e25, device="cuda"), torch.full((n,), 1e25, device="cuda")
+    b = torch.arange(n, device="cuda") % 100 + 0.5
+    assert not px.int8_scores(q, qs, x, xs, dtype=dtype).any()
+    assert torch.equal(px.int8_scores(q, qs, x, xs, bias=b, dtype=dtype), b.to(dtype).expand(33, n))
