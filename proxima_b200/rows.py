@@ -18,6 +18,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -94,15 +95,57 @@ def _stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _tangent(a) -> bool:
+    return forward_ad.unpack_dual(a).tangent is not None
+
+
+def _wanted(*tensors) -> bool:
+    """Whether a derivative with respect to one of the tensors may be asked
+    for: it requires a gradient, or carries a tangent (forward mode), of which
+    requires_grad says nothing."""
+    if torch.is_grad_enabled() and any(a is not None and a.requires_grad for a in tensors):
+        return True
+    # The level is -1 outside forward mode, where looking for tangents costs time.
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(a is not None and _tangent(a) for a in tensors)
+
+
+class _NoDerivative(torch.autograd.Function):
+    """An operator without a derivative: its results belong to the graph of
+    its inputs, and a backward pass that reaches them raises."""
+
+    @staticmethod
+    def forward(ctx, name, call, *tensors):
+        ctx.name = name
+        out = call()
+        if isinstance(out, tuple):
+            ctx.mark_non_differentiable(*(a for a in out if not a.is_floating_point()))
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no derivative: detach its inputs, or its results")
+
+
+def _without_derivative(name, call, *tensors):
+    """call(), as a step that cannot be differentiated in `tensors`."""
+    return _NoDerivative.apply(name, call, *tensors) if _wanted(*tensors) else call()
+
+
 def quantize_rows(x):
     """Cuts each row of x (n x dim, float32, float16 or bfloat16) to signed
     8-bit codes with one scale: ``scales = max|x| / 127`` (float32) and
     ``codes = x / scales`` rounded to nearest, ties to even. Returns (codes
     int8 n x dim, scales float32 n); the rows of codes start on 16-byte
     boundaries, as ``int8_scores`` reads them. A row of zeros has scale 0; a
-    row with a NaN or an infinity has scale NaN and codes 0."""
+    row with a NaN or an infinity has scale NaN and codes 0. Not
+    differentiable: a backward pass that reaches the scales raises."""
     _check(x, "x", 2, tuple(_TYPES))
-    n, dim, dev = x.shape[0], _dim(x, "x"), x.device
+    _dim(x, "x")
+    return _without_derivative("quantize_rows", lambda: _quantize(x), x)
+
+
+def _quantize(x):
+    (n, dim), dev = x.shape, x.device
     x = _plain(x)
     codes = _empty_rows(n, dim, torch.int8, dev)
     scales = torch.empty(n, dtype=torch.float32, device=dev)
@@ -116,7 +159,8 @@ def quantize_rows(x):
 
 def dequantize_rows(codes, scales, dtype=torch.float32):
     """The values 8-bit rows stand for: ``codes * scales[:, None]``, rounded
-    once to ``dtype`` (float32, float16 or bfloat16)."""
+    once to ``dtype`` (float32, float16 or bfloat16). Not differentiable: a
+    backward pass that reaches the result raises."""
     _check(codes, "codes", 2, (torch.int8,))
     _check(scales, "scales", 1, (torch.float32,))
     if dtype not in _TYPES:
@@ -125,6 +169,11 @@ def dequantize_rows(codes, scales, dtype=torch.float32):
     if scales.shape[0] != n:
         raise ValueError(f"scales length {scales.shape[0]} must equal the number of rows {n}")
     _same_device(codes.device, scales=scales)
+    return _without_derivative("dequantize_rows", lambda: _dequantize(codes, scales, dtype), scales)
+
+
+def _dequantize(codes, scales, dtype):
+    n, dim = codes.shape
     codes, scales = _plain(codes), scales.contiguous()
     out = torch.empty((n, dim), dtype=dtype, device=codes.device)
     if n:
@@ -141,7 +190,8 @@ def int8_scores(q_codes, q_scales, codes, scales, bias=None, dtype=torch.float32
     32-bit integers (dim <= 131071). ``bias`` (float32, n) is added to each
     base row's scores; with ``bias = -0.5 * |row|^2`` scores order rows as L2
     distance does. ``out`` receives the result if given (its rows may be
-    strided). Not differentiable."""
+    strided). Not differentiable: a backward pass that reaches the result
+    raises, and with ``out`` no input may require a gradient."""
     _check(q_codes, "q_codes", 2, (torch.int8,))
     _check(q_scales, "q_scales", 1, (torch.float32,))
     _check(codes, "codes", 2, (torch.int8,))
@@ -163,9 +213,7 @@ def int8_scores(q_codes, q_scales, codes, scales, bias=None, dtype=torch.float32
     if bias is not None and bias.shape[0] != n:
         raise ValueError(f"bias length {bias.shape[0]} must equal the number of rows {n}")
     _same_device(dev, q_codes=q_codes, q_scales=q_scales, scales=scales, bias=bias, out=out)
-    if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=dev)
-    else:
+    if out is not None:
         _check(out, "out", 2, (dtype,))
         if out.shape != (m, n):
             raise ValueError(f"out has shape {tuple(out.shape)}, expected {(m, n)}")
@@ -173,6 +221,16 @@ def int8_scores(q_codes, q_scales, codes, scales, bias=None, dtype=torch.float32
             raise ValueError("out must not require a gradient")
         if n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n:
             raise ValueError("out must have contiguous columns and rows that do not overlap")
+        if _wanted(q_scales, scales, bias):
+            raise ValueError("out cannot be given where a derivative may be asked for: detach the scales and the bias")
+    return _without_derivative("int8_scores", lambda: _scores(q_codes, q_scales, codes, scales, bias, dtype, out),
+                               q_scales, scales, bias)
+
+
+def _scores(q_codes, q_scales, codes, scales, bias, dtype, out):
+    (m, dim), n, dev = q_codes.shape, codes.shape[0], codes.device
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=dev)
     if m and n:
         (qc, ldq), (xc, ldx) = _tiled(q_codes), _tiled(codes)
         qs, xs = q_scales.contiguous(), scales.contiguous()
@@ -243,8 +301,8 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     """Cross entropy of queries (t x dim) under a softmax over all base rows
     (v x dim), both float16 or bfloat16, without keeping the t x v logits
     ``scale * queries @ rows.T + bias``: ``log sum_j exp z_ij - z_i,target``,
-    float32. Differentiable (once) in queries and rows; the backward computes
-    the logits again, in pieces of the base.
+    float32. Differentiable (once, backward) in queries and rows; the backward
+    computes the logits again, in pieces of the base.
 
     targets: int64, row numbers; ``ignore_index`` gives a query loss 0 and no
     gradient, any other number outside [0, v) loss NaN and no gradient. bias
@@ -283,7 +341,7 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
         loss = queries.float().sum(1) + rows[:0].float().sum()
         return {"none": lambda: loss, "sum": loss.sum, "mean": loss.mean}[reduction]()
     args = (queries, rows, targets, scale, bias, ignore_index, _REDUCTIONS[reduction])
-    if torch.is_grad_enabled() and (queries.requires_grad or rows.requires_grad):
+    if _wanted(queries, rows, bias):
         return _SoftmaxCrossEntropy.apply(*args)
     return _xent_forward(*args)[0]
 

@@ -2,6 +2,7 @@
 beyond their argument checks."""
 
 import pytest
+import torch
 
 
 @pytest.mark.parametrize("t,v,d", [(1, 10_000_000, 64), (1, 100_000_000, 8), (65, 2_000_000, 64), (1000, 100_000, 384), (5000, 60_000, 128)])
@@ -16,3 +17,35 @@ def test_gradient_pieces_keep_their_bound(px, t, v, d):
     columns = piece // (4 * padded)
     parts = 2 * (columns // 64 + 4) * ((t + 255) // 256 * 8)
     assert 0 < need <= piece + 148 * 256 * 256 * 4 + parts + 4096
+
+
+def test_operators_without_a_derivative_say_so():
+    from torch.autograd import forward_ad
+
+    from proxima_b200 import rows
+
+    x = torch.ones(3, requires_grad=True)
+
+    def call():
+        return torch.ones(3, dtype=torch.int8), torch.ones(3)
+
+    codes, scales = rows._without_derivative("op", call, x, None)
+    assert scales.requires_grad and not codes.requires_grad
+    with pytest.raises(RuntimeError, match="op has no derivative"):
+        scales.sum().backward()
+    with pytest.raises(RuntimeError, match="op has no derivative"):
+        torch.autograd.grad((scales * x).sum(), x)
+    # Nothing asked for: the results as they are.
+    with torch.no_grad():
+        assert not rows._without_derivative("op", call, x)[1].requires_grad
+    assert not rows._without_derivative("op", call, x.detach(), None)[1].requires_grad
+    with forward_ad.dual_level():
+        plain = x.detach()
+        dual = forward_ad.make_dual(plain, torch.ones(3))
+        assert rows._wanted(None, dual) and not rows._wanted(plain, None)
+        with torch.no_grad():
+            assert rows._wanted(dual)
+        with pytest.raises(NotImplementedError):
+            rows._without_derivative("op", call, dual)
+        rows._without_derivative("op", call, plain)
+    assert not rows._wanted(plain)

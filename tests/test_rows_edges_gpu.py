@@ -282,3 +282,50 @@ def test_int8_scores_of_zero_sums(px, dtype, n):
     b = torch.arange(n, device="cuda") % 100 + 0.5
     assert not px.int8_scores(q, qs, x, xs, dtype=dtype).any()
     assert torch.equal(px.int8_scores(q, qs, x, xs, bias=b, dtype=dtype), b.to(dtype).expand(33, n))
+
+
+# ---------------------------------------------------------------- derivatives that do not exist
+
+def test_derivatives_do_not_vanish(px):
+    """Where an operator has no derivative, asking for one raises; nothing
+    comes back as if the derivative were zero."""
+    from torch.autograd import forward_ad
+
+    x, codes = _rand(5, 32, seed=1), torch.ones(5, 32, dtype=torch.int8, device="cuda")
+    scales, bias = torch.ones(5, device="cuda"), torch.zeros(5, device="cuda")
+    q, r, y, _ = _xent_case(4, 9, 32, torch.bfloat16, 2)
+    uses = {
+        "quantize_rows": [lambda a: px.quantize_rows(a)[1], x],
+        "dequantize_rows": [lambda a: px.dequantize_rows(codes, a), scales],
+        "int8_scores": [lambda a: px.int8_scores(codes, a, codes, scales), scales],
+        "int8_scores rows": [lambda a: px.int8_scores(codes, scales, codes, a), scales],
+        "int8_scores bias": [lambda a: px.int8_scores(codes, scales, codes, scales, bias=a), bias],
+    }
+    for name, (use, a) in uses.items():
+        want = use(a)
+        got = use(a.clone().requires_grad_())
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match=f"{name.split()[0]} has no derivative"):
+            got.sum().backward()
+        with torch.no_grad():
+            assert not use(a.clone().requires_grad_()).requires_grad
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError):
+                use(forward_ad.make_dual(a.clone(), torch.ones_like(a)))
+            assert torch.equal(use(a), want)
+    out = torch.empty(5, 5, device="cuda")
+    with pytest.raises(ValueError, match="out cannot be given"):
+        px.int8_scores(codes, scales, codes, scales, bias=bias.clone().requires_grad_(), out=out)
+    with torch.no_grad():
+        assert px.int8_scores(codes, scales, codes, scales, bias=bias.clone().requires_grad_(), out=out) is out
+    # The loss has a backward derivative only.
+    loss = px.softmax_cross_entropy(q, r, y)
+    with forward_ad.dual_level():
+        b = torch.zeros(9, device="cuda")
+        for args, kw in (((forward_ad.make_dual(q, q), r, y), {}), ((q, forward_ad.make_dual(r, r), y), {}),
+                         ((q, r, y), {"bias": forward_ad.make_dual(b, b)})):
+            with pytest.raises(NotImplementedError):
+                px.softmax_cross_entropy(*args, **kw)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                px.softmax_cross_entropy(*args, **kw)
+        assert torch.equal(px.softmax_cross_entropy(q, r, y), loss)
