@@ -14,9 +14,9 @@ imported when one of them is first used.
 from ._core import FlatIndex, Metric, PqIndex, PX_MAX_K, PxError  # noqa: F401
 from ._lib import device_count, launch_count, set_profiling, LIB_PATH  # noqa: F401
 
+# Not the operators on tensors: a star import would need torch.
 __all__ = ["FlatIndex", "PqIndex", "Metric", "PxError", "PX_MAX_K", "device_count",
-           "launch_count", "set_profiling", "quantize_rows", "dequantize_rows", "int8_scores",
-           "softmax_cross_entropy", "rows_status"]
+           "launch_count", "set_profiling"]
 __version__ = "0.1.0"
 
 _ROWS = ("quantize_rows", "dequantize_rows", "int8_scores", "softmax_cross_entropy", "rows_status")
@@ -28,3 +28,7 @@ def __getattr__(name):
         globals().update({n: getattr(rows, n) for n in _ROWS})
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_ROWS})

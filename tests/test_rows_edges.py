@@ -49,3 +49,26 @@ def test_operators_without_a_derivative_say_so():
             rows._without_derivative("op", call, dual)
         rows._without_derivative("op", call, plain)
     assert not rows._wanted(plain)
+
+
+def test_the_package_needs_no_torch():
+    """A star import in a process that has no torch: the searches are there,
+    and the operators on tensors say what they miss when they are first used."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import sys
+sys.modules["torch"] = None  # importing it raises
+from proxima_b200 import *
+import proxima_b200
+assert FlatIndex and PqIndex and Metric and PxError and "softmax_cross_entropy" in dir(proxima_b200)
+try:
+    proxima_b200.quantize_rows
+except ImportError:
+    print("no torch")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip() == "no torch", r.stderr[-2000:]
