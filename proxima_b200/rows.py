@@ -10,7 +10,8 @@ Each call runs on the current torch stream of its tensors' device and returns
 without waiting. Tensors must be CUDA tensors of one device (TypeError /
 ValueError otherwise); arrays whose columns are not contiguous, or whose rows
 do not start on 16-byte boundaries where the tensor cores read them, are
-copied first. The kernels are libproxima_b200's; there is no fallback.
+copied first. The kernels are libproxima_b200's; there is no fallback, and the
+calls cannot be traced (RuntimeError; torch.compile runs them between graphs).
 """
 
 from __future__ import annotations
@@ -25,6 +26,14 @@ from . import _lib
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _INT8_MAX_DIM = 131071
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _not_traced(name: str) -> None:
+    """A trace would record the empty results, not what the kernels write to
+    their memory."""
+    if torch._C._is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None:
+        raise RuntimeError(f"{name} cannot be traced: its kernels run on the tensors' memory")
 
 
 def _check(a, name: str, ndim: int, dtypes) -> None:
@@ -139,6 +148,7 @@ def quantize_rows(x):
     boundaries, as ``int8_scores`` reads them. A row of zeros has scale 0; a
     row with a NaN or an infinity has scale NaN and codes 0. Not
     differentiable: a backward pass that reaches the scales raises."""
+    _not_traced("quantize_rows")
     _check(x, "x", 2, tuple(_TYPES))
     _dim(x, "x")
     return _without_derivative("quantize_rows", lambda: _quantize(x), x)
@@ -161,6 +171,7 @@ def dequantize_rows(codes, scales, dtype=torch.float32):
     """The values 8-bit rows stand for: ``codes * scales[:, None]``, rounded
     once to ``dtype`` (float32, float16 or bfloat16). Not differentiable: a
     backward pass that reaches the result raises."""
+    _not_traced("dequantize_rows")
     _check(codes, "codes", 2, (torch.int8,))
     _check(scales, "scales", 1, (torch.float32,))
     if dtype not in _TYPES:
@@ -192,6 +203,7 @@ def int8_scores(q_codes, q_scales, codes, scales, bias=None, dtype=torch.float32
     distance does. ``out`` receives the result if given (its rows may be
     strided). Not differentiable: a backward pass that reaches the result
     raises, and with ``out`` no input may require a gradient."""
+    _not_traced("int8_scores")
     _check(q_codes, "q_codes", 2, (torch.int8,))
     _check(q_scales, "q_scales", 1, (torch.float32,))
     _check(codes, "codes", 2, (torch.int8,))
@@ -312,6 +324,7 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     positive number (one over the temperature). reduction: "mean" (over the
     queries not ignored; NaN if there are none), "sum" or "none". Queries and
     rows must be finite even where ignored or left out."""
+    _not_traced("softmax_cross_entropy")
     _check(queries, "queries", 2, (torch.float16, torch.bfloat16))
     _check(rows, "rows", 2, (queries.dtype,))
     _check(targets, "targets", 1, (torch.int64,))

@@ -72,3 +72,16 @@ except ImportError:
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.strip() == "no torch", r.stderr[-2000:]
+
+
+def test_traces_are_refused(px):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, codes, y = torch.ones(3, 8), torch.ones(3, 8, dtype=torch.int8), torch.zeros(3, dtype=torch.int64)
+    for name, use in (("quantize_rows", lambda a: px.quantize_rows(a)[1]),
+                      ("dequantize_rows", lambda a: px.dequantize_rows(codes, a[:, 0])),
+                      ("int8_scores", lambda a: px.int8_scores(codes, a[:, 0], codes, a[:, 0])),
+                      ("softmax_cross_entropy", lambda a: px.softmax_cross_entropy(a, a, y))):
+        for trace in (lambda: torch.jit.trace(use, x, check_trace=False), lambda: make_fx(use)(x)):
+            with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+                trace()

@@ -329,3 +329,27 @@ def test_derivatives_do_not_vanish(px):
             with torch.no_grad(), pytest.raises(NotImplementedError):
                 px.softmax_cross_entropy(*args, **kw)
         assert torch.equal(px.softmax_cross_entropy(q, r, y), loss)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_row_operators_in_compiled_functions(px):
+    # A compiled function runs the operators between its graphs.
+    import torch._dynamo
+
+    q, r, y, b = _xent_case(20, 300, 40, torch.bfloat16, 9, bias=True)
+
+    def step(q, r):
+        loss = px.softmax_cross_entropy(q * 0.5, r, y, scale=2.0, bias=b) * 3
+        codes, scales = px.quantize_rows(r.detach().float() + 0.0)
+        qc, qs = px.quantize_rows(q.detach() * 2)
+        return loss, px.int8_scores(qc, qs, codes, scales) + 1, px.dequantize_rows(codes, scales * 2)
+
+    def all_of(f):
+        a, c = q.detach().clone().requires_grad_(), r.detach().clone().requires_grad_()
+        loss, *rest = f(a, c)
+        return [loss.detach(), *torch.autograd.grad(loss, (a, c)), *rest]
+
+    want = all_of(step)
+    torch._dynamo.reset()
+    got = all_of(torch.compile(step, backend="eager"))
+    assert all(torch.equal(x, w) for x, w in zip(got, want))
