@@ -321,9 +321,10 @@ PX_API px_status px_int8_scores_device(int32_t device, const int8_t* q, int64_t 
  * a row out of the softmax.
  * A query whose target is ignore_index has loss 0 (its lse is still written);
  * one whose target is any other number outside [0, v) has loss NaN; one whose
- * target is left out, +infinity. total (2 floats) receives, for PX_REDUCE_SUM
- * and PX_REDUCE_MEAN, the reduced loss and what it was divided by (1, or the
- * number of queries not ignored; a mean over none is NaN). workspace: 16-byte
+ * target is left out, +infinity. For PX_REDUCE_SUM and PX_REDUCE_MEAN, total
+ * (one float) receives the reduced loss and divisor (one float) what it was
+ * divided by (1, or the number of queries not ignored; a mean over none is NaN,
+ * with zero gradients). Both may be NULL for PX_REDUCE_NONE. workspace: 16-byte
  * aligned, px_softmax_xent_workspace_bytes(..., backward = 0) bytes, free
  * once the call's work is done. */
 enum { PX_REDUCE_NONE = 0, PX_REDUCE_SUM = 1, PX_REDUCE_MEAN = 2 };
