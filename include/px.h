@@ -357,7 +357,9 @@ PX_API px_status px_softmax_xent_backward_device(int32_t device, const void* que
 
 /* Waits for `stream` and returns PX_ETIMEOUT if a bounded device-side wait of
  * a row operator on `device` has given up since the last call (what it left
- * undone is NaN in its outputs). */
+ * undone is NaN in its outputs). There is one such record per device, for all
+ * streams and threads, and the call clears it: it may report another caller's
+ * timeout, and take it from them. The NaNs stay with the outputs. */
 PX_API px_status px_rows_status_device(int32_t device, void* stream);
 
 #ifdef __cplusplus

@@ -362,6 +362,7 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
 def rows_status(device=None) -> None:
     """Waits for the device's current stream and raises PxError (ETIMEOUT) if
     a bounded device-side wait of one of these operators has given up since
-    the last call; the results it left undone are NaN."""
+    the last call; the results it left undone are NaN. The record is one per
+    device, for all streams and threads, and the call clears it."""
     device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index)
     _lib.check(_lib.load().px_rows_status_device(device.index, _stream(device.index)))
