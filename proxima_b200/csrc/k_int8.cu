@@ -14,8 +14,8 @@
 // What bounds it: the matrix itself. At 4 bytes a score the write takes longer
 // than the products for d up to about 1000, with few queries the base's read
 // is what remains. So the queries are kept in shared memory across base tiles
-// where they fit (KC slices of N/2 rows; d <= 896 at N = 256), and only base
-// rows stream through the ring.
+// where they fit beside 80 KB of ring (KC slices of N/2 rows; at N = 256 d <= 768,
+// or 1024 where nothing is staged), and only base rows stream through the ring.
 // Measured, fp32 out: 64 x 1M x 128 in 75 us and 1000 x 100k x 384 in 98 us,
 // 0.79 and 0.69 of what their bytes take at a copy's rate; runs of 512 bytes
 // per row of `out` are what keeps the writes from more. bf16 out: 10k x 100k x
