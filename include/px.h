@@ -294,7 +294,8 @@ enum { PX_F32 = 0, PX_F16 = 1, PX_BF16 = 2 };
 /* 8-bit rows: scales[i] = max_j |x_ij| / 127 and codes[i][j] = x_ij /
  * scales[i] rounded to nearest (ties to even, exactly rounded quotients). A
  * row of zeros has scale 0 and codes 0; a row holding a NaN or an infinity
- * has scale NaN and codes 0. x is n x dim of `type`. */
+ * has scale NaN and codes 0. Codes stay within 127 also where a scale below
+ * 1e-38 is itself rounded. x is n x dim of `type`. */
 PX_API px_status px_quantize_rows_device(int32_t device, const void* x, int32_t type, int64_t n, int32_t dim,
                                          int64_t ldx, int8_t* codes, int64_t ldc, float* scales, void* stream);
 /* out[i][j] = codes[i][j] * scales[i], n x dim of `type`. */
@@ -318,7 +319,8 @@ PX_API px_status px_int8_scores_device(int32_t device, const int8_t* q, int64_t 
  * queries (t x dim) and rows (v x dim) are PX_F16 or PX_BF16 with rows on
  * 16-byte boundaries; targets are row numbers; bias (v floats, 16-byte
  * aligned) may be NULL, and -infinity in it, or any value below -2e31, leaves
- * a row out of the softmax.
+ * a row out of the softmax; values above 1e31 make losses NaN. scale is positive
+ * and below 2^127.
  * A query whose target is ignore_index has loss 0 (its lse is still written);
  * one whose target is any other number outside [0, v) has loss NaN; one whose
  * target is left out, +infinity. For PX_REDUCE_SUM and PX_REDUCE_MEAN, total

@@ -78,6 +78,8 @@ px_status check_xent(int64_t t, int64_t v, int32_t dim, const void* q, int64_t l
   if (type != PX_F16 && type != PX_BF16)
     return set_error(type == PX_F32 ? PX_EUNSUPPORTED : PX_EINVAL, "queries and rows must be PX_F16 or PX_BF16");
   if (!(scale > 0.0f) || std::isinf(scale)) return set_error(PX_EINVAL, "scale must be positive and finite");
+  // Logits are taken in log2 units: scale * log2(e) has to be a number.
+  if (scale >= 0x1p127f) return set_error(PX_EINVAL, "scale must be below 2^127");
   if (t == 0) return PX_OK;
   s = check_tiled(q, ldq, 2, dim, "queries");
   if (s == PX_OK) s = check_tiled(rows, ldr, 2, dim, "rows");

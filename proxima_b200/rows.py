@@ -146,8 +146,10 @@ def quantize_rows(x):
     ``codes = x / scales`` rounded to nearest, ties to even. Returns (codes
     int8 n x dim, scales float32 n); the rows of codes start on 16-byte
     boundaries, as ``int8_scores`` reads them. A row of zeros has scale 0; a
-    row with a NaN or an infinity has scale NaN and codes 0. Not
-    differentiable: a backward pass that reaches the scales raises."""
+    row with a NaN or an infinity has scale NaN and codes 0. Codes stay within
+    127 also where the scale is so small (below 1e-38) that it is itself
+    rounded. Not differentiable: a backward pass that reaches the scales
+    raises."""
     _not_traced("quantize_rows")
     _check(x, "x", 2, tuple(_TYPES))
     _dim(x, "x")
@@ -320,8 +322,8 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     gradient, any other number outside [0, v) loss NaN and no gradient. bias
     (float32, v, no gradient): added to a row's logits, for instance the
     correction for how rows were sampled; -inf (or any value below -2e31)
-    leaves a row out. scale: a
-    positive number (one over the temperature). reduction: "mean" (over the
+    leaves a row out; above 1e31 it
+    makes losses NaN. scale: a positive number (one over the temperature). reduction: "mean" (over the
     queries not ignored; NaN if there are none), "sum" or "none". Queries and
     rows must be finite even where ignored or left out."""
     _not_traced("softmax_cross_entropy")
@@ -335,6 +337,8 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     scale = float(scale)
     if not scale > 0.0 or math.isinf(scale):
         raise ValueError("scale must be positive and finite")
+    if scale >= 2.0 ** 127:
+        raise ValueError("scale must be below 2^127")
     ignore_index = int(ignore_index)
     if not -2 ** 63 <= ignore_index < 2 ** 63:
         raise ValueError("ignore_index must be a 64-bit integer")

@@ -85,3 +85,13 @@ def test_traces_are_refused(px):
         for trace in (lambda: torch.jit.trace(use, x, check_trace=False), lambda: make_fx(use)(x)):
             with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
                 trace()
+
+
+def test_scales_whose_logits_would_not_be_numbers(px):
+    import ctypes
+
+    at = ctypes.c_void_p(16)
+    for scale in (2.0 ** 127, 3.4e38):
+        status = px._lib.load().px_softmax_xent_device(0, at, 8, 4, at, 8, 6, 8, 2, at, -100, scale, None, 0, at, at, at, at,
+                                                       None, 0, None)
+        assert status == px._lib.PX_EINVAL and "scale must be below 2^127" in px._lib.last_error()

@@ -353,3 +353,15 @@ def test_row_operators_in_compiled_functions(px):
     torch._dynamo.reset()
     got = all_of(torch.compile(step, backend="eager"))
     assert all(torch.equal(x, w) for x, w in zip(got, want))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 126, 2.0 ** -140])
+def test_softmax_scales_at_the_ends(px, scale):
+    q, r, y, _ = _xent_case(3, 20, 16, torch.bfloat16, 3)
+    with torch.no_grad():
+        q.zero_()  # logits of zero, whatever the scale
+    loss = px.softmax_cross_entropy(q, r, y, scale=scale, reduction="none")
+    assert ((loss.double() - math.log(20)).abs() <= 1e-5).all()
+    for large in (2.0 ** 127, 1e39, 1e300):
+        with pytest.raises(ValueError, match="scale must be below"):
+            px.softmax_cross_entropy(q, r, y, scale=large)
