@@ -8,8 +8,8 @@ import math
 import pytest
 import torch
 
-from test_rows_gpu import (ACC, HALF, TINY, TYPES, U, _check_xent, _rand, _scores64, _scores_bound, _scores_case, _within,
-                           _xent_case)
+from test_rows_gpu import (ACC, HALF, TINY, TYPES, U, _check_xent, _codes64, _rand, _scores64, _scores_bound, _scores_case,
+                           _within, _xent_case)
 
 pytestmark = pytest.mark.gpu
 
@@ -365,3 +365,24 @@ def test_softmax_scales_at_the_ends(px, scale):
     for large in (2.0 ** 127, 1e39, 1e300):
         with pytest.raises(ValueError, match="scale must be below"):
             px.softmax_cross_entropy(q, r, y, scale=large)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [1025, 2048, 5000])
+def test_quantize_long_strided_rows(px, dtype, d):
+    # Rows longer than a group's registers hold, with something between them:
+    # values on and beside halves of the scale, zeros, infinities, NaN at the end.
+    s = torch.tensor([1.0, 0.375, 2.0 ** -12], dtype=torch.float64)
+    at = (torch.arange(d, dtype=torch.float64) % 253 - 126.5)
+    x = torch.full((9, d + 40), math.nan, dtype=torch.float64)
+    x[:3, :d] = s[:, None] * at
+    x[3:6, :d] = torch.nextafter((s[:, None] * at).to(dtype), torch.full((3, d), 300.0, dtype=dtype)).double()
+    x[:6, d - 1] = torch.cat([s, s]) * 127
+    x[6:, :d] = 0.0
+    x[7, 3], x[8, 5] = math.inf, 1.0
+    x[8, d - 1] = math.nan
+    x = x.to(dtype).cuda()[:, :d]
+    codes, scales = px.quantize_rows(x)
+    assert scales[6] == 0 and scales[7:].isnan().all() and not codes[6:].any()
+    want, want_scales = _codes64(x[:6])
+    assert torch.equal(scales[:6], want_scales) and torch.equal(codes[:6], want)
