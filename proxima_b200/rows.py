@@ -27,12 +27,13 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _INT8_MAX_DIM = 131071
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _dispatch_mode, _is_grad_enabled = torch._C._is_tracing, torch._C._get_dispatch_mode, torch.is_grad_enabled
 
 
 def _not_traced(name: str) -> None:
     """A trace would record the empty results, not what the kernels write to
     their memory."""
-    if torch._C._is_tracing() or torch._C._get_dispatch_mode(_PROXY) is not None:
+    if _is_tracing() or _dispatch_mode(_PROXY) is not None:
         raise RuntimeError(f"{name} cannot be traced: its kernels run on the tensors' memory")
 
 
@@ -104,18 +105,17 @@ def _stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _tangent(a) -> bool:
-    return forward_ad.unpack_dual(a).tangent is not None
-
-
 def _wanted(*tensors) -> bool:
     """Whether a derivative with respect to one of the tensors may be asked
     for: it requires a gradient, or carries a tangent (forward mode), of which
     requires_grad says nothing."""
-    if torch.is_grad_enabled() and any(a is not None and a.requires_grad for a in tensors):
-        return True
+    if _is_grad_enabled():
+        for a in tensors:
+            if a is not None and a.requires_grad:
+                return True
     # The level is -1 outside forward mode, where looking for tangents costs time.
-    return getattr(forward_ad, "_current_level", 0) >= 0 and any(a is not None and _tangent(a) for a in tensors)
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        a is not None and forward_ad.unpack_dual(a).tangent is not None for a in tensors)
 
 
 class _NoDerivative(torch.autograd.Function):
@@ -123,9 +123,9 @@ class _NoDerivative(torch.autograd.Function):
     its inputs, and a backward pass that reaches them raises."""
 
     @staticmethod
-    def forward(ctx, name, call, *tensors):
+    def forward(ctx, name, call, *args):
         ctx.name = name
-        out = call()
+        out = call(*args)
         if isinstance(out, tuple):
             ctx.mark_non_differentiable(*(a for a in out if not a.is_floating_point()))
         return out
@@ -133,11 +133,6 @@ class _NoDerivative(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         raise RuntimeError(f"{ctx.name} has no derivative: detach its inputs, or its results")
-
-
-def _without_derivative(name, call, *tensors):
-    """call(), as a step that cannot be differentiated in `tensors`."""
-    return _NoDerivative.apply(name, call, *tensors) if _wanted(*tensors) else call()
 
 
 def quantize_rows(x):
@@ -153,7 +148,7 @@ def quantize_rows(x):
     _not_traced("quantize_rows")
     _check(x, "x", 2, tuple(_TYPES))
     _dim(x, "x")
-    return _without_derivative("quantize_rows", lambda: _quantize(x), x)
+    return _NoDerivative.apply("quantize_rows", _quantize, x) if _wanted(x) else _quantize(x)
 
 
 def _quantize(x):
@@ -182,7 +177,8 @@ def dequantize_rows(codes, scales, dtype=torch.float32):
     if scales.shape[0] != n:
         raise ValueError(f"scales length {scales.shape[0]} must equal the number of rows {n}")
     _same_device(codes.device, scales=scales)
-    return _without_derivative("dequantize_rows", lambda: _dequantize(codes, scales, dtype), scales)
+    args = (codes, scales, dtype)
+    return _NoDerivative.apply("dequantize_rows", _dequantize, *args) if _wanted(scales) else _dequantize(*args)
 
 
 def _dequantize(codes, scales, dtype):
@@ -235,10 +231,12 @@ def int8_scores(q_codes, q_scales, codes, scales, bias=None, dtype=torch.float32
             raise ValueError("out must not require a gradient")
         if n > 1 and out.stride(1) != 1 or m > 1 and out.stride(0) < n:
             raise ValueError("out must have contiguous columns and rows that do not overlap")
-        if _wanted(q_scales, scales, bias):
-            raise ValueError("out cannot be given where a derivative may be asked for: detach the scales and the bias")
-    return _without_derivative("int8_scores", lambda: _scores(q_codes, q_scales, codes, scales, bias, dtype, out),
-                               q_scales, scales, bias)
+    args = (q_codes, q_scales, codes, scales, bias, dtype, out)
+    if not _wanted(q_scales, scales, bias):
+        return _scores(*args)
+    if out is not None:
+        raise ValueError("out cannot be given where a derivative may be asked for: detach the scales and the bias")
+    return _NoDerivative.apply("int8_scores", _scores, *args)
 
 
 def _scores(q_codes, q_scales, codes, scales, bias, dtype, out):

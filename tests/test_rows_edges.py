@@ -26,10 +26,13 @@ def test_operators_without_a_derivative_say_so():
 
     x = torch.ones(3, requires_grad=True)
 
-    def call():
+    def call(a, b):
         return torch.ones(3, dtype=torch.int8), torch.ones(3)
 
-    codes, scales = rows._without_derivative("op", call, x, None)
+    def use(a, b=None):
+        return rows._NoDerivative.apply("op", call, a, b) if rows._wanted(a, b) else call(a, b)
+
+    codes, scales = use(x)
     assert scales.requires_grad and not codes.requires_grad
     with pytest.raises(RuntimeError, match="op has no derivative"):
         scales.sum().backward()
@@ -37,8 +40,8 @@ def test_operators_without_a_derivative_say_so():
         torch.autograd.grad((scales * x).sum(), x)
     # Nothing asked for: the results as they are.
     with torch.no_grad():
-        assert not rows._without_derivative("op", call, x)[1].requires_grad
-    assert not rows._without_derivative("op", call, x.detach(), None)[1].requires_grad
+        assert not rows._wanted(x) and not use(x)[1].requires_grad
+    assert not rows._wanted(x.detach(), None) and not use(x.detach())[1].requires_grad
     with forward_ad.dual_level():
         plain = x.detach()
         dual = forward_ad.make_dual(plain, torch.ones(3))
@@ -46,8 +49,8 @@ def test_operators_without_a_derivative_say_so():
         with torch.no_grad():
             assert rows._wanted(dual)
         with pytest.raises(NotImplementedError):
-            rows._without_derivative("op", call, dual)
-        rows._without_derivative("op", call, plain)
+            use(dual)
+        use(plain)
     assert not rows._wanted(plain)
 
 
