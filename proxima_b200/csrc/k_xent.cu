@@ -927,6 +927,7 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
             for (int j = 0; j < 16; ++j)
               w[16 * h + j] = pack2<BF>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])) ^ sign;
           }
+          if (mine) top = max2(top, fabsf(at_target));
           two = __any_sync(0xffffffffu, !(top <= kLarge * fabsf(factor)));
           // The columns are in registers: the accumulator is free.
           if (!two) release();

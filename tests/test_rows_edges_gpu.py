@@ -64,10 +64,12 @@ def _check_gradients(px, q, r, y, b, scale):
 
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("t,v,d", [(1, 2, 64), (40, 300, 64), (200, 5000, 200), (33, 66, 520), (70, 1000, 19), (300, 260_009, 64)])
-def test_softmax_hard_negatives(px, dtype, t, v, d):
+@pytest.mark.parametrize("behind", [0.0, 7.0])
+def test_softmax_hard_negatives(px, dtype, t, v, d, behind):
     # Each query is its own row, and one other row differs from that in one
-    # place by a little: both hold about half of the softmax, and in all other
-    # places their parts of dq cancel. The values are whole sixteenths.
+    # place by a little: both hold about half of the softmax (or, the target
+    # being behind, the other nearly all), and in all other places their parts of
+    # dq cancel. The values are whole sixteenths.
     g = torch.Generator(device="cuda").manual_seed(t + v + d)
     r = torch.randint(-16, 17, (v, d), device="cuda", generator=g).double() / 16
     order = torch.randperm(v, device="cuda", generator=g)
@@ -79,6 +81,7 @@ def test_softmax_hard_negatives(px, dtype, t, v, d):
     scale = 2.0 ** round(math.log2(24 / float(q.square().sum(1).mean())))
     b = torch.full((v,), -24.0, device="cuda")
     b[order[:2 * t]] = 0.0
+    b[y] = -behind
     unit = 8 * ((d + 7) // 8)
     qx, rx = (torch.zeros(n, unit, dtype=dtype, device="cuda")[:, :d] for n in (t, v))
     _check_gradients(px, qx.copy_(q), rx.copy_(r), y, b, scale)
