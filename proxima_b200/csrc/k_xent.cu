@@ -916,38 +916,40 @@ xent_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
               }
             }
           };
-          uint32_t w[32];
-          float top = 0.0f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t v[32];
-            entries(v, h);
-            top = max2(top, largest(v));
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              w[16 * h + j] = pack2<BF>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])) ^ sign;
-          }
-          if (mine) top = max2(top, fabsf(at_target));
-          two = __any_sync(0xffffffffu, !(top <= kLarge * fabsf(factor)));
-          // The columns are in registers: the accumulator is free.
-          if (!two) release();
-          if (mine) put(w, at_target);
-          leave(w, 0);
-          if (two) {
-            // The products once more, for what the rounding took.
+          // A pass over the columns for each part, the second from the products again: the
+          // same code, with no registers kept in between (with biases the first part's
+          // entries, kept, made a piece of 333 x 50,021 x 100 take 45 us in place of 35).
+#pragma unroll 1
+          for (int part = 0; part == 0 || (part == 1 && two); ++part) {
+            uint32_t w[32];
+            float top = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t v[32];
               entries(v, h);
-              if (h == 1) release();
+              if (part == 0) {
+                top = max2(top, largest(v));
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float2 r = widen2<BF>(w[16 * h + j] ^ sign);
-                w[16 * h + j] = pack2<BF>(__uint_as_float(v[2 * j]) - r.x, __uint_as_float(v[2 * j + 1]) - r.y) ^ sign;
+                for (int j = 0; j < 16; ++j)
+                  w[16 * h + j] = pack2<BF>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])) ^ sign;
+              } else {
+                // What the rounding took. The last columns are in registers: the accumulator is free.
+                if (h == 1) release();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  const float a = __uint_as_float(v[2 * j]), b = __uint_as_float(v[2 * j + 1]);
+                  const float2 r = widen2<BF>(pack2<BF>(a, b));
+                  w[16 * h + j] = pack2<BF>(a - r.x, b - r.y) ^ sign;
+                }
               }
             }
-            if (mine) put(w, at_target - rounded<BF>(at_target));
-            leave(w, 1);
+            if (part == 0) {
+              if (mine) top = max2(top, fabsf(at_target));
+              two = __any_sync(0xffffffffu, !(top <= kLarge * fabsf(factor)));
+              if (!two) release();
+            }
+            if (mine) put(w, part == 0 ? at_target : at_target - rounded<BF>(at_target));
+            leave(w, part);
           }
         } else {
           release();
