@@ -306,9 +306,10 @@ PX_API px_status px_dequantize_rows_device(int32_t device, const int8_t* codes, 
 /* The whole score matrix of m 8-bit queries and n 8-bit base rows:
  * out[i][j] = (sum_l q[i][l] * x[j][l]) * q_scales[i] * x_scales[j] + bias[j]
  * (bias may be NULL), m x n of `type`, computed in fp32 from left to right. The
- * sums are exact in 32-bit integers (dim <= 131071). With bias[j] = -|x_j|^2 / 2 the descending order of a row
- * of `out` is the ascending order of L2 distance. Code rows start on 16-byte
- * boundaries (q, x 16-byte aligned; ldq, ldx multiples of 16). */
+ * sums are exact in 32-bit integers (dim <= 131071). With bias[j] = -|x_j|^2 / 2
+ * the descending order of a row of `out` is the ascending order of L2 distance.
+ * Code rows start on 16-byte boundaries (q, x 16-byte aligned; ldq, ldx multiples
+ * of 16). */
 PX_API px_status px_int8_scores_device(int32_t device, const int8_t* q, int64_t ldq, const float* q_scales, int64_t m,
                                        const int8_t* x, int64_t ldx, const float* x_scales, int64_t n, int32_t dim,
                                        const float* bias, int32_t type, void* out, int64_t ldo, void* stream);

@@ -16,12 +16,12 @@
 // is what remains. So the queries are kept in shared memory across base tiles
 // where they fit beside 80 KB of ring (KC slices of N/2 rows; at N = 256 d <= 768,
 // or 1024 where nothing is staged), and only base rows stream through the ring.
-// Measured, fp32 out: 64 x 1M x 128 in 75 us and 1000 x 100k x 384 in 98 us,
-// 0.79 and 0.69 of what their bytes take at a copy's rate; runs of 512 bytes
-// per row of `out` are what keeps the writes from more. bf16 out: 10k x 100k x
-// 768 in 800 us, 1.92 POP/s; 640 us without its stores and 544 us with no
-// epilogue at all, under the power cap (677 us when the GPU is cool), where
-// the 2 GB of scores cost energy as well as time.
+// Measured, fp32 out: 64 x 1M x 128 in 75 us and 1000 x 100k x 384 in 97 us,
+// 0.79 and 0.70 of what their bytes take at a copy's rate; longer runs per row
+// of `out` (1 KB) did not change that. bf16 out: 10k x 100k x 768 in 804-818 us,
+// 1.9 POP/s, under the power cap; 786 us back to back, 642 without its stores
+// and 544 with no epilogue at all, and 677, 553 and 461 when the GPU is cool. So
+// the epilogue and its stores take 216 us that the products do not hide.
 //
 // Order. Clusters form teams. The clusters of a team take neighbouring base
 // tiles of one query group, so what is written at any time is long runs of 256

@@ -67,13 +67,14 @@
 // them); the forward at small d by the exponentials (one per logit, 16 per SM
 // and clock: 2048 clocks per tile against 512 per slice of products). Computing
 // a quarter or three eighths of them by a polynomial on the FMA pipe was slower
-// (1000 x 1M x 128: 374 and 396 us against 351 then): issue slots run short.
-// Measured, bf16: forward 1000 x 1M x 128 327 us (2900 clocks per tile), 4096 x
+// (1000 x 1M x 128: 374 and 396 us against 351 then), though issue slots are 52% busy.
+// Measured, bf16: forward 1000 x 1M x 128 327-345 us (2900 clocks per tile), 4096 x
 // 100k x 384 1.53 PFLOP/s and, with the epilogue left out, 1.60; past the kept
 // slices the operands' way from L2 counts (d = 768: 1.25, 1.30). A training
-// step of 1000 x 100k x 384: 380 us in two pieces; 8192 x 8192 x 768 (fp16): 495
-// us with targets at random, so that four slices of G in five have a second
-// part. One part throughout: 343 and 418; two throughout: 499 and 551.
+// step of 1000 x 100k x 384: 355-395 us in two pieces; 8192 x 8192 x 768 (fp16):
+// 403-414 us with each query's own row as its target, 489-509 with targets at
+// random, so that four slices of G in five have a second part. One part
+// throughout: 343 and 418; two throughout: 499 and 551.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

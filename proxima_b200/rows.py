@@ -323,7 +323,9 @@ def softmax_cross_entropy(queries, rows, targets, scale=1.0, bias=None, ignore_i
     leaves a row out; above 1e31 it
     makes losses NaN. scale: a positive number (one over the temperature). reduction: "mean" (over the
     queries not ignored; NaN if there are none), "sum" or "none". Queries and
-    rows must be finite even where ignored or left out."""
+    rows must be finite even where ignored or left out. With float16 the
+    gradients of one call's losses should lie within a few orders of magnitude:
+    what is below 2^-39 of the largest is lost."""
     _not_traced("softmax_cross_entropy")
     _check(queries, "queries", 2, (torch.float16, torch.bfloat16))
     _check(rows, "rows", 2, (queries.dtype,))
