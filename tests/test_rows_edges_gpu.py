@@ -105,7 +105,8 @@ def test_softmax_rows_with_many_queries(px, dtype, mine, others, v):
 
 
 @pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("t,v,d", [(33, 64, 24), (40, 300, 64), (257, 700, 200), (520, 900, 390), (1000, 300, 32), (300, 230_009, 16)])
+@pytest.mark.parametrize("t,v,d", [(33, 64, 24), (40, 300, 64), (257, 700, 200), (520, 900, 390), (1000, 300, 32), (300, 230_009, 16),
+                                   (150_000, 1100, 16)])
 def test_softmax_large_entries_anywhere(px, dtype, t, v, d):
     # Queries from certain of their target to far from it, in no order, so that
     # entries of all sizes, and blocks with and without large ones, meet in all
